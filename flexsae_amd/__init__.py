@@ -13,6 +13,7 @@ from .ops import (check_index_flag, hier_stage_bytes, hierarchical_sae_sgd_step,
                   set_hier_min_slice_cols, set_hier_scratch_bytes, set_hier_stage_bytes, set_hot_latents,
                   set_index_checking, set_topk_residual_bf16, shared_pair_list, triton_hierarchical_sae_loss,
                   triton_topk_sae_loss)
+from .optim import AdamW, adamw8_moments, adamw8_state, adamw8_step, adamw_counter, adamw_step, grad_norm
 from .reference import hierarchical_sae_loss, topk_sae_loss
 
 # spelled-out aliases for new code
@@ -45,4 +46,11 @@ __all__ = [
     "set_dense_latents",
     "set_topk_residual_bf16",
     "shared_pair_list",
+    "grad_norm",
+    "adamw_step",
+    "adamw8_step",
+    "adamw8_moments",
+    "adamw8_state",
+    "adamw_counter",
+    "AdamW",
 ]

@@ -42,6 +42,7 @@ BWD_HOT_BLOCKS_32 = 8192
 BWD_RAGGED_ROWS = 16384
 TOPK_BWD_FP32_RESIDUAL = 256
 TOPK_BWD_AS_LARGE = 32768
+ADAMW_UNIT_ROWS = 1
 
 
 class Shape(ctypes.Structure):
@@ -52,6 +53,36 @@ class Shape(ctypes.Structure):
         ("weight_dtype", ctypes.c_int32), ("vals_dtype", ctypes.c_int32),
         ("bias_dtype", ctypes.c_int32), ("target_dtype", ctypes.c_int32),
     ]
+
+
+class Grad(ctypes.Structure):
+    """Mirror of ``flexsae_grad``."""
+
+    _fields_ = [("grad", ctypes.c_void_p), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """Mirror of ``flexsae_adamw_tensor``."""
+
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("master", ctypes.c_void_p),
+                ("state0", ctypes.c_void_p), ("state1", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("lr", ctypes.c_float), ("weight_decay", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
+class AdamwConfig(ctypes.Structure):
+    """Mirror of ``flexsae_adamw_config``."""
+
+    _fields_ = [("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("grad_scale", ctypes.c_float), ("max_norm", ctypes.c_float), ("grad_norm", ctypes.c_void_p),
+                ("lr", ctypes.c_void_p), ("counter", ctypes.c_void_p), ("state_bits", ctypes.c_int32),
+                ("flags", ctypes.c_int32)]
+
+
+class Adamw8State(ctypes.Structure):
+    """Mirror of ``flexsae_adamw8_state``."""
+
+    _fields_ = [("codes", ctypes.c_void_p), ("absmax", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+                ("exp_avg_sq", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
 
 
 class FlexSAELibraryError(RuntimeError):
@@ -101,6 +132,10 @@ SIGNATURES = {
     "flexsae_hier_hot_stats": (_int, [_shape_p, _p, _p, _p]),
     "flexsae_hier_pair_stats": (_int, [_shape_p, _p, _p, _p]),
     "flexsae_hier_fwd_bwd_workspace_bytes_flags": (_sz, [_shape_p, _i64, _int]),
+    "flexsae_grad_norm_workspace_bytes": (_sz, [_i64]),
+    "flexsae_grad_norm": (_int, [ctypes.POINTER(Grad), _i64, _p, _p, _sz, _p]),
+    "flexsae_adamw_step": (_int, [ctypes.POINTER(AdamwTensor), _i64, ctypes.POINTER(AdamwConfig), _p]),
+    "flexsae_adamw8_moments": (_int, [ctypes.POINTER(Adamw8State), _i64, _int, _p]),
 }
 
 _lib = None

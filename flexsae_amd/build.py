@@ -11,6 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libflexsae_amd.so")
 EAGER_PATH = os.path.join(HERE, "_eager.so")
+HIP_SOURCES = ["flexsae_amd.hip", "optimizer.hip"]  # the losses; the optimiser
 
 # gfx950 only: some kernels use more LDS per workgroup than the 64 KiB of earlier gfx9 parts
 # (csr_sort_long_kernel 65 600 bytes, the hot-latent variant of the training-step kernel more), the
@@ -78,7 +79,7 @@ def build(verbose: bool = False, extra_flags=()) -> str:
     build_eager(verbose, extra_flags)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, f'-DFLEXSAE_BUILD_ID="{source_id(extra_flags)}"', "-o", LIB_PATH,
-           os.path.join(CSRC, "flexsae_amd.hip")]
+           *(os.path.join(CSRC, f) for f in HIP_SOURCES)]
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)

@@ -1,5 +1,5 @@
-// Ordinary eager calls without Python between the launches: the checks of a call, its allocations, the C-ABI entry points and
-// the autograd nodes of the two losses, as an extension module of CPython over torch's C++ interface.
+// Ordinary eager calls without Python between the launches: the checks of a call, its allocations, the C-ABI entry points,
+// the autograd nodes of the two losses and the optimiser's calls, as an extension module of CPython over torch's C++ interface.
 //
 // A small step is host work: with the same steps in Python (ctypes, torch.empty, an autograd.Function whose backward takes the
 // interpreter's lock on autograd's device thread) B=64, K=32, F=4096, D=256 fp32 takes 160 us (TopK) and 195 us
@@ -11,6 +11,7 @@
 #include <dlfcn.h>
 
 #include <atomic>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -37,7 +38,8 @@ using torch::autograd::variable_list;
 #define FLEXSAE_ENTRIES(X)                                                                                              \
   X(abi_version) X(fwd_workspace_bytes) X(topk_fwd_best_workspace_bytes) X(topk_fwd) X(hier_fwd)                        \
   X(topk_bwd_from_indices_workspace_bytes) X(topk_bwd_from_indices) X(hier_bwd_workspace_bytes) X(hier_bwd)             \
-  X(hier_fwd_bwd_workspace_bytes_flags) X(hier_step) X(finish_grads)
+  X(hier_fwd_bwd_workspace_bytes_flags) X(hier_step) X(finish_grads)                                                    \
+  X(grad_norm_workspace_bytes) X(grad_norm) X(adamw_step) X(adamw8_moments)
 struct Library {
 #define X(name) decltype(&flexsae_##name) name = nullptr;
   FLEXSAE_ENTRIES(X)
@@ -576,6 +578,201 @@ PyObject *py_hier_sgd(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the optimiser -------------------------------------------------------------------------
+// The tensors of a list or tuple, each one plain and of `device` (undefined: the first one's); false: not this module's business.
+bool take_tensors(PyObject *o, std::vector<Tensor> &out, c10::optional<c10::Device> &device) {
+  if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  PyObject **const items = PySequence_Fast_ITEMS(o);
+  out.reserve(static_cast<size_t>(n));
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!THPVariable_CheckExact(items[i])) return false;
+    const Tensor &t = THPVariable_Unpack(items[i]);
+    if (!plain_tensor(t) || (device && t.device() != *device)) return false;
+    if (!device) device = t.device();
+    out.push_back(t);
+  }
+  return true;
+}
+
+// A tensor that a call changes: its memory as it is.
+bool changeable(const Tensor &t) { return t.is_contiguous() && !t.is_inference(); }
+
+double real(PyObject *o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw_python();
+  return v;
+}
+
+// The i-th of a list or tuple of numbers, or the number itself.
+double real_at(PyObject *o, Py_ssize_t i) {
+  return PyList_CheckExact(o) || PyTuple_CheckExact(o) ? real(PySequence_Fast_GET_ITEM(o, i)) : real(o);
+}
+bool reals(PyObject *o, size_t n) {
+  return PyList_CheckExact(o) || PyTuple_CheckExact(o) ? PySequence_Fast_GET_SIZE(o) == static_cast<Py_ssize_t>(n)
+                                                        : PyFloat_Check(o) || PyLong_Check(o);
+}
+
+// One fp32 number of `device`; None: none.
+bool take_scalar(PyObject *o, const c10::Device &device, Tensor &out) {
+  if (o == Py_None) return true;
+  if (!THPVariable_Check(o)) return false;
+  out = THPVariable_Unpack(o);
+  return plain_tensor(out) && out.device() == device && out.scalar_type() == c10::ScalarType::Float && out.numel() == 1;
+}
+
+// grad_norm(grads) -> norm
+PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 1)) return nullptr;
+  std::vector<Tensor> grads;
+  c10::optional<c10::Device> device;
+  if (!plain_surroundings() || !take_tensors(args[0], grads, device) || grads.empty()) Py_RETURN_NONE;
+  for (const Tensor &g : grads)
+    if (dtype_of(g.scalar_type()) < 0) Py_RETURN_NONE;
+  Tensor norm;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::AutoGradMode no_grad(false);
+    const c10::DeviceGuard guard(*device);
+    std::vector<flexsae_grad> list;
+    list.reserve(grads.size());
+    for (Tensor &g : grads) {
+      if (!g.is_contiguous()) g = g.contiguous();
+      list.push_back({g.const_data_ptr(), g.numel(), dtype_of(g.scalar_type())});
+    }
+    const auto count = static_cast<int64_t>(list.size());
+    const size_t bytes = lib.grad_norm_workspace_bytes(count);
+    const Tensor workspace = make_workspace(grads[0], bytes);
+    norm = make(grads[0], {}, c10::ScalarType::Float);
+    check(lib.grad_norm(list.data(), count, f32(norm), workspace.data_ptr(), bytes, stream_of(norm)), "flexsae_grad_norm");
+  }
+  return THPVariable_Wrap(norm);
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw(bits, params, grads, state0s, state1s, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm,
+// max_norm, unit_rows) -> True
+PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 16)) return nullptr;
+  const bool eight = number(args[0]) == 8, unit = number(args[15]) != 0;
+  std::vector<Tensor> params, grads, s0, s1, masters;
+  c10::optional<c10::Device> device;
+  if (!plain_surroundings() || !take_tensors(args[1], params, device) || params.empty() ||
+      !take_tensors(args[2], grads, device) || !take_tensors(args[3], s0, device) || !take_tensors(args[4], s1, device) ||
+      (args[5] != Py_None && !take_tensors(args[5], masters, device)))
+    Py_RETURN_NONE;
+  const size_t count = params.size();
+  if (grads.size() != count || s0.size() != count || s1.size() != count || (args[5] != Py_None && masters.size() != count) ||
+      !THPVariable_Check(args[6]))
+    Py_RETURN_NONE;
+  const Tensor counter = THPVariable_Unpack(args[6]);
+  if (!plain_tensor(counter) || counter.device() != *device || counter.scalar_type() != c10::ScalarType::Long ||
+      counter.numel() != 2 || !changeable(counter))
+    Py_RETURN_NONE;
+  const bool device_lr = THPVariable_Check(args[7]);
+  Tensor lr, norm;
+  if ((device_lr ? !take_scalar(args[7], *device, lr) : !reals(args[7], count)) || !reals(args[8], count) ||
+      !take_scalar(args[13], *device, norm))
+    Py_RETURN_NONE;
+  std::vector<flexsae_adamw_tensor> list(count);
+  for (size_t i = 0; i < count; ++i) {
+    const Tensor &p = params[i];
+    const int dtype = dtype_of(p.scalar_type());
+    if (dtype < 0 || grads[i].scalar_type() != p.scalar_type() || grads[i].sizes() != p.sizes() || !changeable(p) ||
+        !changeable(s0[i]) || !changeable(s1[i]) || (unit && p.dim() < 2))
+      Py_RETURN_NONE;
+    const int64_t cols = unit ? p.size(-1) : p.numel(), rows = unit ? (cols ? p.numel() / cols : 0) : 1;
+    if (eight) {
+      const at::IntArrayRef sizes = s0[i].sizes();
+      if (s0[i].scalar_type() != c10::ScalarType::Byte || s1[i].scalar_type() != c10::ScalarType::Float ||
+          s0[i].dim() != p.dim() + 1 || sizes.back() != 2 || sizes.slice(0, sizes.size() - 1) != p.sizes() ||
+          s1[i].dim() != 3 || s1[i].size(0) != rows || s1[i].size(1) != (cols + 255) / 256 || s1[i].size(2) != 2 ||
+          reinterpret_cast<uintptr_t>(s1[i].const_data_ptr()) % 8 || reinterpret_cast<uintptr_t>(s0[i].const_data_ptr()) % 2)
+        Py_RETURN_NONE;
+    } else if (s0[i].scalar_type() != c10::ScalarType::Float || s1[i].scalar_type() != c10::ScalarType::Float ||
+               s0[i].sizes() != p.sizes() || s1[i].sizes() != p.sizes()) {
+      Py_RETURN_NONE;
+    }
+    void *master = nullptr;
+    if (!masters.empty() && dtype != FLEXSAE_F32) {
+      if (masters[i].scalar_type() != c10::ScalarType::Float || masters[i].sizes() != p.sizes() || !changeable(masters[i]))
+        Py_RETURN_NONE;
+      master = masters[i].data_ptr();
+    }
+    if (!grads[i].is_contiguous()) grads[i] = grads[i].contiguous();
+    const auto at = static_cast<Py_ssize_t>(i);
+    list[i] = {p.data_ptr(), grads[i].const_data_ptr(), master, s0[i].data_ptr(), s1[i].data_ptr(), rows, cols,
+               device_lr ? 1.f : static_cast<float>(real_at(args[7], at)), static_cast<float>(real_at(args[8], at)), dtype};
+  }
+  const flexsae_adamw_config config = {real(args[9]),
+                                       real(args[10]),
+                                       real(args[11]),
+                                       static_cast<float>(real(args[12])),
+                                       static_cast<float>(real(args[14])),
+                                       norm.defined() ? f32(norm) : nullptr,
+                                       lr.defined() ? f32(lr) : nullptr,
+                                       counter.data_ptr<int64_t>(),
+                                       eight ? 8 : 32,
+                                       unit ? FLEXSAE_ADAMW_UNIT_ROWS : 0};
+  int status = FLEXSAE_OK;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(*device);
+    status = lib.adamw_step(list.data(), static_cast<int64_t>(count), &config, stream_of(counter));
+    if (status == FLEXSAE_OK || status == FLEXSAE_ERR_LAUNCH)  // (else nothing was launched)
+      for (const auto *changed : {&params, &s0, &s1, &masters})
+        for (const Tensor &t : *changed) torch::autograd::impl::bump_version(t);
+    if (status != FLEXSAE_ERR_INVALID_ARGUMENT) check(status, "flexsae_adamw_step");
+    torch::autograd::impl::bump_version(counter);
+  }
+  if (status != FLEXSAE_OK) Py_RETURN_NONE;  // optim.py says what is wrong
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw8_moments(codes, absmax, dtype) -> (exp_avgs, exp_avg_sqs)
+PyObject *py_adamw8_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 3)) return nullptr;
+  const int64_t dtype = number(args[2]);
+  std::vector<Tensor> codes, absmax, m, v;
+  c10::optional<c10::Device> device;
+  if (!plain_surroundings() || !take_tensors(args[0], codes, device) || codes.empty() || !take_tensors(args[1], absmax, device) ||
+      absmax.size() != codes.size() || dtype < 0 || dtype > 2)
+    Py_RETURN_NONE;
+  std::vector<flexsae_adamw8_state> list(codes.size());
+  const c10::ScalarType type = dtype == FLEXSAE_F32    ? c10::ScalarType::Float
+                               : dtype == FLEXSAE_BF16 ? c10::ScalarType::BFloat16
+                                                       : c10::ScalarType::Half;
+  for (size_t i = 0; i < codes.size(); ++i) {
+    const Tensor &c = codes[i], &a = absmax[i];
+    if (c.scalar_type() != c10::ScalarType::Byte || a.scalar_type() != c10::ScalarType::Float || c.dim() < 1 || c.size(-1) != 2 ||
+        a.dim() != 3 || a.size(2) != 2 || !c.is_contiguous() || !a.is_contiguous() ||
+        reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 2 || reinterpret_cast<uintptr_t>(a.const_data_ptr()) % 8)
+      Py_RETURN_NONE;
+    const int64_t rows = a.size(0), cols = rows ? c.numel() / 2 / rows : 0;
+    if (rows * cols != c.numel() / 2 || (rows && a.size(1) != (cols + 255) / 256)) Py_RETURN_NONE;
+    m.push_back(make(c, c.sizes().slice(0, c.dim() - 1), type));
+    v.push_back(make(c, c.sizes().slice(0, c.dim() - 1), type));
+    list[i] = {c.const_data_ptr(), a.const_data_ptr<float>(), m[i].data_ptr(), v[i].data_ptr(), rows, cols};
+  }
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(*device);
+    check(lib.adamw8_moments(list.data(), static_cast<int64_t>(list.size()), static_cast<int>(dtype), stream_of(codes[0])),
+          "flexsae_adamw8_moments");
+  }
+  auto list_of = [](const std::vector<Tensor> &tensors) {
+    auto l = pybind11::reinterpret_steal<pybind11::object>(PyList_New(static_cast<Py_ssize_t>(tensors.size())));
+    for (size_t i = 0; i < tensors.size(); ++i) PyList_SET_ITEM(l.ptr(), static_cast<Py_ssize_t>(i), THPVariable_Wrap(tensors[i]));
+    return l;
+  };
+  return Py_BuildValue("NN", list_of(m).release().ptr(), list_of(v).release().ptr());
+  END_HANDLE_TH_ERRORS
+}
+
 // set_flag(device, flag)
 PyObject *py_set_flag(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -621,7 +818,8 @@ PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
 #define FLEXSAE_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FLEXSAE_METHOD(init),       FLEXSAE_METHOD(set_flag),    FLEXSAE_METHOD(settings),
                          FLEXSAE_METHOD(topk_loss),  FLEXSAE_METHOD(hier_loss),   FLEXSAE_METHOD(hier_sliced),
-                         FLEXSAE_METHOD(hier_late),  FLEXSAE_METHOD(hier_sgd),    {nullptr, nullptr, 0, nullptr}};
+                         FLEXSAE_METHOD(hier_late),  FLEXSAE_METHOD(hier_sgd),    FLEXSAE_METHOD(grad_norm),
+                         FLEXSAE_METHOD(adamw),      FLEXSAE_METHOD(adamw8_moments), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_eager", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

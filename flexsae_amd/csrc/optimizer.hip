@@ -1,0 +1,232 @@
+// C-ABI entry points of the optimiser (include/flexsae_amd.h): argument validation, tables of tensors and launches.  No
+// allocation, no synchronisation, no global state.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include "adamw_kernels.hpp"
+
+using namespace flexsae;
+
+namespace {
+
+bool valid_dtype(int d) { return d == FLEXSAE_F32 || d == FLEXSAE_BF16 || d == FLEXSAE_F16; }
+size_t dtype_size(int d) { return d == FLEXSAE_F32 ? 4 : 2; }
+bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
+int launch_status() { return hipGetLastError() == hipSuccess ? FLEXSAE_OK : FLEXSAE_ERR_LAUNCH; }
+
+constexpr int64_t kMostElements = int64_t{1} << 40;  // of a tensor: tiles are counted in 32 bits
+
+// Blocks of a launch: enough to fill the chip several times over; each then takes one tile after another, so that what a block
+// does once (the step's factors, counting the step) is paid a bounded number of times.
+constexpr int64_t kStepBlocks = 2048;
+constexpr int64_t kNormBlocks = 1024;
+
+unsigned blocks_for(int64_t tiles, int64_t most) { return static_cast<unsigned>(tiles < 1 ? 1 : tiles > most ? most : tiles); }
+
+int check_tensor(const flexsae_adamw_tensor &t, const flexsae_adamw_config &c) {
+  if (t.rows < 0 || t.cols < 0 || !valid_dtype(t.dtype)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (!(t.lr >= 0.f) || !(t.weight_decay >= 0.f)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (t.rows == 0 || t.cols == 0) return FLEXSAE_OK;
+  if (t.rows > kMostElements / t.cols) return FLEXSAE_ERR_UNSUPPORTED;
+  if (!t.param || !t.grad || !t.state0 || !t.state1) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (t.master && t.dtype == FLEXSAE_F32) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  const size_t es = dtype_size(t.dtype);
+  if (!aligned(t.param, es) || !aligned(t.grad, es) || !aligned(t.master, 4)) return FLEXSAE_ERR_ALIGNMENT;
+  if (c.state_bits == 32 ? !aligned(t.state0, 4) || !aligned(t.state1, 4) : !aligned(t.state0, 2) || !aligned(t.state1, 8))
+    return FLEXSAE_ERR_ALIGNMENT;
+  return FLEXSAE_OK;
+}
+
+int check_config(const flexsae_adamw_config *c) {
+  if (!c || !c->counter) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (c->state_bits != 32 && c->state_bits != 8) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (!(c->beta1 >= 0. && c->beta1 < 1.) || !(c->beta2 >= 0. && c->beta2 < 1.) || !(c->eps >= 0.)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (!(c->grad_scale > 0.f) || !isfinite(c->grad_scale) || !isfinite(1.f / c->grad_scale)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (!(c->max_norm >= 0.f) || (c->max_norm > 0.f && !c->grad_norm)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (!aligned(c->counter, 8) || !aligned(c->grad_norm, 4) || !aligned(c->lr, 4)) return FLEXSAE_ERR_ALIGNMENT;
+  return FLEXSAE_OK;
+}
+
+AdamwTable table_of(const flexsae_adamw_config &c) {
+  AdamwTable a{};
+  a.beta1 = static_cast<float>(c.beta1);
+  a.one_minus_beta1 = static_cast<float>(1. - c.beta1);
+  a.beta2 = static_cast<float>(c.beta2);
+  a.one_minus_beta2 = static_cast<float>(1. - c.beta2);
+  a.eps = static_cast<float>(c.eps);
+  a.inv_scale = 1.f / c.grad_scale;
+  a.max_norm = c.max_norm;
+  a.log_beta1 = log(c.beta1);  // (of zero: minus infinity, whose exponential is zero)
+  a.log_beta2 = log(c.beta2);
+  a.grad_norm = c.grad_norm;
+  a.lr = c.lr;
+  a.counter = c.counter;
+  return a;
+}
+
+using Kernel = void (*)(const AdamwTable);
+
+// How the rows of a tensor are shared out: the fewest wavefronts that hold a row in registers.
+struct RowPlan {
+  Kernel kernel;
+  int threads, rows;  // of a block
+};
+
+template <typename T, bool MASTER, bool EIGHT>
+RowPlan row_plan(int64_t cols) {
+  constexpr int64_t kSegment = kWave * kAdamwLane;
+  if (cols <= kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 1>, 256, 4};
+  if (cols <= 2 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 2>, 256, 4};
+  if (cols <= 3 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 3>, 256, 4};
+  if (cols <= 5 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 5>, 256, 4};
+  if (cols <= 8 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 4, 2>, 256, 1};
+  if (cols <= 16 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 4, 4>, 256, 1};
+  if (cols <= 32 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 16, 2>, 1024, 1};
+  return {adamw_rows_kernel<T, MASTER, EIGHT, 16, 0>, 1024, 1};
+}
+
+template <bool EIGHT>
+RowPlan row_plan(const flexsae_adamw_tensor &t) {
+  if (t.dtype == FLEXSAE_F32) return row_plan<float, false, EIGHT>(t.cols);
+  if (t.dtype == FLEXSAE_BF16) return t.master ? row_plan<bf16_t, true, EIGHT>(t.cols) : row_plan<bf16_t, false, EIGHT>(t.cols);
+  return t.master ? row_plan<f16_t, true, EIGHT>(t.cols) : row_plan<f16_t, false, EIGHT>(t.cols);
+}
+
+// Adds a tensor of `tiles` tiles; false: the table is full.
+bool add(AdamwTable &a, const flexsae_adamw_tensor &t, int64_t tiles, bool flat) {
+  if (a.count == kAdamwTensors || a.first[a.count] + tiles > (int64_t{1} << 31)) return false;
+  a.tensor[a.count] = {t.param, t.grad, t.state0, t.state1, static_cast<float *>(t.master), flat ? 1 : t.rows,
+                       flat ? t.rows * t.cols : t.cols, t.lr, t.weight_decay, t.dtype};
+  a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(tiles);
+  ++a.count;
+  return true;
+}
+
+int launch(Kernel kernel, int threads, AdamwTable &a, bool last, hipStream_t stream) {
+  a.last = last;
+  kernel<<<blocks_for(a.first[a.count], kStepBlocks), threads, 0, stream>>>(a);
+  a.count = 0;
+  return launch_status();
+}
+
+}  // namespace
+
+extern "C" {
+
+int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const flexsae_adamw_config *config, void *stream) {
+  if (const int rc = check_config(config)) return rc;
+  if (count < 0 || (count > 0 && !tensors)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (config->flags & ~FLEXSAE_ADAMW_UNIT_ROWS) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  for (int64_t i = 0; i < count; ++i)
+    if (const int rc = check_tensor(tensors[i], *config)) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool eight = config->state_bits == 8, unit = config->flags & FLEXSAE_ADAMW_UNIT_ROWS;
+  const Kernel flat = eight ? adamw_kernel<true> : adamw_kernel<false>;
+  AdamwTable a = table_of(*config);
+  // Tensors that the same kernel takes go into one launch; a table that is full, or another kernel's turn, ends a launch.
+  Kernel kernel = flat;
+  int threads = kAdamwThreads;
+  for (int64_t i = 0; i < count; ++i) {
+    const flexsae_adamw_tensor &t = tensors[i];
+    if (t.rows == 0 || t.cols == 0) continue;
+    const RowPlan plan = !unit ? RowPlan{flat, kAdamwThreads, 1} : eight ? row_plan<true>(t) : row_plan<false>(t);
+    const int64_t tiles = unit ? ceil_div(t.rows, plan.rows) : ceil_div(t.rows * t.cols, kAdamwTile);
+    if (tiles > (int64_t{1} << 31)) return FLEXSAE_ERR_UNSUPPORTED;
+    if (a.count > 0 && plan.kernel != kernel)
+      if (const int rc = launch(kernel, threads, a, false, s)) return rc;
+    kernel = plan.kernel;
+    threads = plan.threads;
+    if (add(a, t, tiles, !unit)) continue;
+    if (const int rc = launch(kernel, threads, a, false, s)) return rc;
+    (void)add(a, t, tiles, !unit);
+  }
+  return launch(kernel, threads, a, true, s);
+}
+
+size_t flexsae_grad_norm_workspace_bytes(int64_t count) {
+  if (count < 0) return 0;
+  return static_cast<size_t>(ceil_div(count > 0 ? count : 1, kNormTensors)) * kNormBlocks * sizeof(double);
+}
+
+int flexsae_grad_norm(const flexsae_grad *grads, int64_t count, float *norm, void *workspace, size_t workspace_bytes, void *stream) {
+  if (count < 0 || (count > 0 && !grads) || !norm) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  if (!aligned(norm, 4)) return FLEXSAE_ERR_ALIGNMENT;
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < flexsae_grad_norm_workspace_bytes(count)) return FLEXSAE_ERR_WORKSPACE;
+  int64_t all = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (grads[i].n < 0 || !valid_dtype(grads[i].dtype)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+    if (grads[i].n > kMostElements - all) return FLEXSAE_ERR_UNSUPPORTED;
+    all += grads[i].n;
+    if (grads[i].n > 0 && !grads[i].grad) return FLEXSAE_ERR_INVALID_ARGUMENT;
+    if (!aligned(grads[i].grad, dtype_size(grads[i].dtype))) return FLEXSAE_ERR_ALIGNMENT;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  double *const partial = static_cast<double *>(workspace);
+  int64_t sums = 0;
+  NormTable a;
+  a.count = 0;
+  a.first[0] = 0;
+  auto launch_norm = [&]() {
+    a.partial = partial + sums;
+    const unsigned blocks = blocks_for(a.first[a.count], kNormBlocks);
+    norm_partial_kernel<<<blocks, kAdamwThreads, 0, s>>>(a);
+    sums += blocks;
+    a.count = 0;
+    return launch_status();
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    if (grads[i].n == 0) continue;
+    const int64_t tiles = ceil_div(grads[i].n, kAdamwTile);
+    if (a.count == kNormTensors)
+      if (const int rc = launch_norm()) return rc;
+    a.tensor[a.count] = {grads[i].grad, grads[i].n, grads[i].dtype};
+    a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(tiles);
+    ++a.count;
+  }
+  if (a.count > 0)
+    if (const int rc = launch_norm()) return rc;
+  norm_finish_kernel<<<1, kAdamwThreads, 0, s>>>(partial, sums, norm);
+  return launch_status();
+}
+
+int flexsae_adamw8_moments(const flexsae_adamw8_state *states, int64_t count, int dtype, void *stream) {
+  if (count < 0 || (count > 0 && !states) || !valid_dtype(dtype)) return FLEXSAE_ERR_INVALID_ARGUMENT;
+  for (int64_t i = 0; i < count; ++i) {
+    const flexsae_adamw8_state &t = states[i];
+    if (t.rows < 0 || t.cols < 0) return FLEXSAE_ERR_INVALID_ARGUMENT;
+    if (t.rows == 0 || t.cols == 0) continue;
+    if (t.rows > kMostElements / t.cols) return FLEXSAE_ERR_UNSUPPORTED;
+    if (!t.codes || !t.absmax || !t.exp_avg || !t.exp_avg_sq) return FLEXSAE_ERR_INVALID_ARGUMENT;
+    if (!aligned(t.codes, 2) || !aligned(t.absmax, 8) || !aligned(t.exp_avg, dtype_size(dtype)) || !aligned(t.exp_avg_sq, dtype_size(dtype)))
+      return FLEXSAE_ERR_ALIGNMENT;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const auto kernel = dtype == FLEXSAE_F32 ? adamw8_moments_kernel<float> : dtype == FLEXSAE_BF16 ? adamw8_moments_kernel<bf16_t>
+                                                                                                   : adamw8_moments_kernel<f16_t>;
+  MomentsTable a;
+  a.count = 0;
+  a.first[0] = 0;
+  auto launch_moments = [&]() {
+    if (a.count == 0) return static_cast<int>(FLEXSAE_OK);
+    kernel<<<blocks_for(a.first[a.count], int64_t{1} << 20), kAdamwThreads, 0, s>>>(a);
+    a.count = 0;
+    return launch_status();
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    const flexsae_adamw8_state &t = states[i];
+    if (t.rows == 0 || t.cols == 0) continue;
+    const bool flat = t.cols % kAdamwQuant == 0;  // blocks do not ask where rows begin
+    const int64_t rows = flat ? 1 : t.rows, cols = flat ? t.rows * t.cols : t.cols;
+    const int64_t tiles = rows * ceil_div(cols, kAdamwTile);
+    if (tiles > (int64_t{1} << 31)) return FLEXSAE_ERR_UNSUPPORTED;
+    if (a.count == kMomentsTensors || a.first[a.count] + tiles > (int64_t{1} << 31))
+      if (const int rc = launch_moments()) return rc;
+    a.tensor[a.count] = {t.codes, t.absmax, t.exp_avg, t.exp_avg_sq, rows, cols};
+    a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(tiles);
+    ++a.count;
+  }
+  return launch_moments();
+}
+
+}  // extern "C"

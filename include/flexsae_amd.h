@@ -476,6 +476,77 @@ int flexsae_finish_grads(void *dW, int dW_dtype, const void *dW_unit, int dW_uni
                          int dvals_dtype, const float *dvals_unit, int64_t n_dvals, void *dbias, int dbias_dtype,
                          const float *dbias_unit, int64_t n_dbias, const float *scale, void *stream);
 
+/* ---- the optimiser -----------------------------------------------------------------------------------------------
+ * No counterpart in the reference (its loop takes an optimizer of torch, example.py:76-77).  Any number of tensors in a
+ * call; the arrays that describe them are host memory and may be reused when the call returns.
+ */
+
+typedef struct {
+  const void *grad; /* n elements of `dtype`, aligned to the element */
+  int64_t n;
+  int32_t dtype;
+} flexsae_grad;
+
+/* Bytes of workspace of flexsae_grad_norm for `count` gradients. */
+size_t flexsae_grad_norm_workspace_bytes(int64_t count);
+
+/* norm[0] = sqrt(sum of the squares of all elements of all gradients), fp32 (device).  Squares are summed in 64 bits, in an
+ * order that the sizes fix: the result is the same bits on every run.  Infinities and NaN reach the norm. */
+int flexsae_grad_norm(const flexsae_grad *grads, int64_t count, float *norm, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+/* One parameter of an AdamW step: rows * cols contiguous elements, aligned to the element.  A tensor without elements is
+ * left out. */
+typedef struct {
+  void *param;      /* in/out, `dtype` */
+  const void *grad; /* `dtype` */
+  void *master;     /* in/out, fp32, or NULL: the weight that a 16-bit param is the rounded copy of (param is then written only) */
+  void *state0;     /* in/out: exp_avg, fp32[rows*cols]; 8 bits: codes, uint8[rows*cols][2] (aligned to 2) */
+  void *state1;     /* in/out: exp_avg_sq, fp32[rows*cols]; 8 bits: maxima, fp32[blocks][2] (aligned to 8); blocks: rows *      */
+                    /* ceil(cols/256) with FLEXSAE_ADAMW_UNIT_ROWS, else ceil(rows*cols/256).  A new state is all zeros.        */
+  int64_t rows, cols;
+  float lr, weight_decay;
+  int32_t dtype; /* flexsae_dtype */
+} flexsae_adamw_tensor;
+
+enum {
+  FLEXSAE_ADAMW_UNIT_ROWS = 1 /* rows are held at length one: the part of the gradient along the row is left out, and the  */
+                              /* moved row is divided by its length (a row of zeros stays one)                             */
+};
+
+typedef struct {
+  double beta1, beta2, eps;
+  float grad_scale;       /* gradients are divided by it (a loss scale; 1: as they are) */
+  float max_norm;         /* 0: no clipping; else gradients are multiplied by min(1, max_norm / (norm / grad_scale + 1e-6)) */
+  const float *grad_norm; /* device, of the gradients as they are, or NULL.  Not finite: the call changes nothing */
+  const float *lr;        /* device, or NULL: a factor of every tensor's lr (schedules of captured graphs) */
+  int64_t *counter;       /* device, [2]: steps taken, which the call counts up; and a zero that it works with */
+  int32_t state_bits;     /* 32 or 8 */
+  int32_t flags;
+} flexsae_adamw_config;
+
+/*
+ * AdamW step of all tensors, t = counter[0] + 1:
+ *   m = b1 m + (1-b1) g, v = b2 v + (1-b2) g^2, w = (1 - lr wd) w - lr (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
+ * 8-bit states, blocks of 256: codes[0] = c stands for sign(c-128) ((c-128)/127)^2 max|m|, codes[1] = c for (c/255)^4 max v
+ * (at least 1 for a v above zero); the update uses m and v before they are rounded to their codes.  A maximum below the
+ * smallest normal number is kept as zero; infinities and NaN make their block NaN.
+ * Calls that share a counter have to be ordered (one stream).  After a call that returns FLEXSAE_ERR_LAUNCH some of the
+ * tensors may have been stepped.
+ */
+int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const flexsae_adamw_config *config, void *stream);
+
+/* 8-bit states of rows * cols elements, rows as in state1 above (1 where the blocks are those of the whole tensor). */
+typedef struct {
+  const void *codes;
+  const float *absmax;
+  void *exp_avg, *exp_avg_sq; /* out, rows * cols elements each */
+  int64_t rows, cols;
+} flexsae_adamw8_state;
+
+/* The values that 8-bit states stand for, in `dtype`. */
+int flexsae_adamw8_moments(const flexsae_adamw8_state *states, int64_t count, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
