@@ -20,11 +20,12 @@
 namespace flexsae {
 
 constexpr int kAdamwThreads = 256;
-constexpr int kAdamwLane = 8;                              // consecutive elements of a lane
-constexpr int kAdamwTile = kAdamwThreads * kAdamwLane;     // of a block at a time
+constexpr int kAdamwTile = 2048;                           // elements of a block at a time
 constexpr int kAdamwQuant = 256;                           // elements that share the maxima of 8-bit states
 constexpr int kAdamwTensors = 48;                          // of one launch: the table travels in the kernel's arguments (4 KiB)
 constexpr int kNormTensors = 128;
+constexpr int kNormTile = 8192;
+constexpr int kNormSums = 4;  // of a thread
 
 struct AdamwTensor {
   void *param;
@@ -40,12 +41,17 @@ struct AdamwTable {
   AdamwTensor tensor[kAdamwTensors];
   uint32_t first[kAdamwTensors + 1];  // tile (unit rows: group of rows) at which each tensor begins; the number of them
   int32_t count;
+  uint32_t per_block;  // consecutive tiles of a block
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, inv_scale, max_norm;
-  int32_t last;  // the call's last launch: counts the step
+  int32_t counting;  // who counts the step (kCounted*)
   double log_beta1, log_beta2;
   const float *grad_norm, *lr;  // device (NULL: none)
-  int64_t *counter;             // device: steps taken; blocks of this launch that have ended
+  int64_t *counter;             // device: steps taken; and a word to work with
 };
+// Every block needs the number of the step, so nobody may count it before all have read it.  A launch of few blocks has its last
+// one do it, known by a ticket that each draws at its end; tickets come at 160 a microsecond, which a launch of many blocks would
+// wait for (148 000 of them: 1.8 ms instead of 0.7), so there a kernel of one thread before the first launch counts.
+enum { kNotCountedYet = 0, kCountedByTicket = 1, kCountedBefore = 2 };
 static_assert(sizeof(AdamwTable) <= 4096, "kernel arguments");
 
 struct AdamwCoefs {
@@ -53,9 +59,20 @@ struct AdamwCoefs {
   bool go;
 };
 
+// 1 - b^t = -(e^x - 1) for x = t log(b) <= 0, without cancellation: the series to x^9 where x is small (off by less than
+// 2^-30 of it), one exponential elsewhere.
+__device__ __forceinline__ float one_minus_power(double t, double log_b) {
+  const float x = static_cast<float>(t * log_b);
+  if (x < -0.5f) return 1.f - __expf(x);
+  float s = 1.f;
+#pragma unroll
+  for (int k = 9; k > 1; --k) s = fmaf(s, x * (1.f / static_cast<float>(k)), 1.f);
+  return -x * s;
+}
+
 __device__ __forceinline__ AdamwCoefs adamw_coefs(const AdamwTable &a) {
+#pragma clang fp contract(off)
   AdamwCoefs c;
-  const double t = static_cast<double>(a.counter[0] + 1);
   c.b1 = a.beta1;
   c.omb1 = a.one_minus_beta1;
   c.b2 = a.beta2;
@@ -68,17 +85,16 @@ __device__ __forceinline__ AdamwCoefs adamw_coefs(const AdamwTable &a) {
     c.go = __builtin_isfinite(norm);
     if (a.max_norm > 0.f) c.grad *= fminf(1.f, a.max_norm / (norm * a.inv_scale + 1e-6f));
   }
-  // 1 - b^t without cancellation
-  c.inv_bc1 = -1.f / expm1f(static_cast<float>(t * a.log_beta1));
-  c.inv_sqrt_bc2 = 1.f / sqrtf(-expm1f(static_cast<float>(t * a.log_beta2)));
+  const double t = static_cast<double>(a.counter[0] + (a.counting == kCountedBefore ? 0 : 1));
   c.lr = a.lr ? *a.lr : 1.f;
-  c.inv_bc1 *= c.lr;
+  c.inv_bc1 = c.lr / one_minus_power(t, a.log_beta1);
+  c.inv_sqrt_bc2 = 1.f / sqrtf(one_minus_power(t, a.log_beta2));
   return c;
 }
 
-// The last block of the call's last launch counts the step: by then every block has read the number of steps.
+// The end of a block.
 __device__ __forceinline__ void adamw_count(const AdamwTable &a) {
-  if (!a.last) return;
+  if (a.counting != kCountedByTicket) return;
   __syncthreads();
   if (threadIdx.x == 0) {
     unsigned long long *ended = reinterpret_cast<unsigned long long *>(a.counter + 1);
@@ -87,6 +103,10 @@ __device__ __forceinline__ void adamw_count(const AdamwTable &a) {
       a.counter[0] += 1;
     }
   }
+}
+
+__global__ void adamw_count_kernel(int64_t *counter, const float *grad_norm) {
+  if (!grad_norm || __builtin_isfinite(*grad_norm)) counter[0] += 1;
 }
 
 // The tensor of a tile: the largest i with first[i] <= tile (tensors without tiles are not in the table).
@@ -99,110 +119,158 @@ __device__ __forceinline__ int tensor_of(const Table &a, uint32_t tile) {
   return i;
 }
 
-// Sixteen bytes through memory that is aligned to ALIGN (2 or 4: to the elements; rows and views start anywhere).
-typedef uint32_t words_at4_t __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t words_at2_t __attribute__((ext_vector_type(4), aligned(2)));
-template <int ALIGN>
-__device__ __forceinline__ void load16(const void *p, uint32_t *w) {
-  vec_t<uint32_t, 4> x;
-  if constexpr (ALIGN == 4) x = __builtin_nontemporal_load(static_cast<const words_at4_t *>(p));
-  else x = __builtin_nontemporal_load(static_cast<const words_at2_t *>(p));
-#pragma unroll
-  for (int k = 0; k < 4; ++k) w[k] = x[k];
-}
-template <int ALIGN>
-__device__ __forceinline__ void store16(void *p, const uint32_t *w) {
-  const vec_t<uint32_t, 4> x = {w[0], w[1], w[2], w[3]};
-  if constexpr (ALIGN == 4) __builtin_nontemporal_store(x, static_cast<words_at4_t *>(p));
-  else __builtin_nontemporal_store(x, static_cast<words_at2_t *>(p));
-}
-
-// Eight elements as stored.
-template <typename T>
-struct Raw8 {
-  static constexpr int kWords = 2 * static_cast<int>(sizeof(typename Traits<T>::store_t));
+// N consecutive elements of a lane as stored.  Vector accesses ask for the elements' own alignment only (rows and views start
+// anywhere); they stream: every byte is used once in a call.
+template <typename T, int N>
+struct Raw {
+  static constexpr int kWords = N * static_cast<int>(sizeof(typename Traits<T>::store_t)) / 4;
   uint32_t w[kWords];
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const void *base, int64_t at, int left, Raw8<T> &r) {
-  using S = typename Traits<T>::store_t;
-  const S *p = static_cast<const S *>(base) + at;
-  if (left >= kAdamwLane) {
-#pragma unroll
-    for (int j = 0; j < Raw8<T>::kWords; j += 4) load16<sizeof(S)>(reinterpret_cast<const char *>(p) + 4 * j, r.w + j);
+typedef uint32_t words4_at4_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t words4_at2_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t words2_at4_t __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t words2_at2_t __attribute__((ext_vector_type(2), aligned(2)));
+
+// WORDS (2, 4 or 8) dwords through memory that is aligned to ALIGN (2 or 4) bytes
+template <int WORDS, int ALIGN>
+__device__ __forceinline__ void load_words(const void *p, uint32_t *w) {
+  if constexpr (WORDS == 2) {
+    vec_t<uint32_t, 2> x;
+    if constexpr (ALIGN == 4) x = __builtin_nontemporal_load(static_cast<const words2_at4_t *>(p));
+    else x = __builtin_nontemporal_load(static_cast<const words2_at2_t *>(p));
+    w[0] = x[0];
+    w[1] = x[1];
   } else {
-    S x[kAdamwLane];
 #pragma unroll
-    for (int j = 0; j < kAdamwLane; ++j) x[j] = j < left ? p[j] : S{};
+    for (int j = 0; j < WORDS; j += 4) {
+      const void *at = static_cast<const char *>(p) + 4 * j;
+      vec_t<uint32_t, 4> x;
+      if constexpr (ALIGN == 4) x = __builtin_nontemporal_load(static_cast<const words4_at4_t *>(at));
+      else x = __builtin_nontemporal_load(static_cast<const words4_at2_t *>(at));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[j + k] = x[k];
+    }
+  }
+}
+template <int WORDS, int ALIGN>
+__device__ __forceinline__ void store_words(void *p, const uint32_t *w) {
+  if constexpr (WORDS == 2) {
+    const vec_t<uint32_t, 2> x = {w[0], w[1]};
+    if constexpr (ALIGN == 4) __builtin_nontemporal_store(x, static_cast<words2_at4_t *>(p));
+    else __builtin_nontemporal_store(x, static_cast<words2_at2_t *>(p));
+  } else {
+#pragma unroll
+    for (int j = 0; j < WORDS; j += 4) {
+      void *at = static_cast<char *>(p) + 4 * j;
+      const vec_t<uint32_t, 4> x = {w[j], w[j + 1], w[j + 2], w[j + 3]};
+      if constexpr (ALIGN == 4) __builtin_nontemporal_store(x, static_cast<words4_at4_t *>(at));
+      else __builtin_nontemporal_store(x, static_cast<words4_at2_t *>(at));
+    }
+  }
+}
+
+// Where a lane's elements are: `start` and `block`, the same for the wavefront where it works on one row, stay in scalar registers,
+// and the lane's part fits 32 bits.
+struct Place {
+  int64_t start;  // element of the tensor at which the row, or the tile, begins
+  int64_t block;  // block of 8-bit states that begins there
+  uint32_t col;   // of the lane's first element
+  int left;       // elements of the lane that exist
+};
+template <typename S>
+__device__ __forceinline__ S *element(S *base, const Place &at) {
+  using C = std::conditional_t<std::is_const_v<S>, const char, char>;
+  return reinterpret_cast<S *>(reinterpret_cast<C *>(base + at.start) + at.col * static_cast<uint32_t>(sizeof(S)));
+}
+
+// at.left (at most N) of the elements exist; the others are zeros, or are not stored.
+template <typename T, int N>
+__device__ __forceinline__ void load_raw_upto(const void *base, const Place &at, Raw<T, N> &r) {
+  using S = typename Traits<T>::store_t;
+  const S *p = element(static_cast<const S *>(base), at);
+  const int left = at.left;
+  if (left >= N) {
+    load_words<Raw<T, N>::kWords, sizeof(S)>(p, r.w);
+  } else {
+    S x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = j < left ? p[j] : S{};
     __builtin_memcpy(r.w, x, sizeof(x));
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const Raw8<T> &r, float (&o)[kAdamwLane]) {
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Raw<T, N> &r, float (&o)[N]) {
   if constexpr (Traits<T>::dtype == FLEXSAE_F32) {
 #pragma unroll
-    for (int j = 0; j < kAdamwLane; ++j) o[j] = __uint_as_float(r.w[j]);
+    for (int j = 0; j < N; ++j) o[j] = __uint_as_float(r.w[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < kAdamwLane; ++j) o[j] = Traits<T>::up(static_cast<uint16_t>(r.w[j / 2] >> (16 * (j % 2))));
+    for (int j = 0; j < N; ++j) o[j] = Traits<T>::up(static_cast<uint16_t>(r.w[j / 2] >> (16 * (j % 2))));
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(void *base, int64_t at, int left, const float (&x)[kAdamwLane]) {
+template <typename T, int N>
+__device__ __forceinline__ void store_upto(void *base, const Place &at, const float (&x)[N]) {
   using S = typename Traits<T>::store_t;
-  S *p = static_cast<S *>(base) + at;
-  if (left >= kAdamwLane) {
-    uint32_t w[Raw8<T>::kWords];
+  S *p = element(static_cast<S *>(base), at);
+  const int left = at.left;
+  if (left >= N) {
+    uint32_t w[Raw<T, N>::kWords];
 #pragma unroll
-    for (int j = 0; j < Raw8<T>::kWords; ++j) {
+    for (int j = 0; j < Raw<T, N>::kWords; ++j) {
       if constexpr (Traits<T>::dtype == FLEXSAE_F32) w[j] = __float_as_uint(x[j]);
       else if constexpr (Traits<T>::dtype == FLEXSAE_BF16) w[j] = f32x2_to_bf16x2_bits(x[2 * j], x[2 * j + 1]);
       else w[j] = static_cast<uint32_t>(f32_to_f16_bits(x[2 * j])) | (static_cast<uint32_t>(f32_to_f16_bits(x[2 * j + 1])) << 16);
     }
-#pragma unroll
-    for (int j = 0; j < Raw8<T>::kWords; j += 4) store16<sizeof(S)>(reinterpret_cast<char *>(p) + 4 * j, w + j);
+    store_words<Raw<T, N>::kWords, sizeof(S)>(p, w);
   } else {
 #pragma unroll
-    for (int j = 0; j < kAdamwLane; ++j)
+    for (int j = 0; j < N; ++j)
       if (j < left) p[j] = Traits<T>::down(x[j]);
   }
 }
 
 // ---- 8-bit states --------------------------------------------------------------------------
-// Sixteen bytes: (code of m, code of v) of eight elements.
-struct Codes8 {
-  uint32_t w[4];
+// (code of m, code of v) of N elements
+template <int N>
+struct Codes {
+  uint32_t w[N / 2];
 };
 
-__device__ __forceinline__ void load_codes(const void *base, int64_t at, int left, Codes8 &c) {
-  const uint16_t *p = static_cast<const uint16_t *>(base) + at;
-  if (left >= kAdamwLane) {
-    load16<2>(p, c.w);
+template <int N>
+__device__ __forceinline__ void load_codes(const void *base, const Place &at, Codes<N> &c) {
+  const uint16_t *p = element(static_cast<const uint16_t *>(base), at);
+  const int left = at.left;
+  if (left >= N) {
+    load_words<N / 2, 2>(p, c.w);
   } else {
-    uint16_t x[kAdamwLane];
+    uint16_t x[N];
 #pragma unroll
-    for (int j = 0; j < kAdamwLane; ++j) x[j] = j < left ? p[j] : uint16_t{128};
+    for (int j = 0; j < N; ++j) x[j] = j < left ? p[j] : uint16_t{128};
     __builtin_memcpy(c.w, x, sizeof(x));
   }
 }
 
-__device__ __forceinline__ void store_codes(void *base, int64_t at, int left, const Codes8 &c) {
-  uint16_t *p = static_cast<uint16_t *>(base) + at;
-  if (left >= kAdamwLane) {
-    store16<2>(p, c.w);
+template <int N>
+__device__ __forceinline__ void store_codes(void *base, const Place &at, const Codes<N> &c) {
+  uint16_t *p = element(static_cast<uint16_t *>(base), at);
+  const int left = at.left;
+  if (left >= N) {
+    store_words<N / 2, 2>(p, c.w);
   } else {
 #pragma unroll
-    for (int j = 0; j < kAdamwLane; ++j)
+    for (int j = 0; j < N; ++j)
       if (j < left) p[j] = static_cast<uint16_t>(c.w[j / 2] >> (16 * (j % 2)));
   }
 }
 
-__device__ __forceinline__ void decode8(const Codes8 &c, float a_m, float a_v, float (&m)[kAdamwLane], float (&v)[kAdamwLane]) {
+template <int N>
+__device__ __forceinline__ void decode(const Codes<N> &c, float a_m, float a_v, float (&m)[N], float (&v)[N]) {
+#pragma clang fp contract(off)
 #pragma unroll
-  for (int j = 0; j < kAdamwLane; ++j) {
+  for (int j = 0; j < N; ++j) {
     const uint32_t pair = c.w[j / 2] >> (16 * (j % 2));
     // (the squares of codes are exact; what follows is a rounding each, and none is raised to a power but that of 1 / 255^2)
     const float x = static_cast<float>(pair & 0xffu) - 128.f;
@@ -213,19 +281,38 @@ __device__ __forceinline__ void decode8(const Codes8 &c, float a_m, float a_v, f
   }
 }
 
-// The largest of the 32 lanes of each half of the wavefront.  As whole numbers: the bits of non-negative floats are in their
-// order, infinity and NaN above all.
-__device__ __forceinline__ uint32_t half_wave_max(uint32_t x) {
-  auto move = [](uint32_t y, auto ctrl) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(y), decltype(ctrl)::value, 0xf, 0xf, false));
+// Sum or maximum over each LANES (16, 32 or 64) consecutive lanes, in all of them.
+template <int LANES, typename T, typename F>
+__device__ __forceinline__ T across_lanes(T x, F join) {
+  static_assert(sizeof(T) == 4 && (LANES == 16 || LANES == 32 || LANES == 64), "");
+  auto bits = [](T y) {
+    uint32_t u;
+    __builtin_memcpy(&u, &y, 4);
+    return u;
   };
-  x = max(x, move(x, std::integral_constant<int, 0xB1>{}));   // lane ^ 1
-  x = max(x, move(x, std::integral_constant<int, 0x4E>{}));   // lane ^ 2
-  x = max(x, move(x, std::integral_constant<int, 0x141>{}));  // the other quad of each 8
-  x = max(x, move(x, std::integral_constant<int, 0x140>{}));  // the other half of each 16-lane row
+  auto value = [](uint32_t u) {
+    T y;
+    __builtin_memcpy(&y, &u, 4);
+    return y;
+  };
+  auto move = [&](T y, auto ctrl) {
+    return value(static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(bits(y)), decltype(ctrl)::value, 0xf, 0xf, false)));
+  };
+  x = join(x, move(x, std::integral_constant<int, 0xB1>{}));   // lane ^ 1
+  x = join(x, move(x, std::integral_constant<int, 0x4E>{}));   // lane ^ 2
+  x = join(x, move(x, std::integral_constant<int, 0x141>{}));  // the other quad of each 8
+  x = join(x, move(x, std::integral_constant<int, 0x140>{}));  // the other half of each 16-lane row
   typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-  const u32x2 r = __builtin_amdgcn_permlane16_swap(x, x, false, false);  // the other row of each two
-  return max(r[0], r[1]);
+  if constexpr (LANES >= 32) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(bits(x), bits(x), false, false);  // the other row of each two
+    x = join(value(r[0]), value(r[1]));
+  }
+  if constexpr (LANES == 64) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(bits(x), bits(x), false, false);  // the other half
+    x = join(value(r[0]), value(r[1]));
+  }
+  return x;
 }
 
 // What a maximum is kept as: zero below the smallest normal number (its inverse would overflow), NaN where the block has
@@ -234,148 +321,219 @@ __device__ __forceinline__ float kept_max(uint32_t bits) {
   return bits < 0x00800000u ? 0.f : bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(bits);
 }
 
-__device__ __forceinline__ void maxima8(const float (&m)[kAdamwLane], const float (&v)[kAdamwLane], float &a_m, float &a_v) {
+// The maxima of a block that LANES lanes hold.  As whole numbers: the bits of non-negative floats are in their order, infinity and
+// NaN above all.
+template <int LANES, int N>
+__device__ __forceinline__ void maxima(const float (&m)[N], const float (&v)[N], float &a_m, float &a_v) {
+  auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
   uint32_t bm = 0, bv = 0;
 #pragma unroll
-  for (int j = 0; j < kAdamwLane; ++j) {
+  for (int j = 0; j < N; ++j) {
     bm = max(bm, __float_as_uint(m[j]) & 0x7fffffffu);
     bv = max(bv, __float_as_uint(v[j]) & 0x7fffffffu);
   }
-  a_m = kept_max(half_wave_max(bm));
-  a_v = kept_max(half_wave_max(bv));
+  a_m = kept_max(across_lanes<LANES>(bm, larger));
+  a_v = kept_max(across_lanes<LANES>(bv, larger));
 }
 
-__device__ __forceinline__ void encode8(const float (&m)[kAdamwLane], const float (&v)[kAdamwLane], float a_m, float a_v, Codes8 &c) {
-  const float per_m = a_m > 0.f ? 1.f / a_m : 0.f, per_v = a_v > 0.f ? 1.f / a_v : 0.f;
+// Codes of two elements, (m, v) each, from |m| / a_m and v / a_v.  They are what correctly rounded roots give, whatever unit
+// computes them: EXACT takes such roots.  The hardware's are off by a unit in the last place each, which matters within kTie of
+// the middle between two codes only (2^-23 of 255 for the outer root, half of it for the inner one, and the products' rounding);
+// otherwise `root_m` = sqrt(|m| / a_m) and `root_v` = sqrt(v / a_v) come from there, and the result is the largest distance from a code.
+// Adding kMagic rounds to a whole number, which then stands in the low bits.
+constexpr float kTie = 7e-5f;
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+
+template <bool EXACT>
+__device__ __forceinline__ float codes_of_two(const float *m, const float *v, float per_m, float per_v, const float *root_v, uint32_t &w) {
+#pragma clang fp contract(off)
+  auto root = [](float x) { return EXACT ? sqrtf(x) : __builtin_amdgcn_sqrtf(x); };
+  float off = 0.f;
+  uint32_t pair[2];
 #pragma unroll
-  for (int j = 0; j < kAdamwLane / 2; ++j) {
-    uint32_t w = 0;
+  for (int k = 0; k < 2; ++k) {
+    const float x = copysignf(root(fabsf(m[k]) * per_m) * 127.f, m[k]), rx = x + (kMagic + 128.f);
+    const float q = EXACT ? sqrtf(v[k] * per_v) : root_v[k];
+    const float y = root(q) * 255.f, ry = y + kMagic;
+    if constexpr (!EXACT) off = fmaxf(off, fmaxf(fabsf(x - (rx - (kMagic + 128.f))), fabsf(y - (ry - kMagic))));
+    // (a v above zero never becomes zero)
+    const uint32_t cv = max(__float_as_uint(ry) & 0xffu, min(__float_as_uint(q), 1u));
+    pair[k] = __builtin_amdgcn_perm(cv, __float_as_uint(rx), 0x0c0c0400u);
+  }
+  w = pair[0] | (pair[1] << 16);
+  return off;
+}
+
+// s: the hardware's square roots of v
+template <int N>
+__device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], const float (&s)[N], float a_m, float a_v, Codes<N> &c) {
+  const float per_m = a_m > 0.f ? 1.f / a_m : 0.f, per_v = a_v > 0.f ? 1.f / a_v : 0.f, root_per_v = sqrtf(per_v);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      // (the hardware's square root, one unit in the last place: which of two codes a value between them gets)
-      const float x = __builtin_amdgcn_sqrtf(fabsf(m[2 * j + k]) * per_m);
-      const uint32_t cm = static_cast<uint32_t>(fmaf(copysignf(x, m[2 * j + k]), 127.f, 128.5f));
-      const float part = v[2 * j + k] * per_v;
-      const float y = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(part));
-      const uint32_t cv = max(static_cast<uint32_t>(fmaf(y, 255.f, 0.5f)), part > 0.f ? 1u : 0u);
-      w |= (cm | (cv << 8)) << (16 * k);
-    }
-    c.w[j] = w;
+  for (int j = 0; j < N; j += 2) {
+    const float root_v[2] = {s[j] * root_per_v, s[j + 1] * root_per_v};
+    const float off = codes_of_two<false>(m + j, v + j, per_m, per_v, root_v, c.w[j / 2]);
+    if (__any(off > 0.5f - kTie)) (void)codes_of_two<true>(m + j, v + j, per_m, per_v, root_v, c.w[j / 2]);
   }
 }
 
 // ---- the step ------------------------------------------------------------------------------
-__device__ __forceinline__ void adamw_moments(const AdamwCoefs &c, const float (&g)[kAdamwLane], float (&m)[kAdamwLane],
-                                              float (&v)[kAdamwLane]) {
+constexpr float kRootFloor = 1.0842022e-19f;  // 2^-63
+
+template <int N>
+__device__ __forceinline__ void adamw_moments(const AdamwCoefs &c, const float (&g)[N], float (&m)[N], float (&v)[N]) {
+// (each operation rounded by itself, like the roots of the codes: 8-bit states do not depend on what a compiler contracts)
+#pragma clang fp contract(off)
 #pragma unroll
-  for (int j = 0; j < kAdamwLane; ++j) {
-    m[j] = fmaf(c.b1, m[j], c.omb1 * g[j]);
-    v[j] = fmaf(c.b2, v[j], c.omb2 * g[j] * g[j]);
+  for (int j = 0; j < N; ++j) {
+    m[j] = m[j] * c.b1 + g[j] * c.omb1;
+    v[j] = v[j] * c.b2 + g[j] * g[j] * c.omb2;
   }
 }
 
-__device__ __forceinline__ void adamw_move(const AdamwCoefs &c, float step, float keep, const float (&m)[kAdamwLane],
-                                           const float (&v)[kAdamwLane], float (&w)[kAdamwLane]) {
+// s: square roots of v.  The hardware's root and reciprocal, each off by a unit in the last place: of the update, which is a small
+// part of the weight.  (It takes a v below the smallest normal number for zero: the root's floor keeps the quotient finite
+// where eps is zero.)
+template <int N>
+__device__ __forceinline__ void adamw_move(const AdamwCoefs &c, float step, float keep, const float (&m)[N], const float (&s)[N],
+                                           float (&w)[N]) {
 #pragma unroll
-  for (int j = 0; j < kAdamwLane; ++j) {
-    const float by = m[j] / fmaf(sqrtf(v[j]), c.inv_sqrt_bc2, c.eps);
-    w[j] = fmaf(-step, by, keep * w[j]);
+  for (int j = 0; j < N; ++j) {
+    const float per = __builtin_amdgcn_rcpf(fmaf(fmaxf(s[j], kRootFloor), c.inv_sqrt_bc2, c.eps));
+    w[j] = fmaf(-step, m[j] * per, keep * w[j]);
   }
 }
 
-// A lane's eight elements of the tensors that a step works on: as loaded, and as numbers.
+// Elements of a lane that follow each other: as many as make sixteen bytes of the widest tensor, so that every access of a
+// wavefront is one stretch of memory (two accesses of half a stretch each cost a tenth of the bandwidth).
 template <typename T, bool MASTER, bool EIGHT>
-struct AdamwLane {
-  using W = std::conditional_t<MASTER, float, T>;
-  Raw8<T> rg;
-  Raw8<W> rw;
-  Raw8<float> rm, rv;  // states in 32 bits,
-  Codes8 codes;        // in 8
-  float2 top;
-  int64_t at, block;
-  int left;
+constexpr int kUnit = EIGHT && !MASTER && sizeof(typename Traits<T>::store_t) == 2 ? 8 : 4;
 
-  // elements [at, at + 8) of a tensor, of which `left` (at most 8) exist; block: that of their 8-bit states
-  __device__ __forceinline__ void load(const AdamwTensor &t, int64_t at_, int64_t rest, int64_t block_) {
-    at = at_;
-    block = block_;
-    left = rest > kAdamwLane ? kAdamwLane : rest < 0 ? 0 : static_cast<int>(rest);
-    load8<T>(t.grad, at, left, rg);
-    load8<W>(MASTER ? t.master : t.param, at, left, rw);
+// A lane's elements of the tensors that a step works on: as loaded, and as numbers.
+template <typename T, bool MASTER, bool EIGHT>
+struct AdamwUnit {
+  static constexpr int N = kUnit<T, MASTER, EIGHT>;
+  static constexpr int kQuantLanes = kAdamwQuant / N;  // that hold a block of 8-bit states
+  using W = std::conditional_t<MASTER, float, T>;
+  Raw<T, N> rg;
+  Raw<W, N> rw;
+  Raw<float, EIGHT ? 0 : N> rm, rv;  // states in 32 bits,
+  Codes<EIGHT ? N : 0> codes;        // in 8
+  float2 top;
+
+  __device__ __forceinline__ void load(const AdamwTensor &t, const Place &at) {
+    load_raw_upto(t.grad, at, rg);
+    load_raw_upto(MASTER ? t.master : t.param, at, rw);
     if constexpr (EIGHT) {
-      load_codes(t.s0, at, left, codes);
-      top = left > 0 ? static_cast<const float2 *>(t.s1)[block] : float2{0.f, 0.f};
+      load_codes(t.s0, at, codes);
+      top = at.left > 0 ? static_cast<const float2 *>(t.s1)[at.block + at.col / kAdamwQuant] : float2{0.f, 0.f};
     } else {
-      load8<float>(t.s0, at, left, rm);
-      load8<float>(t.s1, at, left, rv);
+      load_raw_upto(t.s0, at, rm);
+      load_raw_upto(t.s1, at, rv);
     }
   }
 
-  // m, v from g and what they were; stored; w moved
-  __device__ __forceinline__ void step(const AdamwTensor &t, const AdamwCoefs &c, const float (&g)[kAdamwLane],
-                                       float (&w)[kAdamwLane], bool store) {
-    float m[kAdamwLane], v[kAdamwLane];
+  // m, v from g and what they were; w moved; STORE: m and v stored.  LANES share a row.
+  template <bool STORE, int LANES>
+  __device__ __forceinline__ void step(const AdamwTensor &t, const AdamwCoefs &c, const Place &at, const float (&g)[N], float (&w)[N]) {
+    float m[N], v[N], s[N];
     if constexpr (EIGHT) {
-      decode8(codes, top.x, top.y, m, v);
+      decode(codes, top.x, top.y, m, v);
     } else {
-      unpack8(rm, m);
-      unpack8(rv, v);
+      unpack(rm, m);
+      unpack(rv, v);
     }
     adamw_moments(c, g, m, v);
-    adamw_move(c, t.lr * c.inv_bc1, 1.f - t.lr * c.lr * t.weight_decay, m, v, w);
-    if (!store) return;
-    if constexpr (EIGHT) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[j] = __builtin_amdgcn_sqrtf(v[j]);
+    adamw_move(c, t.lr * c.inv_bc1, 1.f - t.lr * c.lr * t.weight_decay, m, s, w);
+    if constexpr (STORE && EIGHT) {
+      constexpr int kLanes = LANES < kQuantLanes ? LANES : kQuantLanes;
       float a_m, a_v;
-      maxima8(m, v, a_m, a_v);
-      Codes8 now;
-      encode8(m, v, a_m, a_v, now);
-      store_codes(t.s0, at, left, now);
-      if (left > 0 && (threadIdx.x & 31) == 0) static_cast<float2 *>(t.s1)[block] = float2{a_m, a_v};
-    } else {
-      store8<float>(t.s0, at, left, m);
-      store8<float>(t.s1, at, left, v);
+      maxima<kLanes>(m, v, a_m, a_v);
+      Codes<N> now;
+      encode(m, v, s, a_m, a_v, now);
+      store_codes(t.s0, at, now);
+      if (at.left > 0 && (threadIdx.x & (kLanes - 1)) == 0)
+        static_cast<float2 *>(t.s1)[at.block + at.col / kAdamwQuant] = float2{a_m, a_v};
+    } else if constexpr (STORE) {
+      store_upto<float>(t.s0, at, m);
+      store_upto<float>(t.s1, at, v);
     }
   }
 
-  __device__ __forceinline__ void store(const AdamwTensor &t, const float (&w)[kAdamwLane]) const {
-    store8<T>(t.param, at, left, w);
-    if constexpr (MASTER) store8<float>(t.master, at, left, w);
+  __device__ __forceinline__ void store(const AdamwTensor &t, const Place &at, const float (&w)[N]) const {
+    if constexpr (MASTER) {
+      float x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        x[j] = w[j];
+        // the 32-bit number itself is what is rounded (an instruction that multiplies, adds and rounds to fp16 would leave it out)
+        if constexpr (Traits<T>::dtype == FLEXSAE_F16) asm("" : "+v"(x[j]));
+      }
+      store_upto<T>(t.param, at, x);
+      store_upto<float>(t.master, at, x);
+    } else {
+      store_upto<T>(t.param, at, w);
+    }
   }
 };
 
-template <typename T, bool MASTER, bool EIGHT>
+// What exists of N elements of which `rest` are left.
+template <int N>
+__device__ __forceinline__ int upto(int64_t rest) {
+  return rest > N ? N : rest < 0 ? 0 : static_cast<int>(rest);
+}
+
+// FULL: the tile ends within the tensor.
+template <typename T, bool MASTER, bool EIGHT, bool FULL>
 __device__ __forceinline__ void adamw_tile(const AdamwTensor &t, int64_t base, const AdamwCoefs &c) {
-  const int64_t at = base + static_cast<int64_t>(threadIdx.x) * kAdamwLane;
-  AdamwLane<T, MASTER, EIGHT> lane;
-  lane.load(t, at, t.cols - at, at / kAdamwQuant);
-  float g[kAdamwLane], w[kAdamwLane];
-  unpack8(lane.rg, g);
-  unpack8(lane.rw, w);
+  using Unit = AdamwUnit<T, MASTER, EIGHT>;
+  constexpr int N = Unit::N, kUnits = kAdamwTile / (kAdamwThreads * N);
+  Unit unit[kUnits];
+  auto place = [&](int u) -> Place {
+    const uint32_t col = (u * kAdamwThreads + threadIdx.x) * N;
+    return {base, base / kAdamwQuant, col, FULL ? N : upto<N>(t.cols - base - col)};
+  };
 #pragma unroll
-  for (int j = 0; j < kAdamwLane; ++j) g[j] *= c.grad;
-  lane.step(t, c, g, w, true);
-  lane.store(t, w);
+  for (int u = 0; u < kUnits; ++u) unit[u].load(t, place(u));
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    float g[N], w[N];
+    unpack(unit[u].rg, g);
+    unpack(unit[u].rw, w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] *= c.grad;
+    unit[u].template step<true, kWave>(t, c, place(u), g, w);
+    unit[u].store(t, place(u), w);
+  }
 }
 
 template <bool EIGHT>
 __global__ __launch_bounds__(kAdamwThreads) void adamw_kernel(const AdamwTable a) {
   const AdamwCoefs c = adamw_coefs(a);
   if (!c.go) return;
-  for (uint32_t tile = blockIdx.x; tile < a.first[a.count]; tile += gridDim.x) {
+  const uint32_t end = min(a.first[a.count], (blockIdx.x + 1) * a.per_block);
+  for (uint32_t tile = blockIdx.x * a.per_block; tile < end; ++tile) {
     const int i = tensor_of(a, tile);
     const AdamwTensor &t = a.tensor[i];
     const int64_t base = static_cast<int64_t>(tile - a.first[i]) * kAdamwTile;
-    if (t.dtype == FLEXSAE_F32) adamw_tile<float, false, EIGHT>(t, base, c);
-    else if (t.dtype == FLEXSAE_BF16) t.master ? adamw_tile<bf16_t, true, EIGHT>(t, base, c) : adamw_tile<bf16_t, false, EIGHT>(t, base, c);
-    else t.master ? adamw_tile<f16_t, true, EIGHT>(t, base, c) : adamw_tile<f16_t, false, EIGHT>(t, base, c);
+    auto tile_of = [&](auto full) {
+      constexpr bool kFull = decltype(full)::value;
+      if (t.dtype == FLEXSAE_F32) adamw_tile<float, false, EIGHT, kFull>(t, base, c);
+      else if (t.dtype == FLEXSAE_BF16) t.master ? adamw_tile<bf16_t, true, EIGHT, kFull>(t, base, c) : adamw_tile<bf16_t, false, EIGHT, kFull>(t, base, c);
+      else t.master ? adamw_tile<f16_t, true, EIGHT, kFull>(t, base, c) : adamw_tile<f16_t, false, EIGHT, kFull>(t, base, c);
+    };
+    if (base + kAdamwTile <= t.cols) tile_of(std::true_type{});
+    else tile_of(std::false_type{});
   }
   adamw_count(a);
 }
 
-// Sums over the WAVES wavefronts of a row; `turn` alternates between two places so that one barrier a sum is enough.
-template <int WAVES>
+// Sums over a row that LANES lanes of a wavefront, or WAVES wavefronts of a block, hold; `turn` alternates between two places so
+// that one barrier a sum is enough.
+template <int WAVES, int LANES>
 __device__ __forceinline__ float row_sum(float x, float (*place)[16], int turn) {
-  x = wave_sum_bcast(x);
+  x = across_lanes<LANES>(x, [](float y, float z) { return y + z; });
   if constexpr (WAVES > 1) {
     if (lane_id() == 0) place[turn][wave_in_block()] = x;
     __syncthreads();
@@ -386,101 +544,114 @@ __device__ __forceinline__ float row_sum(float x, float (*place)[16], int turn) 
   return x;
 }
 
-// Rows of length one.  WAVES wavefronts hold a row, SEGMENTS stretches of 512 elements each, in registers: every tensor is
-// read and written once.  SEGMENTS = 0: a row of any length is walked three times (the two products; the length of the moved
-// row; the step), nothing stored before the last walk.
-template <typename T, bool MASTER, bool EIGHT, int WAVES, int SEGMENTS>
+// Rows of length one.  LANES (64 at least with more than one) of each of WAVES wavefronts hold a row, UNITS units of elements each,
+// in registers: every tensor is read and written once.  UNITS = 0: a row of any length is walked three times (the two products;
+// the length of the moved row; the step), nothing stored before the last walk.
+template <typename T, bool MASTER, bool EIGHT, int WAVES, int LANES, int UNITS>
 __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * kWave) void adamw_rows_kernel(const AdamwTable a) {
-  constexpr int kRows = WAVES < 4 ? 4 / WAVES : 1;  // of a block at a time
-  constexpr int kSegment = kWave * kAdamwLane;
+  static_assert(LANES == kWave || (WAVES == 1 && UNITS == 1), "less than a wavefront: one unit");
+  using Unit = AdamwUnit<T, MASTER, EIGHT>;
+  constexpr int N = Unit::N, kStretch = LANES * N;
+  constexpr int kRows = WAVES < 4 ? 4 / WAVES * (kWave / LANES) : 1;  // of a block at a time
   __shared__ float place[2][16];
   const AdamwCoefs c = adamw_coefs(a);
   if (!c.go) return;
   const int wave = wave_in_block() % WAVES;
-  for (uint32_t tile = blockIdx.x; tile < a.first[a.count]; tile += gridDim.x) {
+  const uint32_t end = min(a.first[a.count], (blockIdx.x + 1) * a.per_block);
+  for (uint32_t tile = blockIdx.x * a.per_block; tile < end; ++tile) {
     const int i = tensor_of(a, tile);
     const AdamwTensor &t = a.tensor[i];
-    const int64_t row = static_cast<int64_t>(tile - a.first[i]) * kRows + wave_in_block() / WAVES;
+    int64_t row = static_cast<int64_t>(tile - a.first[i]) * kRows + wave_in_block() / WAVES * (kWave / LANES);
     if (row >= t.rows) continue;  // (of a whole wavefront: a block of several rows has no barriers)
-    const int64_t start = row * t.cols, blocks = (t.cols + kAdamwQuant - 1) / kAdamwQuant;
-    auto load = [&](AdamwLane<T, MASTER, EIGHT> &lane, int64_t s) {
-      const int64_t col = (s * WAVES + wave) * kSegment + lane_id() * kAdamwLane;
-      lane.load(t, start + col, t.cols - col, row * blocks + col / kAdamwQuant);
+    if constexpr (LANES < kWave) row += lane_id() / LANES;
+    const bool live = LANES == kWave || row < t.rows;
+    const int cols = static_cast<int>(t.cols);
+    const int64_t start = row * cols, block = row * ((cols + kAdamwQuant - 1) / kAdamwQuant);
+    auto stretch = [&](int u) { return (u * WAVES + wave) * kStretch; };
+    auto at = [&](int u) -> Place {
+      const int col = stretch(u) + lane_id() % LANES * N;
+      return {start, block, static_cast<uint32_t>(col), live ? upto<N>(cols - col) : 0};
     };
-    auto products = [&](const AdamwLane<T, MASTER, EIGHT> &lane, float (&g)[kAdamwLane], float (&w)[kAdamwLane], float &gw, float &ww) {
-      unpack8(lane.rg, g);
-      unpack8(lane.rw, w);
+    auto products = [&](const Unit &unit, float (&g)[N], float (&w)[N], float &gw, float &ww) {
+      unpack(unit.rg, g);
+      unpack(unit.rw, w);
 #pragma unroll
-      for (int j = 0; j < kAdamwLane; ++j) {
+      for (int j = 0; j < N; ++j) {
         g[j] *= c.grad;
         gw = fmaf(g[j], w[j], gw);
         ww = fmaf(w[j], w[j], ww);
       }
     };
-    auto across = [&](float along, float (&g)[kAdamwLane], const float (&w)[kAdamwLane]) {
+    auto across = [&](float along, float (&g)[N], const float (&w)[N]) {
+#pragma clang fp contract(off)
 #pragma unroll
-      for (int j = 0; j < kAdamwLane; ++j) g[j] = fmaf(-along, w[j], g[j]);
+      for (int j = 0; j < N; ++j) g[j] = g[j] - along * w[j];
     };
-    auto squares = [&](const float (&w)[kAdamwLane], float &s) {
+    auto squares = [&](const float (&w)[N], float &s) {
 #pragma unroll
-      for (int j = 0; j < kAdamwLane; ++j) s = fmaf(w[j], w[j], s);
+      for (int j = 0; j < N; ++j) s = fmaf(w[j], w[j], s);
     };
-    auto scaled = [&](float by, float (&w)[kAdamwLane]) {
+    auto scaled = [&](float by, float (&w)[N]) {
 #pragma unroll
-      for (int j = 0; j < kAdamwLane; ++j) w[j] *= by;
+      for (int j = 0; j < N; ++j) w[j] *= by;
     };
     float gw = 0.f, ww = 0.f, nn = 0.f;
-    if constexpr (SEGMENTS > 0) {
-      AdamwLane<T, MASTER, EIGHT> lane[SEGMENTS];
-      float g[SEGMENTS][kAdamwLane], w[SEGMENTS][kAdamwLane];
+    if constexpr (UNITS > 0) {
+      // (units beyond the row's end, the same ones for the whole wavefront, are left out)
+      Unit unit[UNITS];
+      float g[UNITS][N], w[UNITS][N];
 #pragma unroll
-      for (int s = 0; s < SEGMENTS; ++s) load(lane[s], s);
+      for (int u = 0; u < UNITS; ++u)
+        if (u == 0 || stretch(u) < cols) unit[u].load(t, at(u));
 #pragma unroll
-      for (int s = 0; s < SEGMENTS; ++s) products(lane[s], g[s], w[s], gw, ww);
-      gw = row_sum<WAVES>(gw, place, 0);
-      ww = row_sum<WAVES>(ww, place, 1);
+      for (int u = 0; u < UNITS; ++u)
+        if (u == 0 || stretch(u) < cols) products(unit[u], g[u], w[u], gw, ww);
+      gw = row_sum<WAVES, LANES>(gw, place, 0);
+      ww = row_sum<WAVES, LANES>(ww, place, 1);
       const float along = ww > 0.f ? gw / ww : 0.f;
 #pragma unroll
-      for (int s = 0; s < SEGMENTS; ++s) {
-        across(along, g[s], w[s]);
-        lane[s].step(t, c, g[s], w[s], true);
-        squares(w[s], nn);
-      }
-      nn = row_sum<WAVES>(nn, place, 0);
+      for (int u = 0; u < UNITS; ++u)
+        if (u == 0 || stretch(u) < cols) {
+          across(along, g[u], w[u]);
+          unit[u].template step<true, LANES>(t, c, at(u), g[u], w[u]);
+          squares(w[u], nn);
+        }
+      nn = row_sum<WAVES, LANES>(nn, place, 0);
       const float by = nn > 0.f ? 1.f / sqrtf(nn) : 1.f;
 #pragma unroll
-      for (int s = 0; s < SEGMENTS; ++s) {
-        scaled(by, w[s]);
-        lane[s].store(t, w[s]);
-      }
+      for (int u = 0; u < UNITS; ++u)
+        if (u == 0 || stretch(u) < cols) {
+          scaled(by, w[u]);
+          unit[u].store(t, at(u), w[u]);
+        }
     } else {
-      const int64_t segments = (t.cols + WAVES * kSegment - 1) / (WAVES * kSegment);
-      AdamwLane<T, MASTER, EIGHT> lane;
-      float g[kAdamwLane], w[kAdamwLane];
-      for (int64_t s = 0; s < segments; ++s) {
-        load(lane, s);
-        products(lane, g, w, gw, ww);
+      const int units = (cols - 1) / (WAVES * kStretch) + 1;
+      Unit unit;
+      float g[N], w[N];
+      for (int u = 0; u < units; ++u) {
+        unit.load(t, at(u));
+        products(unit, g, w, gw, ww);
       }
-      gw = row_sum<WAVES>(gw, place, 0);
-      ww = row_sum<WAVES>(ww, place, 1);
+      gw = row_sum<WAVES, LANES>(gw, place, 0);
+      ww = row_sum<WAVES, LANES>(ww, place, 1);
       const float along = ww > 0.f ? gw / ww : 0.f;
       float unused_gw = 0.f, unused_ww = 0.f;
-      for (int64_t s = 0; s < segments; ++s) {
-        load(lane, s);
-        products(lane, g, w, unused_gw, unused_ww);
+      for (int u = 0; u < units; ++u) {
+        unit.load(t, at(u));
+        products(unit, g, w, unused_gw, unused_ww);
         across(along, g, w);
-        lane.step(t, c, g, w, false);
+        unit.template step<false, LANES>(t, c, at(u), g, w);
         squares(w, nn);
       }
-      nn = row_sum<WAVES>(nn, place, 0);
+      nn = row_sum<WAVES, LANES>(nn, place, 0);
       const float by = nn > 0.f ? 1.f / sqrtf(nn) : 1.f;
-      for (int64_t s = 0; s < segments; ++s) {
-        load(lane, s);
-        products(lane, g, w, unused_gw, unused_ww);
+      for (int u = 0; u < units; ++u) {
+        unit.load(t, at(u));
+        products(unit, g, w, unused_gw, unused_ww);
         across(along, g, w);
-        lane.step(t, c, g, w, true);
+        unit.template step<true, LANES>(t, c, at(u), g, w);
         scaled(by, w);
-        lane.store(t, w);
+        unit.store(t, at(u), w);
       }
     }
     // (the next row's first sum may write place[0] while a wavefront still reads it for this one's length)
@@ -507,18 +678,23 @@ static_assert(sizeof(NormTable) <= 4096, "kernel arguments");
 
 // Squares are summed in 64 bits: those of finite 32-bit numbers neither overflow nor vanish there, and the order of the sum,
 // which is the same on every run, hardly matters.
-template <typename T>
-__device__ __forceinline__ double squares_of_tile(const void *grad, int64_t n, int64_t base) {
-  double sum = 0.0;
-  const int64_t at = base + static_cast<int64_t>(threadIdx.x) * kAdamwLane;
-  const int64_t rest = n - at;
-  Raw8<T> r;
-  load8<T>(grad, at, rest > kAdamwLane ? kAdamwLane : rest < 0 ? 0 : static_cast<int>(rest), r);
-  float x[kAdamwLane];
-  unpack8(r, x);
+template <typename T, bool FULL>
+__device__ __forceinline__ void squares_of_tile(const void *grad, int64_t n, int64_t base, double (&sum)[kNormSums]) {
+  constexpr int N = 16 / static_cast<int>(sizeof(typename Traits<T>::store_t)), kLoads = kNormTile / (kAdamwThreads * N);
+  Raw<T, N> r[kLoads];
 #pragma unroll
-  for (int j = 0; j < kAdamwLane; ++j) sum = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), sum);
-  return sum;
+  for (int u = 0; u < kLoads; ++u) {
+    const uint32_t col = (u * kAdamwThreads + threadIdx.x) * N;
+    load_raw_upto(grad, Place{base, 0, col, FULL ? N : upto<N>(n - base - col)}, r[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+    float x[N];
+    unpack(r[u], x);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      sum[u % kNormSums] = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), sum[u % kNormSums]);
+  }
 }
 
 // The block's sum, in thread 0 (in a fixed order).
@@ -533,17 +709,25 @@ __device__ __forceinline__ double block_sum(double x) {
 }
 
 __global__ __launch_bounds__(kAdamwThreads) void norm_partial_kernel(const NormTable a) {
-  double sum = 0.0;
+  double sum[kNormSums] = {};
   for (uint32_t tile = blockIdx.x; tile < a.first[a.count]; tile += gridDim.x) {
     const int i = tensor_of(a, tile);
     const NormTensor &t = a.tensor[i];
-    const int64_t base = static_cast<int64_t>(tile - a.first[i]) * kAdamwTile;
-    if (t.dtype == FLEXSAE_F32) sum += squares_of_tile<float>(t.grad, t.n, base);
-    else if (t.dtype == FLEXSAE_BF16) sum += squares_of_tile<bf16_t>(t.grad, t.n, base);
-    else sum += squares_of_tile<f16_t>(t.grad, t.n, base);
+    const int64_t base = static_cast<int64_t>(tile - a.first[i]) * kNormTile;
+    auto tile_of = [&](auto full) {
+      constexpr bool kFull = decltype(full)::value;
+      if (t.dtype == FLEXSAE_F32) squares_of_tile<float, kFull>(t.grad, t.n, base, sum);
+      else if (t.dtype == FLEXSAE_BF16) squares_of_tile<bf16_t, kFull>(t.grad, t.n, base, sum);
+      else squares_of_tile<f16_t, kFull>(t.grad, t.n, base, sum);
+    };
+    if (base + kNormTile <= t.n) tile_of(std::true_type{});
+    else tile_of(std::false_type{});
   }
-  sum = block_sum(sum);
-  if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
+  double all = 0.0;
+#pragma unroll
+  for (int u = 0; u < kNormSums; ++u) all += sum[u];
+  all = block_sum(all);
+  if (threadIdx.x == 0) a.partial[blockIdx.x] = all;
 }
 
 __global__ __launch_bounds__(kAdamwThreads) void norm_finish_kernel(const double *partial, int64_t n, float *norm) {
@@ -571,21 +755,26 @@ static_assert(sizeof(MomentsTable) <= 4096, "kernel arguments");
 // A tile is 2048 elements of one row.
 template <typename T>
 __global__ __launch_bounds__(kAdamwThreads) void adamw8_moments_kernel(const MomentsTable a) {
+  constexpr int N = 16 / static_cast<int>(sizeof(typename Traits<T>::store_t));
   for (uint32_t tile = blockIdx.x; tile < a.first[a.count]; tile += gridDim.x) {
     const int i = tensor_of(a, tile);
     const MomentsTensor &t = a.tensor[i];
     const int64_t per_row = (t.cols + kAdamwTile - 1) / kAdamwTile, blocks = (t.cols + kAdamwQuant - 1) / kAdamwQuant;
     const int64_t row = (tile - a.first[i]) / per_row, part = (tile - a.first[i]) % per_row;
-    const int64_t col = part * kAdamwTile + static_cast<int64_t>(threadIdx.x) * kAdamwLane, rest = t.cols - col;
-    if (rest <= 0) continue;
-    const int left = rest > kAdamwLane ? kAdamwLane : static_cast<int>(rest);
-    Codes8 codes;
-    load_codes(t.codes, row * t.cols + col, left, codes);
-    const float2 top = reinterpret_cast<const float2 *>(t.maxima)[row * blocks + col / kAdamwQuant];
-    float m[kAdamwLane], v[kAdamwLane];
-    decode8(codes, top.x, top.y, m, v);
-    store8<T>(t.m, row * t.cols + col, left, m);
-    store8<T>(t.v, row * t.cols + col, left, v);
+#pragma unroll
+    for (int u = 0; u < kAdamwTile / (kAdamwThreads * N); ++u) {
+      const int64_t from = part * kAdamwTile;
+      const uint32_t col = (u * kAdamwThreads + threadIdx.x) * N;
+      const Place at = {row * t.cols + from, row * blocks + from / kAdamwQuant, col, upto<N>(t.cols - from - col)};
+      if (at.left == 0) continue;
+      Codes<N> codes;
+      load_codes(t.codes, at, codes);
+      const float2 top = reinterpret_cast<const float2 *>(t.maxima)[at.block + col / kAdamwQuant];
+      float m[N], v[N];
+      decode(codes, top.x, top.y, m, v);
+      store_upto<T>(t.m, at, m);
+      store_upto<T>(t.v, at, v);
+    }
   }
 }
 

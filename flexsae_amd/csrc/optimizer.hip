@@ -17,18 +17,25 @@ int launch_status() { return hipGetLastError() == hipSuccess ? FLEXSAE_OK : FLEX
 
 constexpr int64_t kMostElements = int64_t{1} << 40;  // of a tensor: tiles are counted in 32 bits
 
-// Blocks of a launch: enough to fill the chip several times over; each then takes one tile after another, so that what a block
-// does once (the step's factors, counting the step) is paid a bounded number of times.
-constexpr int64_t kStepBlocks = 2048;
-constexpr int64_t kNormBlocks = 1024;
+constexpr int64_t kMostTiles = int64_t{1} << 31;  // of a launch
+constexpr int64_t kTicketTiles = 256;             // up to so many the launch's own blocks count the step
+constexpr int64_t kPairTiles = 8192;              // from so many on a block takes two
+#ifndef FEW
+#define FEW 2048
+#endif
+#ifndef PERB
+#define PERB 4
+#endif
+constexpr int64_t kNormBlocks = 1024;  // each takes one tile after another, and leaves one partial sum
 
 unsigned blocks_for(int64_t tiles, int64_t most) { return static_cast<unsigned>(tiles < 1 ? 1 : tiles > most ? most : tiles); }
 
 int check_tensor(const flexsae_adamw_tensor &t, const flexsae_adamw_config &c) {
+  const bool unit = c.flags & FLEXSAE_ADAMW_UNIT_ROWS;
   if (t.rows < 0 || t.cols < 0 || !valid_dtype(t.dtype)) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (!(t.lr >= 0.f) || !(t.weight_decay >= 0.f)) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (t.rows == 0 || t.cols == 0) return FLEXSAE_OK;
-  if (t.rows > kMostElements / t.cols) return FLEXSAE_ERR_UNSUPPORTED;
+  if (t.rows > kMostElements / t.cols || (unit && t.cols >= (int64_t{1} << 29))) return FLEXSAE_ERR_UNSUPPORTED;
   if (!t.param || !t.grad || !t.state0 || !t.state1) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (t.master && t.dtype == FLEXSAE_F32) return FLEXSAE_ERR_INVALID_ARGUMENT;
   const size_t es = dtype_size(t.dtype);
@@ -75,15 +82,17 @@ struct RowPlan {
 
 template <typename T, bool MASTER, bool EIGHT>
 RowPlan row_plan(int64_t cols) {
-  constexpr int64_t kSegment = kWave * kAdamwLane;
-  if (cols <= kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 1>, 256, 4};
-  if (cols <= 2 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 2>, 256, 4};
-  if (cols <= 3 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 3>, 256, 4};
-  if (cols <= 5 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 5>, 256, 4};
-  if (cols <= 8 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 4, 2>, 256, 1};
-  if (cols <= 16 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 4, 4>, 256, 1};
-  if (cols <= 32 * kSegment) return {adamw_rows_kernel<T, MASTER, EIGHT, 16, 2>, 1024, 1};
-  return {adamw_rows_kernel<T, MASTER, EIGHT, 16, 0>, 1024, 1};
+  constexpr int N = kUnit<T, MASTER, EIGHT>, U = 8 / N;
+  if (cols <= 16 * N) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 16, 1>, 256, 16};
+  if (cols <= 32 * N) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 32, 1>, 256, 8};
+  if (cols <= 64 * N) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 64, 1>, 256, 4};
+  if (cols <= 2 * 64 * N) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 64, 2>, 256, 4};
+  if (cols <= 1024) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 64, 2 * U>, 256, 4};
+  if (cols <= 2560) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 64, 5 * U>, 256, 4};
+  if (cols <= 4096) return {adamw_rows_kernel<T, MASTER, EIGHT, 4, 64, 2 * U>, 256, 1};
+  if (cols <= 8192) return {adamw_rows_kernel<T, MASTER, EIGHT, 4, 64, 4 * U>, 256, 1};
+  if (cols <= 16384) return {adamw_rows_kernel<T, MASTER, EIGHT, 16, 64, 2 * U>, 1024, 1};
+  return {adamw_rows_kernel<T, MASTER, EIGHT, 16, 64, 0>, 1024, 1};
 }
 
 template <bool EIGHT>
@@ -95,7 +104,7 @@ RowPlan row_plan(const flexsae_adamw_tensor &t) {
 
 // Adds a tensor of `tiles` tiles; false: the table is full.
 bool add(AdamwTable &a, const flexsae_adamw_tensor &t, int64_t tiles, bool flat) {
-  if (a.count == kAdamwTensors || a.first[a.count] + tiles > (int64_t{1} << 31)) return false;
+  if (a.count == kAdamwTensors || a.first[a.count] + tiles > kMostTiles) return false;
   a.tensor[a.count] = {t.param, t.grad, t.state0, t.state1, static_cast<float *>(t.master), flat ? 1 : t.rows,
                        flat ? t.rows * t.cols : t.cols, t.lr, t.weight_decay, t.dtype};
   a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(tiles);
@@ -103,11 +112,26 @@ bool add(AdamwTable &a, const flexsae_adamw_tensor &t, int64_t tiles, bool flat)
   return true;
 }
 
-int launch(Kernel kernel, int threads, AdamwTable &a, bool last, hipStream_t stream) {
-  a.last = last;
-  kernel<<<blocks_for(a.first[a.count], kStepBlocks), threads, 0, stream>>>(a);
+int launch(Kernel kernel, int threads, AdamwTable &a, bool eight, bool last, hipStream_t stream) {
+  const int64_t tiles = a.first[a.count];
+  // (two tiles a block where the arithmetic of 8-bit states counts and there are blocks enough: what a block computes once)
+  a.per_block = eight && tiles > kPairTiles ? 2 : 1;
+  const int64_t blocks = tiles < 1 ? 1 : ceil_div(tiles, a.per_block);
+  if (last && a.counting != kCountedBefore) a.counting = kCountedByTicket;
+  kernel<<<static_cast<unsigned>(blocks), threads, 0, stream>>>(a);
   a.count = 0;
   return launch_status();
+}
+
+// Tiles of the tensor in the kernels' sense.
+struct Work {
+  RowPlan plan;
+  int64_t tiles;
+};
+Work work_of(const flexsae_adamw_tensor &t, bool eight, bool unit) {
+  if (!unit) return {{eight ? adamw_kernel<true> : adamw_kernel<false>, kAdamwThreads, 1}, ceil_div(t.rows * t.cols, kAdamwTile)};
+  const RowPlan plan = eight ? row_plan<true>(t) : row_plan<false>(t);
+  return {plan, ceil_div(t.rows, plan.rows)};
 }
 
 }  // namespace
@@ -118,30 +142,35 @@ int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const
   if (const int rc = check_config(config)) return rc;
   if (count < 0 || (count > 0 && !tensors)) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (config->flags & ~FLEXSAE_ADAMW_UNIT_ROWS) return FLEXSAE_ERR_INVALID_ARGUMENT;
-  for (int64_t i = 0; i < count; ++i)
-    if (const int rc = check_tensor(tensors[i], *config)) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool eight = config->state_bits == 8, unit = config->flags & FLEXSAE_ADAMW_UNIT_ROWS;
-  const Kernel flat = eight ? adamw_kernel<true> : adamw_kernel<false>;
+  int64_t all = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (const int rc = check_tensor(tensors[i], *config)) return rc;
+    if (tensors[i].rows == 0 || tensors[i].cols == 0) continue;
+    const int64_t tiles = work_of(tensors[i], eight, unit).tiles;
+    if (tiles > kMostTiles) return FLEXSAE_ERR_UNSUPPORTED;
+    all += tiles;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
   AdamwTable a = table_of(*config);
+  if (all > kTicketTiles) {
+    a.counting = kCountedBefore;
+    adamw_count_kernel<<<1, 1, 0, s>>>(a.counter, a.grad_norm);
+  }
   // Tensors that the same kernel takes go into one launch; a table that is full, or another kernel's turn, ends a launch.
-  Kernel kernel = flat;
-  int threads = kAdamwThreads;
+  RowPlan plan = {eight ? adamw_kernel<true> : adamw_kernel<false>, kAdamwThreads, 1};
   for (int64_t i = 0; i < count; ++i) {
     const flexsae_adamw_tensor &t = tensors[i];
     if (t.rows == 0 || t.cols == 0) continue;
-    const RowPlan plan = !unit ? RowPlan{flat, kAdamwThreads, 1} : eight ? row_plan<true>(t) : row_plan<false>(t);
-    const int64_t tiles = unit ? ceil_div(t.rows, plan.rows) : ceil_div(t.rows * t.cols, kAdamwTile);
-    if (tiles > (int64_t{1} << 31)) return FLEXSAE_ERR_UNSUPPORTED;
-    if (a.count > 0 && plan.kernel != kernel)
-      if (const int rc = launch(kernel, threads, a, false, s)) return rc;
-    kernel = plan.kernel;
-    threads = plan.threads;
-    if (add(a, t, tiles, !unit)) continue;
-    if (const int rc = launch(kernel, threads, a, false, s)) return rc;
-    (void)add(a, t, tiles, !unit);
+    const Work w = work_of(t, eight, unit);
+    if (a.count > 0 && w.plan.kernel != plan.kernel)
+      if (const int rc = launch(plan.kernel, plan.threads, a, eight, false, s)) return rc;
+    plan = w.plan;
+    if (add(a, t, w.tiles, !unit)) continue;
+    if (const int rc = launch(plan.kernel, plan.threads, a, eight, false, s)) return rc;
+    (void)add(a, t, w.tiles, !unit);
   }
-  return launch(kernel, threads, a, true, s);
+  return launch(plan.kernel, plan.threads, a, eight, true, s);
 }
 
 size_t flexsae_grad_norm_workspace_bytes(int64_t count) {
@@ -177,7 +206,7 @@ int flexsae_grad_norm(const flexsae_grad *grads, int64_t count, float *norm, voi
   };
   for (int64_t i = 0; i < count; ++i) {
     if (grads[i].n == 0) continue;
-    const int64_t tiles = ceil_div(grads[i].n, kAdamwTile);
+    const int64_t tiles = ceil_div(grads[i].n, kNormTile);
     if (a.count == kNormTensors)
       if (const int rc = launch_norm()) return rc;
     a.tensor[a.count] = {grads[i].grad, grads[i].n, grads[i].dtype};
