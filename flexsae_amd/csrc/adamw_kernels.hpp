@@ -43,15 +43,9 @@ struct AdamwTable {
   int32_t count;
   uint32_t per_block;  // consecutive tiles of a block
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, inv_scale, max_norm;
-  int32_t counting;  // who counts the step (kCounted*)
-  double log_beta1, log_beta2;
   const float *grad_norm, *lr;  // device (NULL: none)
-  int64_t *counter;             // device: steps taken; and a word to work with
+  const float2 *bias;           // device: 1 / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
-// Every block needs the number of the step, so nobody may count it before all have read it.  A launch of few blocks has its last
-// one do it, known by a ticket that each draws at its end; tickets come at 160 a microsecond, which a launch of many blocks would
-// wait for (148 000 of them: 1.8 ms instead of 0.7), so there a kernel of one thread before the first launch counts.
-enum { kNotCountedYet = 0, kCountedByTicket = 1, kCountedBefore = 2 };
 static_assert(sizeof(AdamwTable) <= 4096, "kernel arguments");
 
 struct AdamwCoefs {
@@ -85,28 +79,22 @@ __device__ __forceinline__ AdamwCoefs adamw_coefs(const AdamwTable &a) {
     c.go = __builtin_isfinite(norm);
     if (a.max_norm > 0.f) c.grad *= fminf(1.f, a.max_norm / (norm * a.inv_scale + 1e-6f));
   }
-  const double t = static_cast<double>(a.counter[0] + (a.counting == kCountedBefore ? 0 : 1));
+  const float2 bias = *a.bias;
   c.lr = a.lr ? *a.lr : 1.f;
-  c.inv_bc1 = c.lr / one_minus_power(t, a.log_beta1);
-  c.inv_sqrt_bc2 = 1.f / sqrtf(one_minus_power(t, a.log_beta2));
+  c.inv_bc1 = bias.x * c.lr;
+  c.inv_sqrt_bc2 = bias.y;
   return c;
 }
 
-// The end of a block.
-__device__ __forceinline__ void adamw_count(const AdamwTable &a) {
-  if (a.counting != kCountedByTicket) return;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    unsigned long long *ended = reinterpret_cast<unsigned long long *>(a.counter + 1);
-    if (atomicAdd(ended, 1ull) + 1 == gridDim.x) {
-      atomicExch(ended, 0ull);
-      a.counter[0] += 1;
-    }
-  }
-}
-
-__global__ void adamw_count_kernel(int64_t *counter, const float *grad_norm) {
-  if (!grad_norm || __builtin_isfinite(*grad_norm)) counter[0] += 1;
+// Every block needs the number of the step, so none may count it before all have read it: a kernel of one thread does, before the
+// first of a call, and leaves what depends on the number in the word beside it.  (Tickets of blocks that end, the last of which
+// counts, come at 160 a microsecond: at 148 000 blocks 1.8 ms instead of 0.6.)
+__global__ void adamw_count_kernel(int64_t *counter, const float *grad_norm, double log_beta1, double log_beta2) {
+  if (grad_norm && !__builtin_isfinite(*grad_norm)) return;
+  const int64_t steps = counter[0] + 1;
+  counter[0] = steps;
+  const double t = static_cast<double>(steps);
+  *reinterpret_cast<float2 *>(counter + 1) = float2{1.f / one_minus_power(t, log_beta1), 1.f / sqrtf(one_minus_power(t, log_beta2))};
 }
 
 // The tensor of a tile: the largest i with first[i] <= tile (tensors without tiles are not in the table).
@@ -317,62 +305,83 @@ __device__ __forceinline__ T across_lanes(T x, F join) {
 
 // What a maximum is kept as: zero below the smallest normal number (its inverse would overflow), NaN where the block has
 // infinities or NaN.
-__device__ __forceinline__ float kept_max(uint32_t bits) {
-  return bits < 0x00800000u ? 0.f : bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(bits);
+__device__ __forceinline__ float kept_max(float a, bool bad) {
+  return bad ? __uint_as_float(0x7fc00000u) : a < 0x1p-126f ? 0.f : a;
 }
 
-// The maxima of a block that LANES lanes hold.  As whole numbers: the bits of non-negative floats are in their order, infinity and
-// NaN above all.
+// The maxima of a block that LANES lanes hold; a_m comes in as what it was.  v's as whole numbers: the bits of non-negative floats
+// are in their order, infinity and NaN above all.  m has infinities or NaN where v has, or had NaN before, which is why the
+// floating-point maximum, which passes over NaN, is enough.
 template <int LANES, int N>
 __device__ __forceinline__ void maxima(const float (&m)[N], const float (&v)[N], float &a_m, float &a_v) {
-  auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
-  uint32_t bm = 0, bv = 0;
+  uint32_t bv = 0;
+  float bm = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    bm = max(bm, __float_as_uint(m[j]) & 0x7fffffffu);
-    bv = max(bv, __float_as_uint(v[j]) & 0x7fffffffu);
+    bm = fmaxf(bm, fabsf(m[j]));
+    bv = max(bv, __float_as_uint(v[j]));
   }
-  a_m = kept_max(across_lanes<LANES>(bm, larger));
-  a_v = kept_max(across_lanes<LANES>(bv, larger));
+  bm = across_lanes<LANES>(bm, [](float x, float y) { return fmaxf(x, y); });
+  bv = across_lanes<LANES>(bv, [](uint32_t x, uint32_t y) { return max(x, y); });
+  const bool bad = bv >= 0x7f800000u;
+  a_m = kept_max(bm, bad || a_m != a_m);
+  a_v = kept_max(__uint_as_float(bv), bad);
 }
 
-// Codes of two elements, (m, v) each, from |m| / a_m and v / a_v.  They are what correctly rounded roots give, whatever unit
-// computes them: EXACT takes such roots.  The hardware's are off by a unit in the last place each, which matters within kTie of
-// the middle between two codes only (2^-23 of 255 for the outer root, half of it for the inner one, and the products' rounding);
-// otherwise `root_m` = sqrt(|m| / a_m) and `root_v` = sqrt(v / a_v) come from there, and the result is the largest distance from a code.
+// Codes of two elements, (m, v) each, from |m| / a_m and v / a_v: whole numbers nearest to 127 sqrt and 255 sqrt sqrt of them, as
+// correctly rounded operations give them, whatever unit computes them.  EXACT: such operations.  Otherwise the hardware's roots,
+// `root_v` = sqrt(v) sqrt(1 / a_v) among them, off by a unit in the last place each: with the roundings on either side 2.5e-7 of
+// the result for m and 5.5e-7 for v.  Both ends of that stretch are rounded; where they are not the same, true comes back.
 // Adding kMagic rounds to a whole number, which then stands in the low bits.
-constexpr float kTie = 7e-5f;
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+constexpr float kOffM = 2.5e-7f, kOffV = 5.5e-7f;
 
 template <bool EXACT>
-__device__ __forceinline__ float codes_of_two(const float *m, const float *v, float per_m, float per_v, const float *root_v, uint32_t &w) {
+__device__ __forceinline__ bool codes_of_two(const float *m, const float *v, float per_m, float per_v, float root_per_v,
+                                             const float *s, uint32_t &w) {
 #pragma clang fp contract(off)
-  auto root = [](float x) { return EXACT ? sqrtf(x) : __builtin_amdgcn_sqrtf(x); };
-  float off = 0.f;
-  uint32_t pair[2];
+  uint32_t pair[2], differ = 0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const float x = copysignf(root(fabsf(m[k]) * per_m) * 127.f, m[k]), rx = x + (kMagic + 128.f);
-    const float q = EXACT ? sqrtf(v[k] * per_v) : root_v[k];
-    const float y = root(q) * 255.f, ry = y + kMagic;
-    if constexpr (!EXACT) off = fmaxf(off, fmaxf(fabsf(x - (rx - (kMagic + 128.f))), fabsf(y - (ry - kMagic))));
+    float x, y, q;
+    if constexpr (EXACT) {
+      x = copysignf(sqrtf(fabsf(m[k]) * per_m) * 127.f, m[k]) + (kMagic + 128.f);
+      q = v[k] * per_v;
+      y = sqrtf(sqrtf(q)) * 255.f + kMagic;
+    } else {
+      q = s[k] * root_per_v;
+      const float rm = copysignf(__builtin_amdgcn_sqrtf(fabsf(m[k]) * per_m), m[k]), rv = __builtin_amdgcn_sqrtf(q);
+      x = fmaf(rm, 127.f * (1.f + kOffM), kMagic + 128.f);
+      y = fmaf(rv, 255.f * (1.f + kOffV), kMagic);
+      differ |= (__float_as_uint(x) ^ __float_as_uint(fmaf(rm, 127.f * (1.f - kOffM), kMagic + 128.f))) |
+                (__float_as_uint(y) ^ __float_as_uint(fmaf(rv, 255.f * (1.f - kOffV), kMagic)));
+    }
     // (a v above zero never becomes zero)
-    const uint32_t cv = max(__float_as_uint(ry) & 0xffu, min(__float_as_uint(q), 1u));
-    pair[k] = __builtin_amdgcn_perm(cv, __float_as_uint(rx), 0x0c0c0400u);
+    uint32_t least;
+    asm("v_min_u32 %0, 1, %1" : "=v"(least) : "v"(q));
+    pair[k] = __builtin_amdgcn_perm(max(__float_as_uint(y) & 0xffu, least), __float_as_uint(x), 0x0c0c0400u);
   }
   w = pair[0] | (pair[1] << 16);
-  return off;
+  return differ != 0;
+}
+
+// 1 / a of a positive normal number, rounded once: a reciprocal, its error put right, and the exponent by itself (the result may
+// lie below the normal numbers).
+__device__ __forceinline__ float inverse(float a) {
+  const float x = __builtin_amdgcn_frexp_mantf(a), r = __builtin_amdgcn_rcpf(x);
+  return __builtin_amdgcn_ldexpf(fmaf(r, fmaf(-x, r, 1.f), r), -__builtin_amdgcn_frexp_expf(a));
 }
 
 // s: the hardware's square roots of v
 template <int N>
 __device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], const float (&s)[N], float a_m, float a_v, Codes<N> &c) {
-  const float per_m = a_m > 0.f ? 1.f / a_m : 0.f, per_v = a_v > 0.f ? 1.f / a_v : 0.f, root_per_v = sqrtf(per_v);
+  const float per_m = a_m > 0.f ? inverse(a_m) : 0.f, per_v = a_v > 0.f ? inverse(a_v) : 0.f;
+  const float root_per_v = __builtin_amdgcn_sqrtf(per_v);
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
-    const float root_v[2] = {s[j] * root_per_v, s[j + 1] * root_per_v};
-    const float off = codes_of_two<false>(m + j, v + j, per_m, per_v, root_v, c.w[j / 2]);
-    if (__any(off > 0.5f - kTie)) (void)codes_of_two<true>(m + j, v + j, per_m, per_v, root_v, c.w[j / 2]);
+    // (one wavefront in 40 has such an element)
+    const bool near = codes_of_two<false>(m + j, v + j, per_m, per_v, root_per_v, s + j, c.w[j / 2]);
+    if (__any(near)) (void)codes_of_two<true>(m + j, v + j, per_m, per_v, root_per_v, s + j, c.w[j / 2]);
   }
 }
 
@@ -448,7 +457,7 @@ struct AdamwUnit {
     adamw_move(c, t.lr * c.inv_bc1, 1.f - t.lr * c.lr * t.weight_decay, m, s, w);
     if constexpr (STORE && EIGHT) {
       constexpr int kLanes = LANES < kQuantLanes ? LANES : kQuantLanes;
-      float a_m, a_v;
+      float a_m = top.x, a_v;
       maxima<kLanes>(m, v, a_m, a_v);
       Codes<N> now;
       encode(m, v, s, a_m, a_v, now);
@@ -501,8 +510,10 @@ __device__ __forceinline__ void adamw_tile(const AdamwTensor &t, int64_t base, c
     float g[N], w[N];
     unpack(unit[u].rg, g);
     unpack(unit[u].rw, w);
+    if (c.grad != 1.f) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) g[j] *= c.grad;
+      for (int j = 0; j < N; ++j) g[j] *= c.grad;
+    }
     unit[u].template step<true, kWave>(t, c, place(u), g, w);
     unit[u].store(t, place(u), w);
   }
@@ -526,7 +537,6 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_kernel(const AdamwTable a
     if (base + kAdamwTile <= t.cols) tile_of(std::true_type{});
     else tile_of(std::false_type{});
   }
-  adamw_count(a);
 }
 
 // Sums over a row that LANES lanes of a wavefront, or WAVES wavefronts of a block, hold; `turn` alternates between two places so
@@ -544,15 +554,19 @@ __device__ __forceinline__ float row_sum(float x, float (*place)[16], int turn) 
   return x;
 }
 
+// (blocks of eight wavefronts and more: registers for two of them on a compute unit)
+constexpr int rows_threads(int waves) { return waves < 4 ? 256 : waves * kWave; }
+
 // Rows of length one.  LANES (64 at least with more than one) of each of WAVES wavefronts hold a row, UNITS units of elements each,
 // in registers: every tensor is read and written once.  UNITS = 0: a row of any length is walked three times (the two products;
 // the length of the moved row; the step), nothing stored before the last walk.
 template <typename T, bool MASTER, bool EIGHT, int WAVES, int LANES, int UNITS>
-__global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * kWave) void adamw_rows_kernel(const AdamwTable a) {
+__global__ __launch_bounds__(rows_threads(WAVES), WAVES < 8 ? 1 : 4) void adamw_rows_kernel(const AdamwTable a) {
   static_assert(LANES == kWave || (WAVES == 1 && UNITS == 1), "less than a wavefront: one unit");
   using Unit = AdamwUnit<T, MASTER, EIGHT>;
   constexpr int N = Unit::N, kStretch = LANES * N;
-  constexpr int kRows = WAVES < 4 ? 4 / WAVES * (kWave / LANES) : 1;  // of a block at a time
+  static_assert(WAVES == 1 || WAVES >= 4, "a block has a barrier only where it holds one row");
+  constexpr int kRows = rows_threads(WAVES) / (WAVES * LANES);  // of a block at a time
   __shared__ float place[2][16];
   const AdamwCoefs c = adamw_coefs(a);
   if (!c.go) return;
@@ -657,7 +671,6 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * kWave) void adamw_rows_ke
     // (the next row's first sum may write place[0] while a wavefront still reads it for this one's length)
     if constexpr (WAVES > 1) __syncthreads();
   }
-  adamw_count(a);
 }
 
 // ---- the gradients' norm -------------------------------------------------------------------
@@ -752,26 +765,49 @@ struct MomentsTable {
 };
 static_assert(sizeof(MomentsTable) <= 4096, "kernel arguments");
 
-// A tile is 2048 elements of one row.
+// A tile is 2048 elements of the flattened tensor, wherever rows end.
 template <typename T>
 __global__ __launch_bounds__(kAdamwThreads) void adamw8_moments_kernel(const MomentsTable a) {
   constexpr int N = 16 / static_cast<int>(sizeof(typename Traits<T>::store_t));
   for (uint32_t tile = blockIdx.x; tile < a.first[a.count]; tile += gridDim.x) {
     const int i = tensor_of(a, tile);
     const MomentsTensor &t = a.tensor[i];
-    const int64_t per_row = (t.cols + kAdamwTile - 1) / kAdamwTile, blocks = (t.cols + kAdamwQuant - 1) / kAdamwQuant;
-    const int64_t row = (tile - a.first[i]) / per_row, part = (tile - a.first[i]) % per_row;
+    const int64_t base = static_cast<int64_t>(tile - a.first[i]) * kAdamwTile, blocks = (t.cols + kAdamwQuant - 1) / kAdamwQuant;
+    const int64_t row = t.rows == 1 ? 0 : base / t.cols, from = base - row * t.cols;
+    const float2 *const top = reinterpret_cast<const float2 *>(t.maxima) + row * blocks;
 #pragma unroll
     for (int u = 0; u < kAdamwTile / (kAdamwThreads * N); ++u) {
-      const int64_t from = part * kAdamwTile;
-      const uint32_t col = (u * kAdamwThreads + threadIdx.x) * N;
-      const Place at = {row * t.cols + from, row * blocks + from / kAdamwQuant, col, upto<N>(t.cols - from - col)};
+      const uint32_t offset = (u * kAdamwThreads + threadIdx.x) * N;
+      const Place at = {base, 0, offset, upto<N>(t.rows * t.cols - base - offset)};
       if (at.left == 0) continue;
+      // the lane's row, counted from the tile's first, and column
+      int64_t col = from + offset;
+      uint32_t r = 0;
+      if (col >= t.cols) {
+        r = t.cols >= 2 * kAdamwTile ? 1u : static_cast<uint32_t>(col) / static_cast<uint32_t>(t.cols);
+        col -= r * t.cols;
+      }
       Codes<N> codes;
       load_codes(t.codes, at, codes);
-      const float2 top = reinterpret_cast<const float2 *>(t.maxima)[at.block + col / kAdamwQuant];
       float m[N], v[N];
-      decode(codes, top.x, top.y, m, v);
+      if (col % kAdamwQuant + at.left <= kAdamwQuant && col + at.left <= t.cols) {
+        const float2 x = top[r * blocks + col / kAdamwQuant];
+        decode(codes, x.x, x.y, m, v);
+      } else {  // more than one block
+        decode(codes, 1.f, 1.f, m, v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (j >= at.left) break;
+          if (col == t.cols) {
+            col = 0;
+            ++r;
+          }
+          const float2 x = top[r * blocks + col / kAdamwQuant];
+          m[j] *= x.x;
+          v[j] *= x.y;
+          ++col;
+        }
+      }
       store_upto<T>(t.m, at, m);
       store_upto<T>(t.v, at, v);
     }

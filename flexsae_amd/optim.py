@@ -89,8 +89,7 @@ def grad_norm(grads: Sequence[Tensor]) -> Tensor:
 
 
 def adamw_counter(device=None, steps: int = 0) -> Tensor:
-    """The ``counter`` of a step's calls: int64[2] on the device, the number of steps taken and a word that the calls work with
-    (zero between them)."""
+    """The ``counter`` of a step's calls: int64[2] on the device, the number of steps taken, and a word that the calls work with."""
     return torch.tensor([steps, 0], dtype=torch.int64, device="cuda" if device is None else device)
 
 

@@ -520,7 +520,7 @@ typedef struct {
   float max_norm;         /* 0: no clipping; else gradients are multiplied by min(1, max_norm / (norm / grad_scale + 1e-6)) */
   const float *grad_norm; /* device, of the gradients as they are, or NULL.  Not finite: the call changes nothing */
   const float *lr;        /* device, or NULL: a factor of every tensor's lr (schedules of captured graphs) */
-  int64_t *counter;       /* device, [2]: steps taken, which the call counts up; and a zero that it works with */
+  int64_t *counter;       /* device, [2]: steps taken, which the call counts up; and a word that it works with */
   int32_t state_bits;     /* 32 or 8 */
   int32_t flags;
 } flexsae_adamw_config;
