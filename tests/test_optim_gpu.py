@@ -627,3 +627,19 @@ def test_refusals():
             flex.adamw8_moments(codes, absmax)
     with pytest.raises(TypeError):
         flex.adamw8_moments([p.s0[0]], [p.s1[0]], torch.float64)
+
+
+@pytest.mark.parametrize("bits,dtype", [(32, F32), (8, BF16), (8, F16)])
+def test_the_example(bits, dtype):
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_sae.py")
+    spec = importlib.util.spec_from_file_location("train_sae", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, model, opt = example.train(F=512, D=64, K=8, B=128, steps=60, bits=bits, dtype=dtype, lr=3e-3)
+    assert losses[-1] < 0.8 * losses[0]
+    # (rounding a row of length one to 16 bits moves its length by less than the rounding of a number)
+    assert float((model.W_dec.detach().double().norm(dim=1) - 1).abs().max()) < {F32: 1e-5, BF16: 2.0 ** -8, F16: 2.0 ** -11}[dtype]
+    assert int(opt.state[model.W_dec]["counter"][0]) == 60
