@@ -22,8 +22,8 @@ namespace flexsae {
 constexpr int kAdamwThreads = 256;
 constexpr int kAdamwTile = 2048;                           // elements of a block at a time
 constexpr int kAdamwQuant = 256;                           // elements that share the maxima of 8-bit states
-constexpr int kAdamwTensors = 48;                          // of one launch: the table travels in the kernel's arguments (4 KiB)
-constexpr int kNormTensors = 128;
+constexpr int kAdamwTensors = 66;                          // of one launch: the table travels in the kernel's arguments (4 KiB)
+constexpr int kNormTensors = 200;
 constexpr int kNormTile = 8192;
 constexpr int kNormSums = 4;  // of a thread
 
@@ -32,10 +32,15 @@ struct AdamwTensor {
   const void *grad;
   void *s0, *s1;  // exp_avg, exp_avg_sq; or codes, maxima
   float *master;  // (NULL: none)
-  int64_t rows, cols;
+  uint64_t size;  // elements and type (sized); unit rows: columns in the high word, rows in the low one
   float lr, weight_decay;
-  int32_t dtype;
 };
+
+// A number of elements (at most 2^40) and a flexsae_dtype in one word.
+constexpr int kDtypeBit = 56;
+constexpr uint64_t sized(int64_t n, int dtype) { return static_cast<uint64_t>(n) | (static_cast<uint64_t>(dtype) << kDtypeBit); }
+__device__ __forceinline__ int64_t elements(uint64_t size) { return static_cast<int64_t>(size & ((uint64_t{1} << kDtypeBit) - 1)); }
+__device__ __forceinline__ int dtype_of(uint64_t size) { return static_cast<int>(size >> kDtypeBit); }
 
 struct AdamwTable {
   AdamwTensor tensor[kAdamwTensors];
@@ -102,7 +107,7 @@ template <typename Table>
 __device__ __forceinline__ int tensor_of(const Table &a, uint32_t tile) {
   int i = 0;
 #pragma unroll
-  for (int s = 64; s > 0; s >>= 1)
+  for (int s = 128; s > 0; s >>= 1)
     if (i + s < a.count && tile >= a.first[i + s]) i += s;
   return i;
 }
@@ -501,7 +506,7 @@ __device__ __forceinline__ void adamw_tile(const AdamwTensor &t, int64_t base, c
   Unit unit[kUnits];
   auto place = [&](int u) -> Place {
     const uint32_t col = (u * kAdamwThreads + threadIdx.x) * N;
-    return {base, base / kAdamwQuant, col, FULL ? N : upto<N>(t.cols - base - col)};
+    return {base, base / kAdamwQuant, col, FULL ? N : upto<N>(elements(t.size) - base - col)};
   };
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) unit[u].load(t, place(u));
@@ -528,13 +533,14 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_kernel(const AdamwTable a
     const int i = tensor_of(a, tile);
     const AdamwTensor &t = a.tensor[i];
     const int64_t base = static_cast<int64_t>(tile - a.first[i]) * kAdamwTile;
+    const int dtype = dtype_of(t.size);
     auto tile_of = [&](auto full) {
       constexpr bool kFull = decltype(full)::value;
-      if (t.dtype == FLEXSAE_F32) adamw_tile<float, false, EIGHT, kFull>(t, base, c);
-      else if (t.dtype == FLEXSAE_BF16) t.master ? adamw_tile<bf16_t, true, EIGHT, kFull>(t, base, c) : adamw_tile<bf16_t, false, EIGHT, kFull>(t, base, c);
+      if (dtype == FLEXSAE_F32) adamw_tile<float, false, EIGHT, kFull>(t, base, c);
+      else if (dtype == FLEXSAE_BF16) t.master ? adamw_tile<bf16_t, true, EIGHT, kFull>(t, base, c) : adamw_tile<bf16_t, false, EIGHT, kFull>(t, base, c);
       else t.master ? adamw_tile<f16_t, true, EIGHT, kFull>(t, base, c) : adamw_tile<f16_t, false, EIGHT, kFull>(t, base, c);
     };
-    if (base + kAdamwTile <= t.cols) tile_of(std::true_type{});
+    if (base + kAdamwTile <= elements(t.size)) tile_of(std::true_type{});
     else tile_of(std::false_type{});
   }
 }
@@ -575,11 +581,12 @@ __global__ __launch_bounds__(rows_threads(WAVES), WAVES < 8 ? 1 : 4) void adamw_
   for (uint32_t tile = blockIdx.x * a.per_block; tile < end; ++tile) {
     const int i = tensor_of(a, tile);
     const AdamwTensor &t = a.tensor[i];
+    const int64_t rows = static_cast<uint32_t>(t.size);
     int64_t row = static_cast<int64_t>(tile - a.first[i]) * kRows + wave_in_block() / WAVES * (kWave / LANES);
-    if (row >= t.rows) continue;  // (of a whole wavefront: a block of several rows has no barriers)
+    if (row >= rows) continue;  // (of a whole wavefront: a block of several rows has no barriers)
     if constexpr (LANES < kWave) row += lane_id() / LANES;
-    const bool live = LANES == kWave || row < t.rows;
-    const int cols = static_cast<int>(t.cols);
+    const bool live = LANES == kWave || row < rows;
+    const int cols = static_cast<int>(t.size >> 32);
     const int64_t start = row * cols, block = row * ((cols + kAdamwQuant - 1) / kAdamwQuant);
     auto stretch = [&](int u) { return (u * WAVES + wave) * kStretch; };
     auto at = [&](int u) -> Place {
@@ -676,8 +683,7 @@ __global__ __launch_bounds__(rows_threads(WAVES), WAVES < 8 ? 1 : 4) void adamw_
 // ---- the gradients' norm -------------------------------------------------------------------
 struct NormTensor {
   const void *grad;
-  int64_t n;
-  int32_t dtype;
+  uint64_t size;
 };
 // (No table here has an array of bytes beside its wider ones: an index that addresses both lets the compiler take the address of
 // a wider entry apart as base + i and 7 i, and scalar loads drop the two low bits of each part.)
@@ -726,14 +732,15 @@ __global__ __launch_bounds__(kAdamwThreads) void norm_partial_kernel(const NormT
   for (uint32_t tile = blockIdx.x; tile < a.first[a.count]; tile += gridDim.x) {
     const int i = tensor_of(a, tile);
     const NormTensor &t = a.tensor[i];
-    const int64_t base = static_cast<int64_t>(tile - a.first[i]) * kNormTile;
+    const int64_t base = static_cast<int64_t>(tile - a.first[i]) * kNormTile, n = elements(t.size);
+    const int dtype = dtype_of(t.size);
     auto tile_of = [&](auto full) {
       constexpr bool kFull = decltype(full)::value;
-      if (t.dtype == FLEXSAE_F32) squares_of_tile<float, kFull>(t.grad, t.n, base, sum);
-      else if (t.dtype == FLEXSAE_BF16) squares_of_tile<bf16_t, kFull>(t.grad, t.n, base, sum);
-      else squares_of_tile<f16_t, kFull>(t.grad, t.n, base, sum);
+      if (dtype == FLEXSAE_F32) squares_of_tile<float, kFull>(t.grad, n, base, sum);
+      else if (dtype == FLEXSAE_BF16) squares_of_tile<bf16_t, kFull>(t.grad, n, base, sum);
+      else squares_of_tile<f16_t, kFull>(t.grad, n, base, sum);
     };
-    if (base + kNormTile <= t.n) tile_of(std::true_type{});
+    if (base + kNormTile <= n) tile_of(std::true_type{});
     else tile_of(std::false_type{});
   }
   double all = 0.0;

@@ -579,8 +579,15 @@ PyObject *py_hier_sgd(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 // ---- the optimiser -------------------------------------------------------------------------
-// The tensors of a list or tuple, each one plain and of `device` (undefined: the first one's); false: not this module's business.
-bool take_tensors(PyObject *o, std::vector<Tensor> &out, c10::optional<c10::Device> &device) {
+// The tensors of a list or tuple, each plain and of `device` (undefined: the first one's); false: not this module's business.  The
+// list keeps them: these functions hold the interpreter's lock, and no reference of their own (a call of 192 tensors is
+// host work: 55 us with references, checks for forward gradients, which optim.py has made, and 48 tensors a launch).
+using Tensors = std::vector<const Tensor *>;
+bool take_tensors(PyObject *o, Tensors &out, c10::optional<c10::Device> &device) {
+  static const uint64_t usual =
+      (c10::DispatchKeySet(c10::DispatchKey::CUDA) | c10::DispatchKeySet(c10::DispatchKey::AutogradCUDA) |
+       c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView) | c10::DispatchKeySet(c10::DispatchKey::AutocastCUDA))
+          .raw_repr();
   if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
   PyObject **const items = PySequence_Fast_ITEMS(o);
@@ -588,9 +595,9 @@ bool take_tensors(PyObject *o, std::vector<Tensor> &out, c10::optional<c10::Devi
   for (Py_ssize_t i = 0; i < n; ++i) {
     if (!THPVariable_CheckExact(items[i])) return false;
     const Tensor &t = THPVariable_Unpack(items[i]);
-    if (!plain_tensor(t) || (device && t.device() != *device)) return false;
+    if (!t.defined() || !t.is_cuda() || (t.key_set().raw_repr() & ~usual) != 0 || (device && t.device() != *device)) return false;
     if (!device) device = t.device();
-    out.push_back(t);
+    out.push_back(&t);
   }
   return true;
 }
@@ -625,28 +632,29 @@ bool take_scalar(PyObject *o, const c10::Device &device, Tensor &out) {
 PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arguments(n, 1)) return nullptr;
-  std::vector<Tensor> grads;
+  Tensors grads;
   c10::optional<c10::Device> device;
   if (!plain_surroundings() || !take_tensors(args[0], grads, device) || grads.empty()) Py_RETURN_NONE;
-  for (const Tensor &g : grads)
-    if (dtype_of(g.scalar_type()) < 0) Py_RETURN_NONE;
-  Tensor norm;
-  {
-    pybind11::gil_scoped_release no_gil;
-    const c10::AutoGradMode no_grad(false);
-    const c10::DeviceGuard guard(*device);
-    std::vector<flexsae_grad> list;
-    list.reserve(grads.size());
-    for (Tensor &g : grads) {
-      if (!g.is_contiguous()) g = g.contiguous();
-      list.push_back({g.const_data_ptr(), g.numel(), dtype_of(g.scalar_type())});
+  const c10::AutoGradMode no_grad(false);
+  const c10::DeviceGuard guard(*device);
+  std::vector<flexsae_grad> list;
+  list.reserve(grads.size());
+  std::vector<Tensor> copies;
+  for (const Tensor *g : grads) {
+    const int dtype = dtype_of(g->scalar_type());
+    if (dtype < 0) Py_RETURN_NONE;
+    if (!g->is_contiguous()) {
+      copies.push_back(g->contiguous());
+      list.push_back({copies.back().const_data_ptr(), g->numel(), dtype});
+    } else {
+      list.push_back({g->const_data_ptr(), g->numel(), dtype});
     }
-    const auto count = static_cast<int64_t>(list.size());
-    const size_t bytes = lib.grad_norm_workspace_bytes(count);
-    const Tensor workspace = make_workspace(grads[0], bytes);
-    norm = make(grads[0], {}, c10::ScalarType::Float);
-    check(lib.grad_norm(list.data(), count, f32(norm), workspace.data_ptr(), bytes, stream_of(norm)), "flexsae_grad_norm");
   }
+  const auto count = static_cast<int64_t>(list.size());
+  const size_t bytes = lib.grad_norm_workspace_bytes(count);
+  const Tensor workspace = make_workspace(*grads[0], bytes);
+  const Tensor norm = make(*grads[0], {}, c10::ScalarType::Float);
+  check(lib.grad_norm(list.data(), count, f32(norm), workspace.data_ptr(), bytes, stream_of(norm)), "flexsae_grad_norm");
   return THPVariable_Wrap(norm);
   END_HANDLE_TH_ERRORS
 }
@@ -657,7 +665,7 @@ PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arguments(n, 16)) return nullptr;
   const bool eight = number(args[0]) == 8, unit = number(args[15]) != 0;
-  std::vector<Tensor> params, grads, s0, s1, masters;
+  Tensors params, grads, s0, s1, masters;
   c10::optional<c10::Device> device;
   if (!plain_surroundings() || !take_tensors(args[1], params, device) || params.empty() ||
       !take_tensors(args[2], grads, device) || !take_tensors(args[3], s0, device) || !take_tensors(args[4], s1, device) ||
@@ -667,7 +675,7 @@ PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (grads.size() != count || s0.size() != count || s1.size() != count || (args[5] != Py_None && masters.size() != count) ||
       !THPVariable_Check(args[6]))
     Py_RETURN_NONE;
-  const Tensor counter = THPVariable_Unpack(args[6]);
+  const Tensor &counter = THPVariable_Unpack(args[6]);
   if (!plain_tensor(counter) || counter.device() != *device || counter.scalar_type() != c10::ScalarType::Long ||
       counter.numel() != 2 || !changeable(counter))
     Py_RETURN_NONE;
@@ -676,34 +684,37 @@ PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if ((device_lr ? !take_scalar(args[7], *device, lr) : !reals(args[7], count)) || !reals(args[8], count) ||
       !take_scalar(args[13], *device, norm))
     Py_RETURN_NONE;
+  const c10::AutoGradMode no_grad(false);
+  const c10::DeviceGuard guard(*device);
   std::vector<flexsae_adamw_tensor> list(count);
+  std::vector<Tensor> copies;
   for (size_t i = 0; i < count; ++i) {
-    const Tensor &p = params[i];
+    const Tensor &p = *params[i], &g = *grads[i], &a = *s0[i], &b = *s1[i];
     const int dtype = dtype_of(p.scalar_type());
-    if (dtype < 0 || grads[i].scalar_type() != p.scalar_type() || grads[i].sizes() != p.sizes() || !changeable(p) ||
-        !changeable(s0[i]) || !changeable(s1[i]) || (unit && p.dim() < 2))
+    if (dtype < 0 || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || !changeable(p) || !changeable(a) ||
+        !changeable(b) || (unit && p.dim() < 2))
       Py_RETURN_NONE;
-    const int64_t cols = unit ? p.size(-1) : p.numel(), rows = unit ? (cols ? p.numel() / cols : 0) : 1;
+    const int64_t numel = p.numel(), cols = unit ? p.size(-1) : numel, rows = unit ? (cols ? numel / cols : 0) : 1;
     if (eight) {
-      const at::IntArrayRef sizes = s0[i].sizes();
-      if (s0[i].scalar_type() != c10::ScalarType::Byte || s1[i].scalar_type() != c10::ScalarType::Float ||
-          s0[i].dim() != p.dim() + 1 || sizes.back() != 2 || sizes.slice(0, sizes.size() - 1) != p.sizes() ||
-          s1[i].dim() != 3 || s1[i].size(0) != rows || s1[i].size(1) != (cols + 255) / 256 || s1[i].size(2) != 2 ||
-          reinterpret_cast<uintptr_t>(s1[i].const_data_ptr()) % 8 || reinterpret_cast<uintptr_t>(s0[i].const_data_ptr()) % 2)
+      const at::IntArrayRef sizes = a.sizes();
+      if (a.scalar_type() != c10::ScalarType::Byte || b.scalar_type() != c10::ScalarType::Float || a.dim() != p.dim() + 1 ||
+          sizes.back() != 2 || sizes.slice(0, sizes.size() - 1) != p.sizes() || b.dim() != 3 || b.size(0) != rows ||
+          b.size(1) != (cols + 255) / 256 || b.size(2) != 2 || reinterpret_cast<uintptr_t>(b.const_data_ptr()) % 8 ||
+          reinterpret_cast<uintptr_t>(a.const_data_ptr()) % 2)
         Py_RETURN_NONE;
-    } else if (s0[i].scalar_type() != c10::ScalarType::Float || s1[i].scalar_type() != c10::ScalarType::Float ||
-               s0[i].sizes() != p.sizes() || s1[i].sizes() != p.sizes()) {
+    } else if (a.scalar_type() != c10::ScalarType::Float || b.scalar_type() != c10::ScalarType::Float || a.sizes() != p.sizes() ||
+               b.sizes() != p.sizes()) {
       Py_RETURN_NONE;
     }
     void *master = nullptr;
     if (!masters.empty() && dtype != FLEXSAE_F32) {
-      if (masters[i].scalar_type() != c10::ScalarType::Float || masters[i].sizes() != p.sizes() || !changeable(masters[i]))
+      if (masters[i]->scalar_type() != c10::ScalarType::Float || masters[i]->sizes() != p.sizes() || !changeable(*masters[i]))
         Py_RETURN_NONE;
-      master = masters[i].data_ptr();
+      master = masters[i]->data_ptr();
     }
-    if (!grads[i].is_contiguous()) grads[i] = grads[i].contiguous();
+    if (!g.is_contiguous()) copies.push_back(g.contiguous());
     const auto at = static_cast<Py_ssize_t>(i);
-    list[i] = {p.data_ptr(), grads[i].const_data_ptr(), master, s0[i].data_ptr(), s1[i].data_ptr(), rows, cols,
+    list[i] = {p.data_ptr(), (g.is_contiguous() ? g : copies.back()).const_data_ptr(), master, a.data_ptr(), b.data_ptr(), rows, cols,
                device_lr ? 1.f : static_cast<float>(real_at(args[7], at)), static_cast<float>(real_at(args[8], at)), dtype};
   }
   const flexsae_adamw_config config = {real(args[9]),
@@ -716,18 +727,14 @@ PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
                                        counter.data_ptr<int64_t>(),
                                        eight ? 8 : 32,
                                        unit ? FLEXSAE_ADAMW_UNIT_ROWS : 0};
-  int status = FLEXSAE_OK;
-  {
-    pybind11::gil_scoped_release no_gil;
-    const c10::DeviceGuard guard(*device);
-    status = lib.adamw_step(list.data(), static_cast<int64_t>(count), &config, stream_of(counter));
-    if (status == FLEXSAE_OK || status == FLEXSAE_ERR_LAUNCH)  // (else nothing was launched)
-      for (const auto *changed : {&params, &s0, &s1, &masters})
-        for (const Tensor &t : *changed) torch::autograd::impl::bump_version(t);
-    if (status != FLEXSAE_ERR_INVALID_ARGUMENT) check(status, "flexsae_adamw_step");
-    torch::autograd::impl::bump_version(counter);
+  const int status = lib.adamw_step(list.data(), static_cast<int64_t>(count), &config, stream_of(counter));
+  if (status == FLEXSAE_ERR_INVALID_ARGUMENT) Py_RETURN_NONE;  // nothing was launched; optim.py says what is wrong
+  if (status == FLEXSAE_OK || status == FLEXSAE_ERR_LAUNCH) {
+    for (const auto *changed : {&params, &s0, &s1, &masters})
+      for (const Tensor *t : *changed) t->unsafeGetTensorImpl()->bump_version();
+    counter.unsafeGetTensorImpl()->bump_version();
   }
-  if (status != FLEXSAE_OK) Py_RETURN_NONE;  // optim.py says what is wrong
+  check(status, "flexsae_adamw_step");
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -737,7 +744,8 @@ PyObject *py_adamw8_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arguments(n, 3)) return nullptr;
   const int64_t dtype = number(args[2]);
-  std::vector<Tensor> codes, absmax, m, v;
+  Tensors codes, absmax;
+  std::vector<Tensor> m, v;
   c10::optional<c10::Device> device;
   if (!plain_surroundings() || !take_tensors(args[0], codes, device) || codes.empty() || !take_tensors(args[1], absmax, device) ||
       absmax.size() != codes.size() || dtype < 0 || dtype > 2)
@@ -747,7 +755,7 @@ PyObject *py_adamw8_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
                                : dtype == FLEXSAE_BF16 ? c10::ScalarType::BFloat16
                                                        : c10::ScalarType::Half;
   for (size_t i = 0; i < codes.size(); ++i) {
-    const Tensor &c = codes[i], &a = absmax[i];
+    const Tensor &c = *codes[i], &a = *absmax[i];
     if (c.scalar_type() != c10::ScalarType::Byte || a.scalar_type() != c10::ScalarType::Float || c.dim() < 1 || c.size(-1) != 2 ||
         a.dim() != 3 || a.size(2) != 2 || !c.is_contiguous() || !a.is_contiguous() ||
         reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 2 || reinterpret_cast<uintptr_t>(a.const_data_ptr()) % 8)
@@ -758,12 +766,9 @@ PyObject *py_adamw8_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
     v.push_back(make(c, c.sizes().slice(0, c.dim() - 1), type));
     list[i] = {c.const_data_ptr(), a.const_data_ptr<float>(), m[i].data_ptr(), v[i].data_ptr(), rows, cols};
   }
-  {
-    pybind11::gil_scoped_release no_gil;
-    const c10::DeviceGuard guard(*device);
-    check(lib.adamw8_moments(list.data(), static_cast<int64_t>(list.size()), static_cast<int>(dtype), stream_of(codes[0])),
-          "flexsae_adamw8_moments");
-  }
+  const c10::DeviceGuard guard(*device);
+  check(lib.adamw8_moments(list.data(), static_cast<int64_t>(list.size()), static_cast<int>(dtype), stream_of(*codes[0])),
+        "flexsae_adamw8_moments");
   auto list_of = [](const std::vector<Tensor> &tensors) {
     auto l = pybind11::reinterpret_steal<pybind11::object>(PyList_New(static_cast<Py_ssize_t>(tensors.size())));
     for (size_t i = 0; i < tensors.size(); ++i) PyList_SET_ITEM(l.ptr(), static_cast<Py_ssize_t>(i), THPVariable_Wrap(tensors[i]));

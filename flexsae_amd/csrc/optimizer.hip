@@ -18,7 +18,6 @@ int launch_status() { return hipGetLastError() == hipSuccess ? FLEXSAE_OK : FLEX
 constexpr int64_t kMostElements = int64_t{1} << 40;  // of a tensor: tiles are counted in 32 bits
 
 constexpr int64_t kMostTiles = int64_t{1} << 31;  // of a launch
-constexpr int64_t kPairTiles = 8192;  // of a launch with 8-bit states, from which on a block takes two
 constexpr int64_t kNormBlocks = 1024;  // each takes one tile after another, and leaves one partial sum
 
 unsigned blocks_for(int64_t tiles, int64_t most) { return static_cast<unsigned>(tiles < 1 ? 1 : tiles > most ? most : tiles); }
@@ -28,7 +27,7 @@ int check_tensor(const flexsae_adamw_tensor &t, const flexsae_adamw_config &c) {
   if (t.rows < 0 || t.cols < 0 || !valid_dtype(t.dtype)) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (!(t.lr >= 0.f) || !(t.weight_decay >= 0.f)) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (t.rows == 0 || t.cols == 0) return FLEXSAE_OK;
-  if (t.rows > kMostElements / t.cols || (unit && t.cols >= (int64_t{1} << 29))) return FLEXSAE_ERR_UNSUPPORTED;
+  if (t.rows > kMostElements / t.cols || (unit && (t.cols >= (int64_t{1} << 29) || t.rows >= (int64_t{1} << 32)))) return FLEXSAE_ERR_UNSUPPORTED;
   if (!t.param || !t.grad || !t.state0 || !t.state1) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (t.master && t.dtype == FLEXSAE_F32) return FLEXSAE_ERR_INVALID_ARGUMENT;
   const size_t es = dtype_size(t.dtype);
@@ -107,22 +106,22 @@ RowPlan row_plan(const flexsae_adamw_tensor &t) {
 // Adds a tensor of `tiles` tiles; false: the table is full.
 bool add(AdamwTable &a, const flexsae_adamw_tensor &t, int64_t tiles, bool flat) {
   if (a.count == kAdamwTensors || a.first[a.count] + tiles > kMostTiles) return false;
-  a.tensor[a.count] = {t.param, t.grad, t.state0, t.state1, static_cast<float *>(t.master), flat ? 1 : t.rows,
-                       flat ? t.rows * t.cols : t.cols, t.lr, t.weight_decay, t.dtype};
+  a.tensor[a.count] = {t.param, t.grad, t.state0, t.state1, static_cast<float *>(t.master),
+                       flat ? sized(t.rows * t.cols, t.dtype) : static_cast<uint64_t>(t.cols) << 32 | static_cast<uint64_t>(t.rows),
+                       t.lr, t.weight_decay};
   a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(tiles);
   ++a.count;
   return true;
 }
 
 // A tile is a block's work: blocks that loop over the chip-wide grid reach 4.3 TB/s where one after another in memory's order
-// they reach 5.7 (302M bf16 parameters with masters).  With 8-bit states arithmetic counts too, and where there are blocks enough
-// two tiles share what a block does once: 534 instead of 571 us (302M bf16 parameters).  Not rows: 121 and 123 us (40M bf16).
-int launch(const RowPlan &plan, AdamwTable &a, bool pairs, hipStream_t stream) {
+// they reach 5.7 (302M bf16 parameters with masters), and two or four tiles in a row are slower too (2.1e9 bf16 parameters with
+// 8-bit states: 3646 us, 3892, 3946).
+int launch(const RowPlan &plan, AdamwTable &a, hipStream_t stream) {
   const int64_t tiles = a.first[a.count];
   if (tiles == 0) return FLEXSAE_OK;
-  a.per_block = pairs && tiles > kPairTiles ? 2 : 1;
   const int64_t most = (int64_t{1} << 31) / plan.threads;  // (a grid's threads are counted in 32 bits)
-  if (ceil_div(tiles, a.per_block) > most) a.per_block = static_cast<uint32_t>(ceil_div(tiles, most));
+  a.per_block = static_cast<uint32_t>(ceil_div(tiles, most));
   plan.kernel<<<static_cast<unsigned>(ceil_div(tiles, a.per_block)), plan.threads, 0, stream>>>(a);
   a.count = 0;
   return launch_status();
@@ -165,13 +164,13 @@ int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const
     if (t.rows == 0 || t.cols == 0) continue;
     const Work w = work_of(t, eight, unit);
     if (a.count > 0 && w.plan.kernel != plan.kernel)
-      if (const int rc = launch(plan, a, eight && !unit, s)) return rc;
+      if (const int rc = launch(plan, a, s)) return rc;
     plan = w.plan;
     if (add(a, t, w.tiles, !unit)) continue;
-    if (const int rc = launch(plan, a, eight && !unit, s)) return rc;
+    if (const int rc = launch(plan, a, s)) return rc;
     (void)add(a, t, w.tiles, !unit);
   }
-  return launch(plan, a, eight && !unit, s);
+  return launch(plan, a, s);
 }
 
 size_t flexsae_grad_norm_workspace_bytes(int64_t count) {
@@ -210,7 +209,7 @@ int flexsae_grad_norm(const flexsae_grad *grads, int64_t count, float *norm, voi
     const int64_t tiles = ceil_div(grads[i].n, kNormTile);
     if (a.count == kNormTensors)
       if (const int rc = launch_norm()) return rc;
-    a.tensor[a.count] = {grads[i].grad, grads[i].n, grads[i].dtype};
+    a.tensor[a.count] = {grads[i].grad, sized(grads[i].n, grads[i].dtype)};
     a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(tiles);
     ++a.count;
   }
