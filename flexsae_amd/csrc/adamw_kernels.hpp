@@ -687,13 +687,16 @@ struct NormTensor {
 };
 // (No table here has an array of bytes beside its wider ones: an index that addresses both lets the compiler take the address of
 // a wider entry apart as base + i and 7 i, and scalar loads drop the two low bits of each part.)
+// TENSORS: a launch with four kilobytes of arguments takes the host a microsecond longer than one with few.
+template <int TENSORS>
 struct NormTable {
-  NormTensor tensor[kNormTensors];
-  uint32_t first[kNormTensors + 1];
+  NormTensor tensor[TENSORS];
+  uint32_t first[TENSORS + 1];
   int32_t count;
   double *partial;  // one of each block
 };
-static_assert(sizeof(NormTable) <= 4096, "kernel arguments");
+constexpr int kNormFew = 8;
+static_assert(sizeof(NormTable<kNormTensors>) <= 4096, "kernel arguments");
 
 // Squares are summed in 64 bits: those of finite 32-bit numbers neither overflow nor vanish there, and the order of the sum,
 // which is the same on every run, hardly matters.
@@ -727,7 +730,8 @@ __device__ __forceinline__ double block_sum(double x) {
   return x;
 }
 
-__global__ __launch_bounds__(kAdamwThreads) void norm_partial_kernel(const NormTable a) {
+template <int TENSORS>
+__global__ __launch_bounds__(kAdamwThreads) void norm_partial_kernel(const NormTable<TENSORS> a) {
   double sum[kNormSums] = {};
   for (uint32_t tile = blockIdx.x; tile < a.first[a.count]; tile += gridDim.x) {
     const int i = tensor_of(a, tile);

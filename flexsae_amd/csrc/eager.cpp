@@ -652,9 +652,9 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
   const auto count = static_cast<int64_t>(list.size());
   const size_t bytes = lib.grad_norm_workspace_bytes(count);
-  const Tensor workspace = make_workspace(*grads[0], bytes);
+  const c10::DataPtr workspace = c10::GetAllocator(c10::DeviceType::CUDA)->allocate(bytes);  // (of the current stream, as tensors')
   const Tensor norm = make(*grads[0], {}, c10::ScalarType::Float);
-  check(lib.grad_norm(list.data(), count, f32(norm), workspace.data_ptr(), bytes, stream_of(norm)), "flexsae_grad_norm");
+  check(lib.grad_norm(list.data(), count, f32(norm), workspace.get(), bytes, stream_of(norm)), "flexsae_grad_norm");
   return THPVariable_Wrap(norm);
   END_HANDLE_TH_ERRORS
 }

@@ -18,6 +18,12 @@ int launch_status() { return hipGetLastError() == hipSuccess ? FLEXSAE_OK : FLEX
 constexpr int64_t kMostElements = int64_t{1} << 40;  // of a tensor: tiles are counted in 32 bits
 
 constexpr int64_t kMostTiles = int64_t{1} << 31;  // of a launch
+// Large steps with 32-bit states ask for LDS that they do not use, so that two blocks share a compute unit instead of eight: fewer
+// places of memory under way at once.  TB/s with two / eight: 20M fp32 parameters 5.70 / 5.65, 40M 5.88 / 5.76, 320M 5.94 / 5.60,
+// 320M bf16 ones with masters 5.96 / 5.64.  Steps that have arithmetic to hide lose by it (302M bf16 parameters with 8-bit states:
+// 818 / 508 us; rows of 1538 columns 5.10 / 5.31 TB/s).
+constexpr int64_t kStreamTiles = 16384;
+constexpr size_t kTwoBlocks = 79 << 10;  // of 160 KiB
 constexpr int64_t kNormBlocks = 1024;  // each takes one tile after another, and leaves one partial sum
 
 unsigned blocks_for(int64_t tiles, int64_t most) { return static_cast<unsigned>(tiles < 1 ? 1 : tiles > most ? most : tiles); }
@@ -120,9 +126,10 @@ bool add(AdamwTable &a, const flexsae_adamw_tensor &t, int64_t tiles, bool flat)
 int launch(const RowPlan &plan, AdamwTable &a, hipStream_t stream) {
   const int64_t tiles = a.first[a.count];
   if (tiles == 0) return FLEXSAE_OK;
+  const size_t lds = plan.kernel == adamw_kernel<false> && tiles > kStreamTiles ? kTwoBlocks : 0;
   const int64_t most = (int64_t{1} << 31) / plan.threads;  // (a grid's threads are counted in 32 bits)
   a.per_block = static_cast<uint32_t>(ceil_div(tiles, most));
-  plan.kernel<<<static_cast<unsigned>(ceil_div(tiles, a.per_block)), plan.threads, 0, stream>>>(a);
+  plan.kernel<<<static_cast<unsigned>(ceil_div(tiles, a.per_block)), plan.threads, lds, stream>>>(a);
   a.count = 0;
   return launch_status();
 }
@@ -136,6 +143,29 @@ Work work_of(const flexsae_adamw_tensor &t, bool eight, bool unit) {
   if (!unit) return {{eight ? adamw_kernel<true> : adamw_kernel<false>, kAdamwThreads, 1}, ceil_div(t.rows * t.cols, kAdamwTile)};
   const RowPlan plan = eight ? row_plan<true>(t) : row_plan<false>(t);
   return {plan, ceil_div(t.rows, plan.rows)};
+}
+
+// Partial sums of all gradients: `sums` of them.
+template <int TENSORS>
+int launch_norms(const flexsae_grad *grads, int64_t count, double *partial, int64_t &sums, hipStream_t stream) {
+  NormTable<TENSORS> a;
+  a.count = 0;
+  a.first[0] = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (grads[i].n > 0) {
+      a.tensor[a.count] = {grads[i].grad, sized(grads[i].n, grads[i].dtype)};
+      a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(ceil_div(grads[i].n, kNormTile));
+      ++a.count;
+    }
+    if (a.count == 0 || (a.count < TENSORS && i + 1 < count)) continue;
+    a.partial = partial + sums;
+    const unsigned blocks = blocks_for(a.first[a.count], kNormBlocks);
+    norm_partial_kernel<TENSORS><<<blocks, kAdamwThreads, 0, stream>>>(a);
+    if (const int rc = launch_status()) return rc;
+    sums += blocks;
+    a.count = 0;
+  }
+  return FLEXSAE_OK;
 }
 
 }  // namespace
@@ -193,28 +223,8 @@ int flexsae_grad_norm(const flexsae_grad *grads, int64_t count, float *norm, voi
   const hipStream_t s = static_cast<hipStream_t>(stream);
   double *const partial = static_cast<double *>(workspace);
   int64_t sums = 0;
-  NormTable a;
-  a.count = 0;
-  a.first[0] = 0;
-  auto launch_norm = [&]() {
-    a.partial = partial + sums;
-    const unsigned blocks = blocks_for(a.first[a.count], kNormBlocks);
-    norm_partial_kernel<<<blocks, kAdamwThreads, 0, s>>>(a);
-    sums += blocks;
-    a.count = 0;
-    return launch_status();
-  };
-  for (int64_t i = 0; i < count; ++i) {
-    if (grads[i].n == 0) continue;
-    const int64_t tiles = ceil_div(grads[i].n, kNormTile);
-    if (a.count == kNormTensors)
-      if (const int rc = launch_norm()) return rc;
-    a.tensor[a.count] = {grads[i].grad, sized(grads[i].n, grads[i].dtype)};
-    a.first[a.count + 1] = a.first[a.count] + static_cast<uint32_t>(tiles);
-    ++a.count;
-  }
-  if (a.count > 0)
-    if (const int rc = launch_norm()) return rc;
+  const int rc = count <= kNormFew ? launch_norms<kNormFew>(grads, count, partial, sums, s) : launch_norms<kNormTensors>(grads, count, partial, sums, s);
+  if (rc) return rc;
   norm_finish_kernel<<<1, kAdamwThreads, 0, s>>>(partial, sums, norm);
   return launch_status();
 }

@@ -360,24 +360,32 @@ class AdamW(torch.optim.Optimizer):
         return s
 
     def _cohorts(self, group):
-        """Lists of the group's parameters with gradients that have taken the same steps.  A parameter that now has none stays
-        behind: the count of those it was stepped with goes on without it."""
-        cohorts, behind, new, device = {}, {}, {}, None
-        state = self.state
+        """What a step takes of the group: (params, grads, moments, masters, counter) of the parameters with gradients that have
+        taken the same steps.  A parameter that now has none stays behind: the count of those it was stepped with goes on
+        without it."""
+        cohorts, behind, new, state = {}, {}, {}, self.state
+        first, second = ("exp_avg", "exp_avg_sq") if group["state_bits"] == 32 else ("codes", "absmax")
         for p in group["params"]:
-            s = state.get(p)
-            if p.grad is None:
+            g, s = p.grad, state.get(p)
+            if g is None:
                 if s:
                     behind.setdefault(id(s["counter"]), []).append(s)
                 continue
-            if p.grad.is_sparse:
-                raise RuntimeError("AdamW takes dense gradients")
             if not s:
-                device = p.device
-                if device not in new:
-                    new[device] = adamw_counter(device)
-                s = state[p] = self._new_state(p, group, new[device])
-            cohorts.setdefault(id(s["counter"]), []).append((p, s))
+                if g.is_sparse:
+                    raise RuntimeError("AdamW takes dense gradients")
+                if p.device not in new:
+                    new[p.device] = adamw_counter(p.device)
+                s = state[p] = self._new_state(p, group, new[p.device])
+            counter = s["counter"]
+            cohort = cohorts.get(id(counter))
+            if cohort is None:
+                cohort = cohorts[id(counter)] = ([], [], [], [], [], counter)
+            cohort[0].append(p)
+            cohort[1].append(g)
+            cohort[2].append(s[first])
+            cohort[3].append(s[second])
+            cohort[4].append(s.get("master", p))
         for key, states in behind.items():
             if key in cohorts:
                 own = states[0]["counter"].clone()
@@ -385,7 +393,6 @@ class AdamW(torch.optim.Optimizer):
                     s["counter"] = own
         return list(cohorts.values())
 
-    @torch.no_grad()
     def step(self, closure=None, *, grad_scale: float = 1.0):
         """One step; ``grad_scale``: the loss scale that the gradients carry (they are left as they are)."""
         loss = None
@@ -397,17 +404,13 @@ class AdamW(torch.optim.Optimizer):
             return loss
         norm = None
         if self.max_norm is not None or self.skip_nonfinite:
-            norm = self.grad_norm = grad_norm([p.grad for _, cohort in calls for p, _ in cohort])
-        for group, cohort in calls:
-            bits = group["state_bits"]
-            names = ("exp_avg", "exp_avg_sq") if bits == 32 else ("codes", "absmax")
-            masters = [s.get("master", p) for p, s in cohort]
-            (adamw_step if bits == 32 else adamw8_step)(
-                [p for p, _ in cohort], [p.grad for p, _ in cohort], [s[names[0]] for _, s in cohort],
-                [s[names[1]] for _, s in cohort], cohort[0][1]["counter"], lr=group["lr"], beta1=group["betas"][0],
-                beta2=group["betas"][1], eps=group["eps"], weight_decay=group["weight_decay"],
-                masters=masters if group["master_weights"] else None, unit_rows=group["unit_rows"], grad_norm=norm,
-                max_norm=self.max_norm, grad_scale=grad_scale)
+            norm = self.grad_norm = grad_norm([g for _, cohort in calls for g in cohort[1]])
+        for group, (params, grads, first, second, masters, counter) in calls:
+            eight = group["state_bits"] == 8
+            beta1, beta2 = group["betas"]
+            _call(8 if eight else 32, _adamw8_op if eight else _adamw_op, params, grads, first, second, counter, group["lr"], beta1,
+                  beta2, group["eps"], group["weight_decay"], masters if group["master_weights"] else None, group["unit_rows"],
+                  norm, self.max_norm, grad_scale)
         return loss
 
     def moments(self, p: Tensor, dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:
