@@ -70,7 +70,7 @@ AdamwTable table_of(const flexsae_adamw_config &c) {
 
 using Kernel = void (*)(const AdamwTable);
 
-// How the rows of a tensor are shared out: the fewest wavefronts that hold a row in registers.
+// How the rows of a tensor are shared out.
 struct RowPlan {
   Kernel kernel;
   int threads, rows;  // of a block
@@ -81,12 +81,17 @@ RowPlan held_by() {
   return {adamw_rows_kernel<T, MASTER, EIGHT, WAVES, kWave, UNITS>, rows_threads(WAVES), rows_threads(WAVES) / (WAVES * kWave)};
 }
 
+// A row goes to as few lanes as hold it in four units each, since what a wavefront does for the row (its sums, its places) is shared
+// by what it holds; and to no fewer, since registers then leave too few wavefronts to cover memory and arithmetic with each other.
+// us with 1 / 4 / 8 wavefronts a row (40M fp32 elements): 1024 columns, states in 8 bits 116 / 115 / 214, in 32 189 / 198 / 183;
+// 2304 columns 214 / 125 / 143 and 204 / 189 / 189; 4096 columns - / 124 / 126 and - / 190 / 187.  Walked three times instead of held,
+// from 1.5 times as long (8192 columns, 32 bits 350 / 198) on.
 template <typename T, bool MASTER, bool EIGHT>
 RowPlan row_plan(int64_t cols) {
   constexpr int N = kUnit<T, MASTER, EIGHT>;
   if (cols <= 16 * N) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 16, 1>, 256, 16};
   if (cols <= 32 * N) return {adamw_rows_kernel<T, MASTER, EIGHT, 1, 32, 1>, 256, 8};
-  switch (cols <= 64 * 64 * N ? ceil_div(cols, 64 * N) : 65) {  // stretches of a wavefront
+  switch (ceil_div(cols, 64 * N)) {  // stretches of a wavefront
     case 1: return held_by<T, MASTER, EIGHT, 1, 1>();
     case 2: return held_by<T, MASTER, EIGHT, 1, 2>();
     case 3: return held_by<T, MASTER, EIGHT, 1, 3>();

@@ -136,7 +136,7 @@ def test_other_betas(betas, eps, bits):
 
 
 ROWS = [1, 2, 48, 63, 64, 65, 100, 128, 255, 256, 257, 511, 512, 513, 1024, 1025, 1536, 1538, 2304, 2560, 2561, 4096, 4099, 8192,
-        8193, 16384, 16390, 20001]
+        8193, 16384, 16390, 20001, 33001]
 
 
 @pytest.mark.parametrize("bits", [32, 8])
