@@ -580,8 +580,8 @@ PyObject *py_hier_sgd(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // ---- the optimiser -------------------------------------------------------------------------
 // The tensors of a list or tuple, each plain and of `device` (undefined: the first one's); false: not this module's business.  The
-// list keeps them: these functions hold the interpreter's lock, and no reference of their own (a call of 192 tensors is
-// host work: 55 us with references, checks for forward gradients, which optim.py has made, and 48 tensors a launch).
+// list keeps them: these functions hold the interpreter's lock, and no reference of their own (a step of 192 tiny tensors is
+// host work: 30 us; 55 with references, with checks for forward gradients, which optim.py has made, and 48 tensors a launch).
 using Tensors = std::vector<const Tensor *>;
 bool take_tensors(PyObject *o, Tensors &out, c10::optional<c10::Device> &device) {
   static const uint64_t usual =
@@ -750,6 +750,7 @@ PyObject *py_adamw8_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!plain_surroundings() || !take_tensors(args[0], codes, device) || codes.empty() || !take_tensors(args[1], absmax, device) ||
       absmax.size() != codes.size() || dtype < 0 || dtype > 2)
     Py_RETURN_NONE;
+  const c10::DeviceGuard guard(*device);
   std::vector<flexsae_adamw8_state> list(codes.size());
   const c10::ScalarType type = dtype == FLEXSAE_F32    ? c10::ScalarType::Float
                                : dtype == FLEXSAE_BF16 ? c10::ScalarType::BFloat16
@@ -766,7 +767,6 @@ PyObject *py_adamw8_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
     v.push_back(make(c, c.sizes().slice(0, c.dim() - 1), type));
     list[i] = {c.const_data_ptr(), a.const_data_ptr<float>(), m[i].data_ptr(), v[i].data_ptr(), rows, cols};
   }
-  const c10::DeviceGuard guard(*device);
   check(lib.adamw8_moments(list.data(), static_cast<int64_t>(list.size()), static_cast<int>(dtype), stream_of(*codes[0])),
         "flexsae_adamw8_moments");
   auto list_of = [](const std::vector<Tensor> &tensors) {

@@ -230,7 +230,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                counter: Tensor, *, lr: Union[_Reals, Tensor] = 1e-3, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
                weight_decay: _Reals = 0.0, masters: Optional[Sequence[Tensor]] = None, unit_rows: bool = False,
                grad_norm: Optional[Tensor] = None, max_norm: Optional[float] = None, grad_scale: float = 1.0) -> None:
-    """One AdamW step of all ``params``, in place, in one launch for up to 48 of them; ``t = counter[0] + 1``::
+    """One AdamW step of all ``params``, in place, in one launch for up to 66 of them; ``t = counter[0] + 1``::
 
         g = c * grad              c = min(1, max_norm / (grad_norm / grad_scale + 1e-6)) / grad_scale
         m = beta1 * m + (1 - beta1) * g

@@ -574,6 +574,26 @@ def test_ops_pass_torchs_own_checks():
     torch.library.opcheck(torch.ops.flexsae_amd.adamw8_moments.default, (p.s0, p.s1, BF16))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_compiled_step(bits):
+    """Traced calls see the ops: no break in the graph, the same bits."""
+    a, b = (Problem([(60, 70), (70,)], BF16, bits, master=True, seed=13) for _ in range(2))
+
+    @torch.compile(fullgraph=True)
+    def compiled(params, grads, s0, s1, masters, counter):
+        norm = flex.grad_norm(grads)
+        (flex.adamw_step if bits == 32 else flex.adamw8_step)(params, grads, s0, s1, counter, masters=masters, lr=1e-2, grad_norm=norm,
+                                                              max_norm=0.1)
+        return norm * 2
+
+    for _ in range(2):
+        norm = flex.grad_norm(a.grads)
+        a.step(lr=1e-2, grad_norm=norm, max_norm=0.1)
+        assert torch.equal(compiled(b.params, b.grads, b.s0, b.s1, b.masters, b.counter), norm * 2)
+        for x, y in zip(a.tensors(), b.tensors()):
+            assert torch.equal(x, y)
+
+
 # ---- refusals ------------------------------------------------------------------------------
 
 
