@@ -308,29 +308,78 @@ __device__ __forceinline__ T across_lanes(T x, F join) {
   return x;
 }
 
-// What a maximum is kept as: zero below the smallest normal number (its inverse would overflow), NaN where the block has
-// infinities or NaN.
-__device__ __forceinline__ float kept_max(float a, bool bad) {
-  return bad ? __uint_as_float(0x7fc00000u) : a < 0x1p-126f ? 0.f : a;
+// 1 / a of a positive normal number, rounded once: a reciprocal, its error put right, and the exponent by itself (the result may
+// lie below the normal numbers).
+__device__ __forceinline__ float inverse(float a) {
+  const float x = __builtin_amdgcn_frexp_mantf(a), r = __builtin_amdgcn_rcpf(x);
+  return __builtin_amdgcn_ldexpf(fmaf(r, fmaf(-x, r, 1.f), r), -__builtin_amdgcn_frexp_expf(a));
 }
 
-// The maxima of a block that LANES lanes hold; a_m comes in as what it was.  v's as whole numbers: the bits of non-negative floats
-// are in their order, infinity and NaN above all.  m has infinities or NaN where v has, or had NaN before, which is why the
-// floating-point maximum, which passes over NaN, is enough.
+// The maxima of |m| and of v over a block that LANES lanes hold, and their inverses (zero for zero).  A maximum is kept as zero
+// below the smallest normal number (its inverse would overflow), as NaN where the block has infinities or NaN: as whole numbers
+// the bits of non-negative floats are in their order, infinity and NaN above all.
+struct Maxima {
+  float m, v, per_m, per_v, root_per_v;
+};
+
+__device__ __forceinline__ float kept(uint32_t bits) {
+  return bits < 0x00800000u ? 0.f : bits < 0x7f800000u ? __uint_as_float(bits) : __uint_as_float(0x7fc00000u);
+}
+
 template <int LANES, int N>
-__device__ __forceinline__ void maxima(const float (&m)[N], const float (&v)[N], float &a_m, float &a_v) {
+__device__ __forceinline__ Maxima maxima(const float (&m)[N], const float (&v)[N], float m_before) {
+  Maxima r;
   uint32_t bv = 0;
-  float bm = 0.f;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    bm = fmaxf(bm, fabsf(m[j]));
-    bv = max(bv, __float_as_uint(v[j]));
+  for (int j = 0; j < N; ++j) bv = max(bv, __float_as_uint(v[j]));
+  if constexpr (N == 4) {
+    // After the first exchange even lanes carry m's and odd lanes v's, so that the other exchanges and the inverses serve both:
+    // what a block costs is shared by few elements (24571 x 1538 fp32 150 -> 147 us, 2.1M fp32 11.6 -> 11.0).  With eight the registers
+    // it takes cost more (302M bf16 512 -> 536 us).
+    uint32_t bm = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) bm = max(bm, __float_as_uint(m[j]) & 0x7fffffffu);
+    auto move = [](uint32_t y, auto ctrl) {
+      return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(y), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    const bool odd = (threadIdx.x & 1) != 0;
+    uint32_t x = odd ? bv : bm;
+    x = max(x, move(odd ? bm : bv, std::integral_constant<int, 0xB1>{}));  // lane ^ 1 gives what it does not carry
+    x = max(x, move(x, std::integral_constant<int, 0x4E>{}));              // lane ^ 2
+    x = max(x, move(x, std::integral_constant<int, 0x124>{}));             // 4 lanes on, in the row of 16
+    x = max(x, move(x, std::integral_constant<int, 0x128>{}));             // 8 lanes on
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    if constexpr (LANES >= 32) {
+      const u32x2 y = __builtin_amdgcn_permlane16_swap(x, x, false, false);  // the other row of each two
+      x = max(y[0], y[1]);
+    }
+    if constexpr (LANES == 64) {
+      const u32x2 y = __builtin_amdgcn_permlane32_swap(x, x, false, false);  // the other half
+      x = max(y[0], y[1]);
+    }
+    const float a = kept(x), per = a > 0.f ? inverse(a) : 0.f;
+    auto even_of = [&](float y) { return __uint_as_float(move(__float_as_uint(y), std::integral_constant<int, 0xA0>{})); };
+    auto odd_of = [&](float y) { return __uint_as_float(move(__float_as_uint(y), std::integral_constant<int, 0xF5>{})); };
+    r.m = even_of(a);
+    r.v = odd_of(a);
+    r.per_m = even_of(per);
+    r.per_v = odd_of(per);
+    r.root_per_v = odd_of(__builtin_amdgcn_sqrtf(per));
+  } else {
+    // m has infinities or NaN where v has, or had NaN before, which is why the floating-point maximum, which passes over NaN, is
+    // enough.
+    float bm = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) bm = fmaxf(bm, fabsf(m[j]));
+    bm = across_lanes<LANES>(bm, [](float x, float y) { return fmaxf(x, y); });
+    bv = across_lanes<LANES>(bv, [](uint32_t x, uint32_t y) { return max(x, y); });
+    r.m = kept(bv >= 0x7f800000u || m_before != m_before ? 0x7fc00000u : __float_as_uint(bm));
+    r.v = kept(bv);
+    r.per_m = r.m > 0.f ? inverse(r.m) : 0.f;
+    r.per_v = r.v > 0.f ? inverse(r.v) : 0.f;
+    r.root_per_v = __builtin_amdgcn_sqrtf(r.per_v);
   }
-  bm = across_lanes<LANES>(bm, [](float x, float y) { return fmaxf(x, y); });
-  bv = across_lanes<LANES>(bv, [](uint32_t x, uint32_t y) { return max(x, y); });
-  const bool bad = bv >= 0x7f800000u;
-  a_m = kept_max(bm, bad || a_m != a_m);
-  a_v = kept_max(__uint_as_float(bv), bad);
+  return r;
 }
 
 // Codes of two elements, (m, v) each, from |m| / a_m and v / a_v: whole numbers nearest to 127 sqrt and 255 sqrt sqrt of them, as
@@ -370,23 +419,14 @@ __device__ __forceinline__ bool codes_of_two(const float *m, const float *v, flo
   return differ != 0;
 }
 
-// 1 / a of a positive normal number, rounded once: a reciprocal, its error put right, and the exponent by itself (the result may
-// lie below the normal numbers).
-__device__ __forceinline__ float inverse(float a) {
-  const float x = __builtin_amdgcn_frexp_mantf(a), r = __builtin_amdgcn_rcpf(x);
-  return __builtin_amdgcn_ldexpf(fmaf(r, fmaf(-x, r, 1.f), r), -__builtin_amdgcn_frexp_expf(a));
-}
-
 // s: the hardware's square roots of v
 template <int N>
-__device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], const float (&s)[N], float a_m, float a_v, Codes<N> &c) {
-  const float per_m = a_m > 0.f ? inverse(a_m) : 0.f, per_v = a_v > 0.f ? inverse(a_v) : 0.f;
-  const float root_per_v = __builtin_amdgcn_sqrtf(per_v);
+__device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], const float (&s)[N], const Maxima &a, Codes<N> &c) {
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
     // (one wavefront in 40 has such an element)
-    const bool near = codes_of_two<false>(m + j, v + j, per_m, per_v, root_per_v, s + j, c.w[j / 2]);
-    if (__any(near)) (void)codes_of_two<true>(m + j, v + j, per_m, per_v, root_per_v, s + j, c.w[j / 2]);
+    const bool near = codes_of_two<false>(m + j, v + j, a.per_m, a.per_v, a.root_per_v, s + j, c.w[j / 2]);
+    if (__any(near)) (void)codes_of_two<true>(m + j, v + j, a.per_m, a.per_v, a.root_per_v, s + j, c.w[j / 2]);
   }
 }
 
@@ -462,13 +502,12 @@ struct AdamwUnit {
     adamw_move(c, t.lr * c.inv_bc1, 1.f - t.lr * c.lr * t.weight_decay, m, s, w);
     if constexpr (STORE && EIGHT) {
       constexpr int kLanes = LANES < kQuantLanes ? LANES : kQuantLanes;
-      float a_m = top.x, a_v;
-      maxima<kLanes>(m, v, a_m, a_v);
+      const Maxima a = maxima<kLanes>(m, v, top.x);
       Codes<N> now;
-      encode(m, v, s, a_m, a_v, now);
+      encode(m, v, s, a, now);
       store_codes(t.s0, at, now);
       if (at.left > 0 && (threadIdx.x & (kLanes - 1)) == 0)
-        static_cast<float2 *>(t.s1)[at.block + at.col / kAdamwQuant] = float2{a_m, a_v};
+        static_cast<float2 *>(t.s1)[at.block + at.col / kAdamwQuant] = float2{a.m, a.v};
     } else if constexpr (STORE) {
       store_upto<float>(t.s0, at, m);
       store_upto<float>(t.s1, at, v);
