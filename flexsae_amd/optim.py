@@ -321,7 +321,8 @@ class AdamW(torch.optim.Optimizer):
     max_norm: the gradients of all groups are clipped to this norm together.  skip_nonfinite: a step whose gradients hold an
     infinity or NaN changes nothing, as always with max_norm.  After a step with either ``grad_norm`` is the norm of the gradients
     as they were, on the device.
-    Parameters without a gradient are left out of a step, their number of steps too."""
+    Parameters without a gradient are left out of a step, their number of steps too.  Whoever changes 16-bit parameters with master
+    weights from outside calls ``reset_masters()``."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, unit_rows: bool = False, master_weights: bool = True,
@@ -421,10 +422,22 @@ class AdamW(torch.optim.Optimizer):
             return m[0], v[0]
         return s["exp_avg"].to(dtype), s["exp_avg_sq"].to(dtype)
 
+    def reset_masters(self) -> None:
+        """Master weights from the parameters as they are: for whoever has changed those from outside (a step would otherwise bring
+        back what the masters hold)."""
+        for p, s in self.state.items():
+            if "master" in s:
+                s["master"].copy_(p.detach())
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite, "grad_norm": None}
+
     def load_state_dict(self, state_dict) -> None:
         """As torch's, with states kept in their own types (torch's own would turn them into the parameter's).  Parameters of a
         group that have taken the same number of steps share a count again."""
         saved = state_dict["state"]
+        if any("counter" not in s for s in saved.values()):
+            raise ValueError("load_state_dict: the states are not those of this optimizer")
         super().load_state_dict({**state_dict, "state": {}})
         for group, old in zip(self.param_groups, state_dict["param_groups"]):
             counters = {}

@@ -1,5 +1,7 @@
 """Host side of the optimiser (no GPU): refusals of the C ABI and of the Python layer, options of the optimizer."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -115,6 +117,29 @@ def test_new_states_of_8_bits(shape, unit, want):
 def test_options_that_are_refused(kw):
     with pytest.raises(ValueError):
         flex.AdamW([torch.nn.Parameter(torch.ones(3))], **kw)
+
+
+def test_copies_keep_the_options_and_states_of_others_are_refused():
+    p = torch.nn.Parameter(torch.ones(3, 4))
+    opt = flex.AdamW([p], lr=0.5, state_bits=8, max_norm=2.0, skip_nonfinite=True)
+    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert again.max_norm == 2.0 and again.skip_nonfinite and again.grad_norm is None
+        assert again.param_groups[0]["state_bits"] == 8 and again.param_groups[0]["lr"] == 0.5
+    its = torch.optim.AdamW([p])
+    p.grad = torch.ones(3, 4)
+    its.step()
+    with pytest.raises(ValueError, match="not those of this optimizer"):
+        opt.load_state_dict(its.state_dict())
+
+
+def test_masters_follow_parameters_that_were_changed_from_outside():
+    p = torch.nn.Parameter(torch.ones(3, 4, dtype=torch.bfloat16))
+    opt = flex.AdamW([p])
+    opt.state[p] = opt._new_state(p, opt.param_groups[0], torch.zeros(2, dtype=torch.int64))
+    with torch.no_grad():
+        p.mul_(3.0)
+    opt.reset_masters()
+    assert torch.equal(opt.state[p]["master"], torch.full((3, 4), 3.0))
 
 
 def test_fake_kernels():
