@@ -245,7 +245,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     before, and the row divided by its length after.  A row of zeros stays one.
     grad_norm: ``grad_norm(grads)``; one that is not finite makes the call change nothing, ``counter`` neither.  max_norm: clips
     by it.  grad_scale: the loss scale that the gradients carry.
-    Arithmetic is in fp32; a weight without a master is rounded once.  The gradients are left as they are."""
+    Arithmetic is in fp32; a weight without a master is rounded once.  The gradients are left as they are.  With ``eps=0`` an
+    element without any gradient so far stays where it is."""
     _call(32, _adamw_op, params, grads, exp_avgs, exp_avg_sqs, counter, lr, beta1, beta2, eps, weight_decay, masters, unit_rows,
           grad_norm, max_norm, grad_scale)
 

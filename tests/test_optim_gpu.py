@@ -135,6 +135,28 @@ def test_other_betas(betas, eps, bits):
     p.checked_step(betas=betas, eps=eps)
 
 
+@pytest.mark.parametrize("steps", [0, 9, 100, 499, 501, 4999, 10 ** 7, 2 ** 40])
+def test_bias_corrections_early_and_late(steps):
+    """On either side of where the series ends (t log b = -0.5), and where the powers are gone."""
+    for bits in (32, 8):
+        p = Problem([(33, 70)], F32, bits, seed=steps % 97)
+        p.counter = flex.adamw_counter(DEV, steps)
+        p.checked_step()
+        assert int(p.counter[0]) == steps + 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_gradient_ever_and_no_eps(bits):
+    """0 / 0 moves nothing."""
+    p = Problem([(5, 300)], F32, bits, fresh=True)
+    p.grads[0][2:] = 0.0
+    w = p.params[0].clone()
+    p.step(eps=0.0, lr=1e-2)
+    assert torch.equal(p.params[0][2:], w[2:])
+    moved = (p.params[0][:2] - w[:2]) / (-1e-2 * p.grads[0][:2].sign())
+    assert torch.allclose(moved, torch.ones_like(moved), rtol=1e-4)  # the first step is the sign (of weights of 0.05, rounded)
+
+
 ROWS = [1, 2, 48, 63, 64, 65, 100, 128, 255, 256, 257, 511, 512, 513, 1024, 1025, 1536, 1538, 2304, 2560, 2561, 4096, 4099, 8192,
         8193, 16384, 16390, 20001, 33001]
 
