@@ -107,10 +107,14 @@ def _check_step(bits, params, grads, state0, state1, masters, counter, lrs, weig
     if n == 0:
         raise ValueError("expected at least one parameter")
     names = ("exp_avgs", "exp_avg_sqs") if bits == 32 else ("codes", "absmax")
-    lists = [("grads", grads), (names[0], state0), (names[1], state1)] + ([("masters", masters)] if masters else [])
+    lists = [("grads", grads), (names[0], state0), (names[1], state1)]
     for name, x in lists + [("lr", lrs), ("weight_decay", weight_decays)]:
         if len(x) != n:
             raise ValueError(f"{n} params and {len(x)} {name}")
+    narrow = sum(p.dtype != torch.float32 for p in params)
+    if masters and len(masters) != narrow:
+        raise ValueError(f"{narrow} params of 16 bits and {len(masters)} masters")
+    master_of = iter(masters)
     for i, p in enumerate(params):
         if p.dtype not in _DTYPES:
             raise TypeError(f"params must be float32, bfloat16 or float16, got {p.dtype}")
@@ -124,8 +128,9 @@ def _check_step(bits, params, grads, state0, state1, masters, counter, lrs, weig
         for name, t, (dtype, shape) in zip(names, (state0[i], state1[i]), want):
             if t.dtype != dtype or tuple(t.shape) != shape:
                 raise ValueError(f"{name}[{i}] is {t.dtype} {tuple(t.shape)}, expected {dtype} {shape}")
-        if masters and p.dtype != torch.float32 and (masters[i].dtype != torch.float32 or masters[i].shape != p.shape):
-            raise ValueError(f"masters[{i}] is {masters[i].dtype} {tuple(masters[i].shape)}, expected float32 {tuple(p.shape)}")
+        master = next(master_of) if masters and p.dtype != torch.float32 else None
+        if master is not None and (master.dtype != torch.float32 or master.shape != p.shape):
+            raise ValueError(f"the master of params[{i}] is {master.dtype} {tuple(master.shape)}, expected float32 {tuple(p.shape)}")
     if counter.dtype != torch.int64 or counter.numel() != 2 or not counter.is_contiguous():
         raise ValueError("counter: expected int64[2] (adamw_counter)")
     for name, t in (("lr", lr), ("grad_norm", grad_norm)):
@@ -141,12 +146,14 @@ def _check_step(bits, params, grads, state0, state1, masters, counter, lrs, weig
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if max_norm > 0 and grad_norm is None:
         raise ValueError("max_norm needs grad_norm, the norm of the gradients")
-    return _on_gpu([*params, *(t for _, x in lists for t in x), counter, *(t for t in (lr, grad_norm) if t is not None)], "tensors")
+    return _on_gpu([*params, *(t for _, x in lists for t in x), *masters, counter,
+                    *(t for t in (lr, grad_norm) if t is not None)], "tensors")
 
 
 def _step(bits, params, grads, state0, state1, masters, counter, lrs, weight_decays, lr, grad_norm, beta1, beta2, eps,
           grad_scale, max_norm, unit_rows) -> None:
-    """One call of flexsae_adamw_step.  Tensors that are not contiguous are stepped as copies."""
+    """One call of flexsae_adamw_step.  ``masters``: those of the 16-bit params, in their order, or none (an op may change every
+    tensor of this list, so that none of them may be one of the params).  Tensors that are not contiguous are stepped as copies."""
     dev = _check_step(bits, params, grads, state0, state1, masters, counter, lrs, weight_decays, lr, grad_norm, beta1, beta2,
                       eps, grad_scale, max_norm, unit_rows)
     lib = _lib.load()
@@ -162,9 +169,10 @@ def _step(bits, params, grads, state0, state1, masters, counter, lrs, weight_dec
     with _on_device(dev):
         grads = [g.contiguous() for g in grads]
         table = (_lib.AdamwTensor * len(params))()
+        master_of = iter(masters)
         for i, p in enumerate(params):
             rows, cols = _layout(p.shape, unit_rows)
-            master = at(masters[i]) if masters and p.dtype != torch.float32 else None
+            master = at(next(master_of)) if masters and p.dtype != torch.float32 else None
             table[i] = (at(p), _ptr(grads[i]), master, at(state0[i], 0 if bits == 32 else 2), at(state1[i], 0 if bits == 32 else 8),
                         rows, cols, lrs[i], weight_decays[i], _DTYPES[p.dtype])
         config = _lib.AdamwConfig(beta1, beta2, eps, grad_scale, max_norm, None if grad_norm is None else _ptr(grad_norm),
@@ -219,8 +227,14 @@ def _call(bits, op, params, grads, state0, state1, counter, lr, beta1, beta2, ep
     on_device = isinstance(lr, Tensor)
     lrs = [1.0] * n if on_device else [float(lr)] * n if isinstance(lr, (int, float)) else [float(x) for x in lr]
     wds = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(x) for x in weight_decay]
+    if masters is None:
+        masters = []
+    elif len(masters) != n:
+        raise ValueError(f"{n} params and {len(masters)} masters")
+    else:
+        masters = [m for m, p in zip(masters, params) if p.dtype != torch.float32]
     with torch.no_grad():
-        args = (params, grads, state0, state1, masters or [], counter, lrs, wds, lr if on_device else None, grad_norm,
+        args = (params, grads, state0, state1, masters, counter, lrs, wds, lr if on_device else None, grad_norm,
                 float(beta1), float(beta2), float(eps), float(grad_scale), float(max_norm), bool(unit_rows))
         _check_step(bits, *args)
         op(*([t.detach() for t in a] if i < 5 else a for i, a in enumerate(args)))

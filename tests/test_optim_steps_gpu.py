@@ -1,0 +1,48 @@
+"""Steps of the optimiser as programs make them."""
+import pytest
+import torch
+
+import flexsae_amd as flex
+from tests.test_optim_gpu import BF16, F16, F32, Problem
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtypes", [[F32, F32], [BF16, F32, F16, F32], [F16, BF16]], ids=str)
+@pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
+def test_a_compiled_step_with_masters_of_fp32_parameters(bits, dtypes, backend):
+    """The entry of an fp32 parameter is ignored, the parameter itself in that place too."""
+    torch._dynamo.reset()  # (compilations of other cases count)
+    a, b = (Problem([(30, 40 + i) for i in range(len(dtypes))], dtypes, bits, seed=21) for _ in range(2))
+
+    @torch.compile(fullgraph=True, backend=backend)
+    def compiled(params, grads, s0, s1, masters, counter):
+        (flex.adamw_step if bits == 32 else flex.adamw8_step)(params, grads, s0, s1, counter, masters=masters, lr=1e-2)
+
+    for p in (a, b):
+        p.master = True
+        p.masters = [w if w.dtype == F32 else m for w, m in zip(p.params, p.masters)]
+    start = [w.clone() for w in a.params]
+    for _ in range(2):
+        a.step(lr=1e-2)
+        compiled(b.params, b.grads, b.s0, b.s1, b.masters, b.counter)
+        for x, y in zip(a.tensors(), b.tensors()):
+            assert torch.equal(x, y)
+    assert not any(torch.equal(x, y) for x, y in zip(start, b.params))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_ops_with_masters_pass_torchs_own_checks(bits):
+    p = Problem([(20, 30), (30,), (7, 9)], [F16, F32, BF16], bits, master=True)
+    op = torch.ops.flexsae_amd.adamw_step_ if bits == 32 else torch.ops.flexsae_amd.adamw8_step_
+    torch.library.opcheck(op.default, (p.params, p.grads, p.s0, p.s1, [p.masters[0], p.masters[2]], p.counter, [1e-3] * 3, [0.0] * 3, None,
+                                       None, 0.9, 0.999, 1e-8, 1.0, 0.0, False))
+
+
+def test_the_op_takes_masters_of_16_bit_parameters_alone():
+    p = Problem([(20, 30), (30,)], [F16, F32], 32, master=True)
+    for masters in (p.masters, [p.masters[1]]):
+        with pytest.raises(ValueError, match="master"):
+            torch.ops.flexsae_amd.adamw_step_(p.params, p.grads, p.s0, p.s1, masters, p.counter, [1e-3] * 2, [0.0] * 2, None, None, 0.9, 0.999,
+                                              1e-8, 1.0, 0.0, False)
