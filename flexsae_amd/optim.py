@@ -410,7 +410,13 @@ class AdamW(torch.optim.Optimizer):
         return list(cohorts.values())
 
     def step(self, closure=None, *, grad_scale: float = 1.0):
-        """One step; ``grad_scale``: the loss scale that the gradients carry (they are left as they are)."""
+        """One step; ``grad_scale``: the loss scale that the gradients carry (they are left as they are).  Within a compiled function
+        it runs as outside of one: which parameters are stepped together is up to the host."""
+        if torch.compiler.is_compiling():
+            return _uncompiled_step(self, closure, grad_scale)
+        return self._step(closure, grad_scale)
+
+    def _step(self, closure, grad_scale: float):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -463,3 +469,8 @@ class AdamW(torch.optim.Optimizer):
                 counter = s["counter"]
                 s["counter"] = counters.setdefault((p.device, int(counter[0])), counter)
                 self.state[p] = s
+
+
+@torch._disable_dynamo  # (torch.compiler.disable, but for the compiler's import here)
+def _uncompiled_step(opt: AdamW, closure, grad_scale: float):
+    return opt._step(closure, grad_scale)

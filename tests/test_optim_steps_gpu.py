@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import flexsae_amd as flex
-from tests.test_optim_gpu import BF16, F16, F32, Problem
+from tests.test_optim_gpu import BF16, F16, F32, Problem, _model, _set_grads
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +30,50 @@ def test_a_compiled_step_with_masters_of_fp32_parameters(bits, dtypes, backend):
         for x, y in zip(a.tensors(), b.tensors()):
             assert torch.equal(x, y)
     assert not any(torch.equal(x, y) for x, y in zip(start, b.params))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtypes", [[F32] * 4, [BF16, F32, F32, BF16]], ids=str)
+def test_a_compiled_step_of_the_optimizer(bits, dtypes):
+    torch._dynamo.reset()
+    models = [[torch.nn.Parameter(p.detach().to(d)) for p, d in zip(_model(), dtypes)] for _ in range(2)]
+    opts = [flex.AdamW([{"params": m[:1], "unit_rows": True}, {"params": m[1:]}], lr=1e-2, state_bits=bits, max_norm=0.1) for m in models]
+    compiled = torch.compile(opts[1].step, backend="aot_eager")
+    for i in range(3):
+        for m in models:
+            _set_grads(m, i)
+        opts[0].step()
+        compiled()
+        for x, y in zip(*models):
+            assert torch.equal(x, y)
+            for k, s in opts[0].state[x].items():
+                assert torch.equal(s, opts[1].state[y][k]), k
+
+
+def test_a_step_within_a_compiled_function():
+    """... with its closure, hooks that run once, and the norm for the caller."""
+    torch._dynamo.reset()
+    a, b = _model(), _model()
+    mine, its = flex.AdamW(a, lr=1e-2, max_norm=0.5), flex.AdamW(b, lr=1e-2, max_norm=0.5)
+
+    def one(opt, params):
+        def loss():
+            opt.zero_grad()
+            total = sum((p * p).sum() for p in params)
+            total.backward()
+            return total.detach()
+        return opt.step(loss, grad_scale=2.0) + opt.grad_norm
+
+    ran = []
+    its.register_step_pre_hook(lambda *_: ran.append("before"))
+    its.register_step_post_hook(lambda *_: ran.append("after"))
+    compiled = torch.compile(one, backend="aot_eager")
+    for _ in range(3):
+        # (the loss and its gradients may be summed in another order)
+        assert torch.allclose(one(mine, a), compiled(its, b), rtol=1e-5)
+        for x, y in zip(a, b):
+            assert torch.allclose(x, y, rtol=1e-4, atol=1e-5)
+    assert ran == ["before", "after"] * 3
 
 
 @pytest.mark.parametrize("bits", [32, 8])
