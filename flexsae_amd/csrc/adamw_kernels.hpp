@@ -446,13 +446,14 @@ __device__ __forceinline__ void adamw_moments(const AdamwCoefs &c, const float (
 
 // s: square roots of v.  The hardware's root and reciprocal, each off by a unit in the last place: of the update, which is a small
 // part of the weight.  (It takes a v below the smallest normal number for zero: the root's floor keeps the quotient finite
-// where eps is zero.)
+// where eps is zero.  The larger of two whole numbers: a NaN, which the larger of two floats passes over, reaches the weight.)
 template <int N>
 __device__ __forceinline__ void adamw_move(const AdamwCoefs &c, float step, float keep, const float (&m)[N], const float (&s)[N],
                                            float (&w)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const float per = __builtin_amdgcn_rcpf(fmaf(fmaxf(s[j], kRootFloor), c.inv_sqrt_bc2, c.eps));
+    const float root = __uint_as_float(max(__float_as_uint(s[j]), __float_as_uint(kRootFloor)));
+    const float per = __builtin_amdgcn_rcpf(fmaf(root, c.inv_sqrt_bc2, c.eps));
     w[j] = fmaf(-step, m[j] * per, keep * w[j]);
   }
 }

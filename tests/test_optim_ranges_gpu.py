@@ -1,0 +1,51 @@
+"""AdamW steps where squares overflow or vanish."""
+import pytest
+import torch
+
+import flexsae_amd as flex
+from tests import optim_reference as ref
+from tests.test_optim_gpu import BF16, DEV, F16, F32, Problem
+
+pytestmark = pytest.mark.gpu
+
+# a NaN in v: bits, type, master, columns of a row (0: as stored); four and eight elements a lane, held and walked rows
+FORMS = [(32, F32, False, 0), (32, BF16, True, 0), (32, F32, False, 300), (32, F32, False, 40), (32, F32, False, 20001),
+         (8, F32, False, 0), (8, BF16, False, 0), (8, BF16, True, 0), (8, F16, False, 0), (8, F32, False, 300), (8, BF16, False, 300),
+         (8, BF16, False, 100), (8, BF16, False, 20001)]
+
+
+@pytest.mark.parametrize("bits,dtype,master,cols", FORMS)
+def test_a_v_that_is_nan_reaches_the_weight(bits, dtype, master, cols):
+    """... of its element (32 bits), or of its block (8 bits), with an m that is finite."""
+    p = Problem([(3, cols)] if cols else [(4, 1000)], dtype, bits, unit=cols > 0, master=master)
+    bad = torch.zeros(p.params[0].shape, dtype=torch.bool, device=DEV)
+    if bits == 32:
+        p.s1[0].view(-1)[37] = float("nan")
+        bad.view(-1)[37] = True
+    else:
+        p.s1[0].view(-1, 2)[0, 1] = float("nan")
+        bad.view(-1)[:min(256, cols or 256)] = True
+    p.step()
+    _, v = p.moments(0)
+    assert torch.equal(v.isnan().view(-1), bad.view(-1))
+    assert torch.equal(p.held(0).isnan(), bad) and torch.equal(p.params[0].isnan(), bad)
+
+
+@pytest.mark.parametrize("dtype,master", [(F32, False), (BF16, True)])
+def test_a_square_that_overflows(dtype, master):
+    """A finite gradient whose square is infinite: v of its block is NaN from then on, m keeps its values, the weights follow in
+    the next step."""
+    p = Problem([(4, 1000)], dtype, 8, master=master, fresh=True)
+    p.grads[0].view(-1)[777] = 1e20
+    assert torch.isfinite(flex.grad_norm(p.grads))
+    p.step()
+    block = torch.zeros(4000, dtype=torch.bool, device=DEV)
+    block[768:1024] = True
+    for again in range(2):
+        m, v = (x[0].view(-1) for x in flex.adamw8_moments(p.s0, p.s1))
+        assert torch.equal(v.isnan(), block)
+        assert torch.isfinite(m).all()
+        assert abs(float(m[777]) / (1e19 * 0.9 ** again) - 1) < 2.0 ** -7  # (1e20 rounded to the type)
+        assert torch.equal(p.held(0).view(-1).isnan(), block if again else torch.zeros_like(block))
+        p.grads[0].view(-1)[777] = 0.0
+        p.step()
