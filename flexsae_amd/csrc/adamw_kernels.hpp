@@ -366,14 +366,20 @@ __device__ __forceinline__ Maxima maxima(const float (&m)[N], const float (&v)[N
     r.per_v = odd_of(per);
     r.root_per_v = odd_of(__builtin_amdgcn_sqrtf(per));
   } else {
-    // m has infinities or NaN where v has, or had NaN before, which is why the floating-point maximum, which passes over NaN, is
-    // enough.
+    // The floating-point maximum passes over NaN, and m has infinities or NaN only where v has, or its maximum was NaN before (a
+    // finite g whose square overflows leaves m as it is): such blocks are asked again.
     float bm = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) bm = fmaxf(bm, fabsf(m[j]));
     bm = across_lanes<LANES>(bm, [](float x, float y) { return fmaxf(x, y); });
     bv = across_lanes<LANES>(bv, [](uint32_t x, uint32_t y) { return max(x, y); });
-    r.m = kept(bv >= 0x7f800000u || m_before != m_before ? 0x7fc00000u : __float_as_uint(bm));
+    r.m = kept(__float_as_uint(bm));
+    if (__any(bv >= 0x7f800000u || m_before != m_before)) {
+      uint32_t all = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) all = max(all, __float_as_uint(m[j]) & 0x7fffffffu);
+      r.m = kept(across_lanes<LANES>(all, [](uint32_t x, uint32_t y) { return max(x, y); }));
+    }
     r.v = kept(bv);
     r.per_m = r.m > 0.f ? inverse(r.m) : 0.f;
     r.per_v = r.v > 0.f ? inverse(r.v) : 0.f;

@@ -31,7 +31,7 @@ def test_a_v_that_is_nan_reaches_the_weight(bits, dtype, master, cols):
     assert torch.equal(p.held(0).isnan(), bad) and torch.equal(p.params[0].isnan(), bad)
 
 
-@pytest.mark.parametrize("dtype,master", [(F32, False), (BF16, True)])
+@pytest.mark.parametrize("dtype,master", [(F32, False), (BF16, False), (BF16, True)])
 def test_a_square_that_overflows(dtype, master):
     """A finite gradient whose square is infinite: v of its block is NaN from then on, m keeps its values, the weights follow in
     the next step."""
@@ -49,3 +49,27 @@ def test_a_square_that_overflows(dtype, master):
         assert torch.equal(p.held(0).view(-1).isnan(), block if again else torch.zeros_like(block))
         p.grads[0].view(-1)[777] = 0.0
         p.step()
+
+
+@pytest.mark.parametrize("dtype,master,cols", [f[1:] for f in FORMS if f[0] == 8])
+def test_m_keeps_its_values_beside_a_v_that_is_nan(dtype, master, cols):
+    p = Problem([(3, cols)] if cols else [(4, 1000)], dtype, 8, unit=cols > 0, master=master)
+    m, v = p.moments(0)
+    m = 0.9 * m
+    p.s1[0].view(-1, 2)[0, 1] = float("nan")
+    p.grads[0].zero_()
+    p.step()
+    # equal decay leaves the codes where the largest has the highest one, and moves a code by half at most elsewhere: half a
+    # code of c is 1 / 2c of the root, 1 / c and a bit of the value
+    got, _ = p.moments(0)
+    top = m.abs().amax()
+    assert bool(((got - m).abs() <= (m.abs() * top).sqrt() / 127 + top / (4 * 127 ** 2) + 1e-6 * m.abs()).all())
+
+
+def test_an_m_that_is_nan_does_not_need_a_v():
+    for dtype in (F32, BF16):
+        p = Problem([(4, 1000)], dtype, 8)
+        p.s1[0].view(-1, 2)[1, 0] = float("nan")
+        p.step()
+        m, v = (x[0].view(-1) for x in flex.adamw8_moments(p.s0, p.s1))
+        assert m.isnan().nonzero().flatten().tolist() == list(range(256, 512)) and torch.isfinite(v).all()
