@@ -393,33 +393,35 @@ __device__ __forceinline__ Maxima maxima(const float (&m)[N], const float (&v)[N
 // `root_v` = sqrt(v) sqrt(1 / a_v) among them, off by a unit in the last place each: with the roundings on either side 2.5e-7 of
 // the result for m and 5.5e-7 for v.  Both ends of that stretch are rounded; where they are not the same, true comes back.
 // Adding kMagic rounds to a whole number, which then stands in the low bits.
+// The hardware's root takes a number below the normal ones for zero.  Maxima above 2^126 have such an inverse, and beside
+// one below 2^-96 such a v has a code above one ((2^-126 / 2^-96)^(1/4) is 1.41 / 255): blocks of these are EXACT (rooted).
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
 constexpr float kOffM = 2.5e-7f, kOffV = 5.5e-7f;
 
+// Whether the hardware's roots serve a block of this maximum of v (one that is kept as zero or NaN has no codes to speak of).
+__device__ __forceinline__ bool rooted(float a_v) { return !(a_v > 0x1p126f || (a_v > 0.f && a_v < 0x1p-96f)); }
+
 template <bool EXACT>
-__device__ __forceinline__ bool codes_of_two(const float *m, const float *v, float per_m, float per_v, float root_per_v,
-                                             const float *s, uint32_t &w) {
+__device__ __forceinline__ bool codes_of_two(const float *m, const float *v, const Maxima &a, uint32_t least, const float *s,
+                                             uint32_t &w) {
 #pragma clang fp contract(off)
   uint32_t pair[2], differ = 0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    float x, y, q;
+    float x, y;
     if constexpr (EXACT) {
-      x = copysignf(sqrtf(fabsf(m[k]) * per_m) * 127.f, m[k]) + (kMagic + 128.f);
-      q = v[k] * per_v;
-      y = sqrtf(sqrtf(q)) * 255.f + kMagic;
+      x = copysignf(sqrtf(fabsf(m[k]) * a.per_m) * 127.f, m[k]) + (kMagic + 128.f);
+      y = sqrtf(sqrtf(v[k] * a.per_v)) * 255.f + kMagic;
     } else {
-      q = s[k] * root_per_v;
-      const float rm = copysignf(__builtin_amdgcn_sqrtf(fabsf(m[k]) * per_m), m[k]), rv = __builtin_amdgcn_sqrtf(q);
+      const float rm = copysignf(__builtin_amdgcn_sqrtf(fabsf(m[k]) * a.per_m), m[k]);
+      const float rv = __builtin_amdgcn_sqrtf(s[k] * a.root_per_v);
       x = fmaf(rm, 127.f * (1.f + kOffM), kMagic + 128.f);
       y = fmaf(rv, 255.f * (1.f + kOffV), kMagic);
       differ |= (__float_as_uint(x) ^ __float_as_uint(fmaf(rm, 127.f * (1.f - kOffM), kMagic + 128.f))) |
                 (__float_as_uint(y) ^ __float_as_uint(fmaf(rv, 255.f * (1.f - kOffV), kMagic)));
     }
-    // (a v above zero never becomes zero)
-    uint32_t least;
-    asm("v_min_u32 %0, 1, %1" : "=v"(least) : "v"(q));
-    pair[k] = __builtin_amdgcn_perm(max(__float_as_uint(y) & 0xffu, least), __float_as_uint(x), 0x0c0c0400u);
+    // (a v above zero never becomes zero: `least` is one where the block has a maximum)
+    pair[k] = __builtin_amdgcn_perm(max(__float_as_uint(y) & 0xffu, min(__float_as_uint(v[k]), least)), __float_as_uint(x), 0x0c0c0400u);
   }
   w = pair[0] | (pair[1] << 16);
   return differ != 0;
@@ -428,11 +430,13 @@ __device__ __forceinline__ bool codes_of_two(const float *m, const float *v, flo
 // s: the hardware's square roots of v
 template <int N>
 __device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], const float (&s)[N], const Maxima &a, Codes<N> &c) {
+  const uint32_t least = a.v > 0.f ? 1u : 0u;
+  const bool all = !rooted(a.v);
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
     // (one wavefront in 40 has such an element)
-    const bool near = codes_of_two<false>(m + j, v + j, a.per_m, a.per_v, a.root_per_v, s + j, c.w[j / 2]);
-    if (__any(near)) (void)codes_of_two<true>(m + j, v + j, a.per_m, a.per_v, a.root_per_v, s + j, c.w[j / 2]);
+    const bool near = codes_of_two<false>(m + j, v + j, a, least, s + j, c.w[j / 2]);
+    if (__any(near || all)) (void)codes_of_two<true>(m + j, v + j, a, least, s + j, c.w[j / 2]);
   }
 }
 

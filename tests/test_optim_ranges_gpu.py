@@ -1,4 +1,4 @@
-"""AdamW steps where squares overflow or vanish."""
+"""AdamW steps where squares overflow or vanish, and codes of 8-bit states at both ends of the range."""
 import pytest
 import torch
 
@@ -73,3 +73,38 @@ def test_an_m_that_is_nan_does_not_need_a_v():
         p.step()
         m, v = (x[0].view(-1) for x in flex.adamw8_moments(p.s0, p.s1))
         assert m.isnan().nonzero().flatten().tolist() == list(range(256, 512)) and torch.isfinite(v).all()
+
+
+WIDTHS = [(F32, False, 0), (BF16, False, 0), (BF16, True, 0), (F32, False, 300), (BF16, False, 300), (BF16, False, 20001)]
+
+
+def _state_with(dtype, master, cols, top, seed):
+    """A state of 8 bits whose maxima of v are `top` times one to two."""
+    p = Problem([(3, cols)] if cols else [(2, 700)], dtype, 8, unit=cols > 0, master=master, seed=seed)
+    a = p.s1[0]
+    a[..., 1] = (torch.rand(a.shape[:-1], generator=torch.Generator(DEV).manual_seed(seed), device=DEV) + 1.0) * top
+    p.grads[0].zero_()
+    return p
+
+
+@pytest.mark.parametrize("dtype,master,cols", WIDTHS)
+def test_codes_below_a_very_large_maximum(dtype, master, cols):
+    """Above 2^126 the inverse of the maximum is no normal number."""
+    for top in (2.0 ** 125, 2.0 ** 126, 1.6e38):
+        p = _state_with(dtype, master, cols, top, 3)
+        p.s0[0][..., 1].view(-1)[::5] = 255
+        p.checked_step()
+        assert int(p.s0[0][..., 1].max()) >= 254
+
+
+@pytest.mark.parametrize("dtype,master,cols", WIDTHS)
+def test_codes_of_values_below_the_normal_numbers(dtype, master, cols):
+    """... beside a maximum that is a normal number: the nearest code, and at least one."""
+    for top in (3e-38, 1e-37, 1e-34, 2.0 ** -98, 2.0 ** -97, 2.0 ** -96, 2.0 ** -95, 1e-27):
+        p = _state_with(dtype, master, cols, top, 4)
+        codes = p.s0[0][..., 1]
+        # (from where 32 bits hold a value at all: (c / 255)^4 top is at least 2^-146)
+        codes.clamp_(max(1, int(255 * (2.0 ** -146 / top) ** 0.25) + 1))
+        codes.view(-1)[::3] = 1 if top > 1e-34 else codes.min()
+        p.checked_step()
+        assert bool((p.s0[0][..., 1] >= 1).all())
