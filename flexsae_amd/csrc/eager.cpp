@@ -580,8 +580,9 @@ PyObject *py_hier_sgd(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // ---- the optimiser -------------------------------------------------------------------------
 // The tensors of a list or tuple, each plain and of `device` (undefined: the first one's); false: not this module's business.  The
-// list keeps them: these functions hold the interpreter's lock, and no reference of their own (a step of 192 tiny tensors is
-// host work: 30 us; 55 with references, with checks for forward gradients, which optim.py has made, and 48 tensors a launch).
+// list keeps them: these functions hold the interpreter's lock and run no Python code once they have taken tensors, and have no
+// reference of their own (a step of 192 tiny tensors is host work: 30 us; 55 with references, with checks for forward gradients,
+// which optim.py has made, and 48 tensors a launch).
 using Tensors = std::vector<const Tensor *>;
 bool take_tensors(PyObject *o, Tensors &out, c10::optional<c10::Device> &device) {
   static const uint64_t usual =
@@ -611,14 +612,28 @@ double real(PyObject *o) {
   return v;
 }
 
-// The i-th of a list or tuple of numbers, or the number itself.
-double real_at(PyObject *o, Py_ssize_t i) {
-  return PyList_CheckExact(o) || PyTuple_CheckExact(o) ? real(PySequence_Fast_GET_ITEM(o, i)) : real(o);
-}
-bool reals(PyObject *o, size_t n) {
-  return PyList_CheckExact(o) || PyTuple_CheckExact(o) ? PySequence_Fast_GET_SIZE(o) == static_cast<Py_ssize_t>(n)
-                                                        : PyFloat_Check(o) || PyLong_Check(o);
-}
+// The numbers of a list or tuple, or a number by itself; false: something else.  Reading one may run Python code (__float__, and a
+// tensor's waits for its device without the interpreter's lock), which may change any list: numbers are read before tensors are
+// taken.
+struct Reals {
+  std::vector<double> values;
+  bool one = false;
+
+  bool take(PyObject *o) {
+    if (PyList_CheckExact(o) || PyTuple_CheckExact(o)) {
+      for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(o); ++i) {
+        const auto item = pybind11::reinterpret_borrow<pybind11::object>(PySequence_Fast_GET_ITEM(o, i));
+        values.push_back(real(item.ptr()));
+      }
+      return true;
+    }
+    one = PyFloat_Check(o) || PyLong_Check(o);
+    if (one) values.push_back(real(o));
+    return one;
+  }
+  bool serve(size_t n) const { return one || values.size() == n; }
+  float at(size_t i) const { return static_cast<float>(values[one ? 0 : i]); }
+};
 
 // One fp32 number of `device`; None: none.
 bool take_scalar(PyObject *o, const c10::Device &device, Tensor &out) {
@@ -664,26 +679,30 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arguments(n, 16)) return nullptr;
-  const bool eight = number(args[0]) == 8, unit = number(args[15]) != 0;
+  if (!plain_surroundings()) Py_RETURN_NONE;
+  const bool eight = number(args[0]) == 8, unit = number(args[15]) != 0, device_lr = THPVariable_Check(args[7]);
+  Reals lrs, weight_decays;
+  if ((!device_lr && !lrs.take(args[7])) || !weight_decays.take(args[8])) Py_RETURN_NONE;
+  flexsae_adamw_config config = {real(args[9]), real(args[10]), real(args[11]), static_cast<float>(real(args[12])),
+                                 static_cast<float>(real(args[14])), nullptr, nullptr, nullptr, eight ? 8 : 32,
+                                 unit ? FLEXSAE_ADAMW_UNIT_ROWS : 0};
+  // (no Python code runs from here on)
   Tensors params, grads, s0, s1, masters;
   c10::optional<c10::Device> device;
-  if (!plain_surroundings() || !take_tensors(args[1], params, device) || params.empty() ||
-      !take_tensors(args[2], grads, device) || !take_tensors(args[3], s0, device) || !take_tensors(args[4], s1, device) ||
+  if (!take_tensors(args[1], params, device) || params.empty() || !take_tensors(args[2], grads, device) ||
+      !take_tensors(args[3], s0, device) || !take_tensors(args[4], s1, device) ||
       (args[5] != Py_None && !take_tensors(args[5], masters, device)))
     Py_RETURN_NONE;
   const size_t count = params.size();
   if (grads.size() != count || s0.size() != count || s1.size() != count || (args[5] != Py_None && masters.size() != count) ||
-      !THPVariable_Check(args[6]))
+      (!device_lr && !lrs.serve(count)) || !weight_decays.serve(count) || !THPVariable_Check(args[6]))
     Py_RETURN_NONE;
   const Tensor &counter = THPVariable_Unpack(args[6]);
   if (!plain_tensor(counter) || counter.device() != *device || counter.scalar_type() != c10::ScalarType::Long ||
       counter.numel() != 2 || !changeable(counter))
     Py_RETURN_NONE;
-  const bool device_lr = THPVariable_Check(args[7]);
   Tensor lr, norm;
-  if ((device_lr ? !take_scalar(args[7], *device, lr) : !reals(args[7], count)) || !reals(args[8], count) ||
-      !take_scalar(args[13], *device, norm))
-    Py_RETURN_NONE;
+  if ((device_lr && !take_scalar(args[7], *device, lr)) || !take_scalar(args[13], *device, norm)) Py_RETURN_NONE;
   const c10::AutoGradMode no_grad(false);
   const c10::DeviceGuard guard(*device);
   std::vector<flexsae_adamw_tensor> list(count);
@@ -713,20 +732,12 @@ PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
       master = masters[i]->data_ptr();
     }
     if (!g.is_contiguous()) copies.push_back(g.contiguous());
-    const auto at = static_cast<Py_ssize_t>(i);
     list[i] = {p.data_ptr(), (g.is_contiguous() ? g : copies.back()).const_data_ptr(), master, a.data_ptr(), b.data_ptr(), rows, cols,
-               device_lr ? 1.f : static_cast<float>(real_at(args[7], at)), static_cast<float>(real_at(args[8], at)), dtype};
+               device_lr ? 1.f : lrs.at(i), weight_decays.at(i), dtype};
   }
-  const flexsae_adamw_config config = {real(args[9]),
-                                       real(args[10]),
-                                       real(args[11]),
-                                       static_cast<float>(real(args[12])),
-                                       static_cast<float>(real(args[14])),
-                                       norm.defined() ? f32(norm) : nullptr,
-                                       lr.defined() ? f32(lr) : nullptr,
-                                       counter.data_ptr<int64_t>(),
-                                       eight ? 8 : 32,
-                                       unit ? FLEXSAE_ADAMW_UNIT_ROWS : 0};
+  config.grad_norm = norm.defined() ? f32(norm) : nullptr;
+  config.lr = lr.defined() ? f32(lr) : nullptr;
+  config.counter = counter.data_ptr<int64_t>();
   const int status = lib.adamw_step(list.data(), static_cast<int64_t>(count), &config, stream_of(counter));
   if (status == FLEXSAE_ERR_INVALID_ARGUMENT) Py_RETURN_NONE;  // nothing was launched; optim.py says what is wrong
   if (status == FLEXSAE_OK || status == FLEXSAE_ERR_LAUNCH) {

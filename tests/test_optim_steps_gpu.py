@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import flexsae_amd as flex
-from tests.test_optim_gpu import BF16, F16, F32, Problem, _model, _set_grads
+from tests.test_optim_gpu import BF16, DEV, F16, F32, Problem, _model, _set_grads
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,45 @@ def test_the_op_takes_masters_of_16_bit_parameters_alone():
         with pytest.raises(ValueError, match="master"):
             torch.ops.flexsae_amd.adamw_step_(p.params, p.grads, p.s0, p.s1, masters, p.counter, [1e-3] * 2, [0.0] * 2, None, None, 0.9, 0.999,
                                               1e-8, 1.0, 0.0, False)
+
+
+# ---- numbers whose reading runs Python code ------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_numbers_that_change_the_lists_as_they_are_read(bits):
+    for where in ("lr", "weight_decay"):
+        p = Problem([(20, 30), (30,)], F32, bits)
+        kept = [*p.params, *p.s0, *p.s1]
+        before = [x.clone() for x in (*kept, p.counter)]
+
+        class Clearing:
+            def __float__(self):
+                for x in (p.params, p.grads, p.s0, p.s1):
+                    x.clear()
+                return 1e-3
+
+        numbers = [Clearing(), 1e-3]
+        with pytest.raises(ValueError, match="at least one parameter"):
+            p.step(**{where: numbers})
+
+        class Shortening:
+            def __float__(self):
+                del numbers[1:]
+                return 1e-3
+
+        p.params, p.s0, p.s1 = kept[:2], kept[2:4], kept[4:]
+        p.grads = [torch.ones_like(x) for x in p.params]
+        numbers[:] = [Shortening(), 1e-3]
+        with pytest.raises(ValueError):
+            p.step(**{where: numbers})
+        assert all(torch.equal(x, y) for x, y in zip(before, (*kept, p.counter)))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_list_of_numbers_on_the_device(bits):
+    a, b = (Problem([(20, 30), (30,)], F32, bits, seed=8) for _ in range(2))
+    a.step(lr=[0.5, 0.25], weight_decay=(0.0, 0.125))
+    b.step(lr=[torch.tensor(0.5, device=DEV), 0.25], weight_decay=(0, torch.tensor(0.125, device=DEV)))
+    for x, y in zip(a.tensors(), b.tensors()):
+        assert torch.equal(x, y)
