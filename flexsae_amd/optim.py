@@ -327,6 +327,14 @@ def adamw8_moments(codes: Sequence[Tensor], absmax: Sequence[Tensor], dtype: tor
 # ---- the optimizer -------------------------------------------------------------------------
 
 
+def _not_captured(device: torch.device, what: str) -> None:
+    """Refuses what every replay of a captured step would do again."""
+    if device.type == "cuda":
+        with _on_device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"AdamW: a step in which {what} cannot be captured: take one with the same gradients first")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW of ``adamw_step`` / ``adamw8_step`` as an optimizer of torch's kind: parameter groups, schedulers, state_dict.
 
@@ -336,8 +344,9 @@ class AdamW(torch.optim.Optimizer):
     max_norm: the gradients of all groups are clipped to this norm together.  skip_nonfinite: a step whose gradients hold an
     infinity or NaN changes nothing, as always with max_norm.  After a step with either ``grad_norm`` is the norm of the gradients
     as they were, on the device.
-    Parameters without a gradient are left out of a step, their number of steps too.  Whoever changes 16-bit parameters with master
-    weights from outside calls ``reset_masters()``."""
+    Parameters without a gradient are left out of a step, their number of steps too.  A step is captured after one with gradients of
+    the same parameters, which makes their states.  Whoever changes 16-bit parameters with master weights from outside calls
+    ``reset_masters()``."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, unit_rows: bool = False, master_weights: bool = True,
@@ -390,6 +399,7 @@ class AdamW(torch.optim.Optimizer):
             if not s:
                 if g.is_sparse:
                     raise RuntimeError("AdamW takes dense gradients")
+                _not_captured(p.device, "a parameter's states begin")
                 if p.device not in new:
                     new[p.device] = adamw_counter(p.device)
                 s = state[p] = self._new_state(p, group, new[p.device])
@@ -404,6 +414,7 @@ class AdamW(torch.optim.Optimizer):
             cohort[4].append(s.get("master", p))
         for key, states in behind.items():
             if key in cohorts:
+                _not_captured(states[0]["counter"].device, "a parameter without a gradient gets a count of its own")
                 own = states[0]["counter"].clone()
                 for s in states:
                     s["counter"] = own

@@ -132,3 +132,57 @@ def test_a_list_of_numbers_on_the_device(bits):
     b.step(lr=[torch.tensor(0.5, device=DEV), 0.25], weight_decay=(0, torch.tensor(0.125, device=DEV)))
     for x, y in zip(a.tensors(), b.tensors()):
         assert torch.equal(x, y)
+
+
+# ---- capture -------------------------------------------------------------------------------
+
+
+def _capture(opt):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    return graph
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_capture_in_which_states_would_begin_is_refused(bits):
+    """Its replays would clear the states each time."""
+    m = _model()
+    opt = flex.AdamW(m, state_bits=bits)
+    _set_grads(m, 0)
+    with pytest.raises(RuntimeError, match="captur"):
+        _capture(opt)
+    assert not opt.state
+    before = [p.detach().clone() for p in m]
+    opt.step()
+    graph = _capture(opt)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(opt.state[m[0]]["counter"][0]) == 2 and not any(torch.equal(x, y) for x, y in zip(before, m))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_capture_that_leaves_a_parameter_behind(bits):
+    """The count of a parameter without a gradient stays what it was over all replays."""
+    a, b = _model(), _model()
+    opts = [flex.AdamW(x, lr=1e-2, state_bits=bits) for x in (a, b)]
+    for x, opt in zip((a, b), opts):
+        _set_grads(x, 0)
+        opt.step()
+        _set_grads(x, 1, but=(2,))
+    with pytest.raises(RuntimeError, match="captur"):
+        _capture(opts[1])
+    for opt in opts:
+        opt.step()
+    graph = _capture(opts[1])
+    for _ in range(3):
+        opts[0].step()
+        graph.replay()
+        torch.cuda.synchronize()
+    assert [int(opts[1].state[p]["counter"][0]) for p in b] == [5, 5, 1, 5]
+    for x, opt in zip((a, b), opts):
+        _set_grads(x, 2)
+        opt.step()
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+        assert int(opts[0].state[x]["counter"][0]) == int(opts[1].state[y]["counter"][0])
