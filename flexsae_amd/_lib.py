@@ -135,6 +135,7 @@ SIGNATURES = {
     "flexsae_grad_norm_workspace_bytes": (_sz, [_i64]),
     "flexsae_grad_norm": (_int, [ctypes.POINTER(Grad), _i64, _p, _p, _sz, _p]),
     "flexsae_adamw_step": (_int, [ctypes.POINTER(AdamwTensor), _i64, ctypes.POINTER(AdamwConfig), _p]),
+    "flexsae_adamw_check": (_int, [ctypes.POINTER(AdamwTensor), _i64, ctypes.POINTER(AdamwConfig)]),
     "flexsae_adamw8_moments": (_int, [ctypes.POINTER(Adamw8State), _i64, _int, _p]),
 }
 

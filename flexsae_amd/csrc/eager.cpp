@@ -39,7 +39,7 @@ using torch::autograd::variable_list;
   X(abi_version) X(fwd_workspace_bytes) X(topk_fwd_best_workspace_bytes) X(topk_fwd) X(hier_fwd)                        \
   X(topk_bwd_from_indices_workspace_bytes) X(topk_bwd_from_indices) X(hier_bwd_workspace_bytes) X(hier_bwd)             \
   X(hier_fwd_bwd_workspace_bytes_flags) X(hier_step) X(finish_grads)                                                    \
-  X(grad_norm_workspace_bytes) X(grad_norm) X(adamw_step) X(adamw8_moments)
+  X(grad_norm_workspace_bytes) X(grad_norm) X(adamw_step) X(adamw_check) X(adamw8_moments)
 struct Library {
 #define X(name) decltype(&flexsae_##name) name = nullptr;
   FLEXSAE_ENTRIES(X)
@@ -674,78 +674,133 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// adamw(bits, params, grads, state0s, state1s, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm,
-// max_norm, unit_rows) -> True
+// A step of AdamW: bits, params, grads, state0s, state1s, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale,
+// grad_norm, max_norm, unit_rows.  All numbers are read before any tensor is taken, and everything is looked at before the launch.
+constexpr Py_ssize_t kAdamwArguments = 16;
+class AdamwCall {
+ public:
+  void read_numbers(PyObject *const *args) {
+    eight_ = number(args[0]) == 8;
+    unit_ = number(args[15]) != 0;
+    device_lr_ = THPVariable_Check(args[7]);
+    numbers_ = (device_lr_ || lrs_.take(args[7])) && weight_decays_.take(args[8]);
+    config_ = {real(args[9]), real(args[10]), real(args[11]), static_cast<float>(real(args[12])), static_cast<float>(real(args[14])),
+               nullptr, nullptr, nullptr, eight_ ? 8 : 32, unit_ ? FLEXSAE_ADAMW_UNIT_ROWS : 0};
+  }
+
+  // False: not this module's business.  (Runs no Python code.)
+  bool take(PyObject *const *args) {
+    Tensors grads;
+    if (!numbers_ || !take_tensors(args[1], params_, device_) || params_.empty() || !take_tensors(args[2], grads, device_) ||
+        !take_tensors(args[3], s0_, device_) || !take_tensors(args[4], s1_, device_) ||
+        (args[5] != Py_None && !take_tensors(args[5], masters_, device_)))
+      return false;
+    const size_t count = params_.size();
+    if (grads.size() != count || s0_.size() != count || s1_.size() != count || (args[5] != Py_None && masters_.size() != count) ||
+        (!device_lr_ && !lrs_.serve(count)) || !weight_decays_.serve(count) || !THPVariable_Check(args[6]))
+      return false;
+    counter_ = &THPVariable_Unpack(args[6]);
+    if (!plain_tensor(*counter_) || counter_->device() != *device_ || counter_->scalar_type() != c10::ScalarType::Long ||
+        counter_->numel() != 2 || !changeable(*counter_))
+      return false;
+    if ((device_lr_ && !take_scalar(args[7], *device_, lr_)) || !take_scalar(args[13], *device_, norm_)) return false;
+    const c10::AutoGradMode no_grad(false);
+    const c10::DeviceGuard guard(*device_);
+    list_.resize(count);
+    for (size_t i = 0; i < count; ++i) {
+      const Tensor &p = *params_[i], &g = *grads[i], &a = *s0_[i], &b = *s1_[i];
+      const int dtype = dtype_of(p.scalar_type());
+      if (dtype < 0 || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || !changeable(p) || !changeable(a) ||
+          !changeable(b) || (unit_ && p.dim() < 2))
+        return false;
+      const int64_t numel = p.numel(), cols = unit_ ? p.size(-1) : numel, rows = unit_ ? (cols ? numel / cols : 0) : 1;
+      if (eight_) {
+        const at::IntArrayRef sizes = a.sizes();
+        if (a.scalar_type() != c10::ScalarType::Byte || b.scalar_type() != c10::ScalarType::Float || a.dim() != p.dim() + 1 ||
+            sizes.back() != 2 || sizes.slice(0, sizes.size() - 1) != p.sizes() || b.dim() != 3 || b.size(0) != rows ||
+            b.size(1) != (cols + 255) / 256 || b.size(2) != 2 || reinterpret_cast<uintptr_t>(b.const_data_ptr()) % 8 ||
+            reinterpret_cast<uintptr_t>(a.const_data_ptr()) % 2)
+          return false;
+      } else if (a.scalar_type() != c10::ScalarType::Float || b.scalar_type() != c10::ScalarType::Float || a.sizes() != p.sizes() ||
+                 b.sizes() != p.sizes()) {
+        return false;
+      }
+      void *master = nullptr;
+      if (!masters_.empty() && dtype != FLEXSAE_F32) {
+        if (masters_[i]->scalar_type() != c10::ScalarType::Float || masters_[i]->sizes() != p.sizes() || !changeable(*masters_[i]))
+          return false;
+        master = masters_[i]->data_ptr();
+      }
+      if (!g.is_contiguous()) copies_.push_back(g.contiguous());
+      list_[i] = {p.data_ptr(), (g.is_contiguous() ? g : copies_.back()).const_data_ptr(), master, a.data_ptr(), b.data_ptr(), rows, cols,
+                  device_lr_ ? 1.f : lrs_.at(i), weight_decays_.at(i), dtype};
+    }
+    config_.grad_norm = norm_.defined() ? f32(norm_) : nullptr;
+    config_.lr = lr_.defined() ? f32(lr_) : nullptr;
+    config_.counter = counter_->data_ptr<int64_t>();
+    return true;
+  }
+
+  int check_alone() const { return lib.adamw_check(list_.data(), static_cast<int64_t>(list_.size()), &config_); }
+
+  int launch() {
+    const c10::DeviceGuard guard(*device_);
+    const int status = lib.adamw_step(list_.data(), static_cast<int64_t>(list_.size()), &config_, stream_of(*counter_));
+    if (status == FLEXSAE_OK || status == FLEXSAE_ERR_LAUNCH) {
+      for (const auto *changed : {&params_, &s0_, &s1_, &masters_})
+        for (const Tensor *t : *changed) t->unsafeGetTensorImpl()->bump_version();
+      counter_->unsafeGetTensorImpl()->bump_version();
+    }
+    return status;
+  }
+
+ private:
+  bool eight_ = false, unit_ = false, device_lr_ = false, numbers_ = false;
+  Reals lrs_, weight_decays_;
+  flexsae_adamw_config config_{};
+  Tensors params_, s0_, s1_, masters_;
+  c10::optional<c10::Device> device_;
+  const Tensor *counter_ = nullptr;
+  Tensor lr_, norm_;
+  std::vector<flexsae_adamw_tensor> list_;
+  std::vector<Tensor> copies_;  // of gradients that are not contiguous
+};
+
+// adamw(the arguments of an AdamwCall) -> True
 PyObject *py_adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arguments(n, 16)) return nullptr;
+  if (!arguments(n, kAdamwArguments)) return nullptr;
   if (!plain_surroundings()) Py_RETURN_NONE;
-  const bool eight = number(args[0]) == 8, unit = number(args[15]) != 0, device_lr = THPVariable_Check(args[7]);
-  Reals lrs, weight_decays;
-  if ((!device_lr && !lrs.take(args[7])) || !weight_decays.take(args[8])) Py_RETURN_NONE;
-  flexsae_adamw_config config = {real(args[9]), real(args[10]), real(args[11]), static_cast<float>(real(args[12])),
-                                 static_cast<float>(real(args[14])), nullptr, nullptr, nullptr, eight ? 8 : 32,
-                                 unit ? FLEXSAE_ADAMW_UNIT_ROWS : 0};
-  // (no Python code runs from here on)
-  Tensors params, grads, s0, s1, masters;
-  c10::optional<c10::Device> device;
-  if (!take_tensors(args[1], params, device) || params.empty() || !take_tensors(args[2], grads, device) ||
-      !take_tensors(args[3], s0, device) || !take_tensors(args[4], s1, device) ||
-      (args[5] != Py_None && !take_tensors(args[5], masters, device)))
-    Py_RETURN_NONE;
-  const size_t count = params.size();
-  if (grads.size() != count || s0.size() != count || s1.size() != count || (args[5] != Py_None && masters.size() != count) ||
-      (!device_lr && !lrs.serve(count)) || !weight_decays.serve(count) || !THPVariable_Check(args[6]))
-    Py_RETURN_NONE;
-  const Tensor &counter = THPVariable_Unpack(args[6]);
-  if (!plain_tensor(counter) || counter.device() != *device || counter.scalar_type() != c10::ScalarType::Long ||
-      counter.numel() != 2 || !changeable(counter))
-    Py_RETURN_NONE;
-  Tensor lr, norm;
-  if ((device_lr && !take_scalar(args[7], *device, lr)) || !take_scalar(args[13], *device, norm)) Py_RETURN_NONE;
-  const c10::AutoGradMode no_grad(false);
-  const c10::DeviceGuard guard(*device);
-  std::vector<flexsae_adamw_tensor> list(count);
-  std::vector<Tensor> copies;
-  for (size_t i = 0; i < count; ++i) {
-    const Tensor &p = *params[i], &g = *grads[i], &a = *s0[i], &b = *s1[i];
-    const int dtype = dtype_of(p.scalar_type());
-    if (dtype < 0 || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || !changeable(p) || !changeable(a) ||
-        !changeable(b) || (unit && p.dim() < 2))
-      Py_RETURN_NONE;
-    const int64_t numel = p.numel(), cols = unit ? p.size(-1) : numel, rows = unit ? (cols ? numel / cols : 0) : 1;
-    if (eight) {
-      const at::IntArrayRef sizes = a.sizes();
-      if (a.scalar_type() != c10::ScalarType::Byte || b.scalar_type() != c10::ScalarType::Float || a.dim() != p.dim() + 1 ||
-          sizes.back() != 2 || sizes.slice(0, sizes.size() - 1) != p.sizes() || b.dim() != 3 || b.size(0) != rows ||
-          b.size(1) != (cols + 255) / 256 || b.size(2) != 2 || reinterpret_cast<uintptr_t>(b.const_data_ptr()) % 8 ||
-          reinterpret_cast<uintptr_t>(a.const_data_ptr()) % 2)
-        Py_RETURN_NONE;
-    } else if (a.scalar_type() != c10::ScalarType::Float || b.scalar_type() != c10::ScalarType::Float || a.sizes() != p.sizes() ||
-               b.sizes() != p.sizes()) {
-      Py_RETURN_NONE;
-    }
-    void *master = nullptr;
-    if (!masters.empty() && dtype != FLEXSAE_F32) {
-      if (masters[i]->scalar_type() != c10::ScalarType::Float || masters[i]->sizes() != p.sizes() || !changeable(*masters[i]))
-        Py_RETURN_NONE;
-      master = masters[i]->data_ptr();
-    }
-    if (!g.is_contiguous()) copies.push_back(g.contiguous());
-    list[i] = {p.data_ptr(), (g.is_contiguous() ? g : copies.back()).const_data_ptr(), master, a.data_ptr(), b.data_ptr(), rows, cols,
-               device_lr ? 1.f : lrs.at(i), weight_decays.at(i), dtype};
-  }
-  config.grad_norm = norm.defined() ? f32(norm) : nullptr;
-  config.lr = lr.defined() ? f32(lr) : nullptr;
-  config.counter = counter.data_ptr<int64_t>();
-  const int status = lib.adamw_step(list.data(), static_cast<int64_t>(count), &config, stream_of(counter));
+  AdamwCall call;
+  call.read_numbers(args);
+  if (!call.take(args)) Py_RETURN_NONE;
+  const int status = call.launch();
   if (status == FLEXSAE_ERR_INVALID_ARGUMENT) Py_RETURN_NONE;  // nothing was launched; optim.py says what is wrong
-  if (status == FLEXSAE_OK || status == FLEXSAE_ERR_LAUNCH) {
-    for (const auto *changed : {&params, &s0, &s1, &masters})
-      for (const Tensor *t : *changed) t->unsafeGetTensorImpl()->bump_version();
-    counter.unsafeGetTensorImpl()->bump_version();
-  }
   check(status, "flexsae_adamw_step");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw_all([the arguments of an AdamwCall, as a tuple, ...]) -> True: all of the steps, or, where one is refused, none
+PyObject *py_adamw_all(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arguments(n, 1)) return nullptr;
+  if (!plain_surroundings() || !PyList_CheckExact(args[0])) Py_RETURN_NONE;
+  std::vector<pybind11::object> tuples;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); ++i) {
+    tuples.push_back(pybind11::reinterpret_borrow<pybind11::object>(PyList_GET_ITEM(args[0], i)));
+    if (!PyTuple_CheckExact(tuples.back().ptr()) || PyTuple_GET_SIZE(tuples.back().ptr()) != kAdamwArguments) Py_RETURN_NONE;
+  }
+  std::vector<AdamwCall> calls(tuples.size());
+  for (size_t i = 0; i < calls.size(); ++i) calls[i].read_numbers(PySequence_Fast_ITEMS(tuples[i].ptr()));
+  for (size_t i = 0; i < calls.size(); ++i)
+    if (!calls[i].take(PySequence_Fast_ITEMS(tuples[i].ptr()))) Py_RETURN_NONE;
+  for (const AdamwCall &call : calls) {
+    const int status = call.check_alone();
+    if (status == FLEXSAE_ERR_INVALID_ARGUMENT) Py_RETURN_NONE;
+    check(status, "flexsae_adamw_check");
+  }
+  for (AdamwCall &call : calls) check(call.launch(), "flexsae_adamw_step");
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -835,7 +890,8 @@ PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyMethodDef methods[] = {FLEXSAE_METHOD(init),       FLEXSAE_METHOD(set_flag),    FLEXSAE_METHOD(settings),
                          FLEXSAE_METHOD(topk_loss),  FLEXSAE_METHOD(hier_loss),   FLEXSAE_METHOD(hier_sliced),
                          FLEXSAE_METHOD(hier_late),  FLEXSAE_METHOD(hier_sgd),    FLEXSAE_METHOD(grad_norm),
-                         FLEXSAE_METHOD(adamw),      FLEXSAE_METHOD(adamw8_moments), {nullptr, nullptr, 0, nullptr}};
+                         FLEXSAE_METHOD(adamw),      FLEXSAE_METHOD(adamw_all),   FLEXSAE_METHOD(adamw8_moments),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_eager", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

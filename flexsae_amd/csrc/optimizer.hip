@@ -177,7 +177,7 @@ int launch_norms(const flexsae_grad *grads, int64_t count, double *partial, int6
 
 extern "C" {
 
-int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const flexsae_adamw_config *config, void *stream) {
+int flexsae_adamw_check(const flexsae_adamw_tensor *tensors, int64_t count, const flexsae_adamw_config *config) {
   if (const int rc = check_config(config)) return rc;
   if (count < 0 || (count > 0 && !tensors)) return FLEXSAE_ERR_INVALID_ARGUMENT;
   if (config->flags & ~FLEXSAE_ADAMW_UNIT_ROWS) return FLEXSAE_ERR_INVALID_ARGUMENT;
@@ -187,6 +187,12 @@ int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const
     if (tensors[i].rows == 0 || tensors[i].cols == 0) continue;
     if (work_of(tensors[i], eight, unit).tiles > kMostTiles) return FLEXSAE_ERR_UNSUPPORTED;
   }
+  return FLEXSAE_OK;
+}
+
+int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const flexsae_adamw_config *config, void *stream) {
+  if (const int rc = flexsae_adamw_check(tensors, count, config)) return rc;
+  const bool eight = config->state_bits == 8, unit = config->flags & FLEXSAE_ADAMW_UNIT_ROWS;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   AdamwTable a = table_of(*config);
   // (of a beta of zero: minus infinity, whose exponential is zero)

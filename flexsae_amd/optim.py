@@ -212,8 +212,8 @@ def _(*args):
 _Reals = Union[float, Sequence[float]]
 
 
-def _call(bits, op, params, grads, state0, state1, counter, lr, beta1, beta2, eps, weight_decay, masters, unit_rows, grad_norm,
-          max_norm, grad_scale) -> None:
+def _call(bits, params, grads, state0, state1, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm,
+          max_norm, unit_rows) -> None:
     if isinstance(params, Tensor) or len(params) == 0:
         raise ValueError("expected a list of at least one parameter")
     if masters is not None and len(masters) == 0:
@@ -223,6 +223,16 @@ def _call(bits, op, params, grads, state0, state1, counter, lr, beta1, beta2, ep
     if native is not None and native.adamw(bits, params, grads, state0, state1, masters, counter, lr, weight_decay, beta1, beta2,
                                            eps, grad_scale, grad_norm, max_norm, unit_rows):
         return
+    with torch.no_grad():
+        args = _checked(bits, params, grads, state0, state1, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale,
+                        grad_norm, max_norm, unit_rows)
+        op = _adamw_op if bits == 32 else _adamw8_op
+        op(*([t.detach() for t in a] if i < 5 else a for i, a in enumerate(args)))
+
+
+def _checked(bits, params, grads, state0, state1, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm,
+             max_norm, unit_rows) -> tuple:
+    """The op's arguments, which are those of a step."""
     n = len(params)
     on_device = isinstance(lr, Tensor)
     lrs = [1.0] * n if on_device else [float(lr)] * n if isinstance(lr, (int, float)) else [float(x) for x in lr]
@@ -233,11 +243,21 @@ def _call(bits, op, params, grads, state0, state1, counter, lr, beta1, beta2, ep
         raise ValueError(f"{n} params and {len(masters)} masters")
     else:
         masters = [m for m, p in zip(masters, params) if p.dtype != torch.float32]
-    with torch.no_grad():
-        args = (params, grads, state0, state1, masters, counter, lrs, wds, lr if on_device else None, grad_norm,
-                float(beta1), float(beta2), float(eps), float(grad_scale), float(max_norm), bool(unit_rows))
-        _check_step(bits, *args)
-        op(*([t.detach() for t in a] if i < 5 else a for i, a in enumerate(args)))
+    args = (params, grads, state0, state1, masters, counter, lrs, wds, lr if on_device else None, grad_norm,
+            float(beta1), float(beta2), float(eps), float(grad_scale), float(max_norm), bool(unit_rows))
+    _check_step(bits, *args)
+    return args
+
+
+def _call_all(calls) -> None:
+    """Steps, each given as the arguments of ``_call``: all of them, or none where one is refused."""
+    native = _native(calls[0][1][0])
+    if native is not None and native.adamw_all(calls):
+        return
+    for call in calls:
+        _checked(*call)
+    for call in calls:
+        _call(*call)
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor], exp_avg_sqs: Sequence[Tensor],
@@ -261,8 +281,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     by it.  grad_scale: the loss scale that the gradients carry.
     Arithmetic is in fp32; a weight without a master is rounded once.  The gradients are left as they are.  With ``eps=0`` an
     element without any gradient so far stays where it is."""
-    _call(32, _adamw_op, params, grads, exp_avgs, exp_avg_sqs, counter, lr, beta1, beta2, eps, weight_decay, masters, unit_rows,
-          grad_norm, max_norm, grad_scale)
+    _call(32, params, grads, exp_avgs, exp_avg_sqs, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm,
+          max_norm, unit_rows)
 
 
 def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], codes: Sequence[Tensor], absmax: Sequence[Tensor],
@@ -274,8 +294,8 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], codes: Sequen
     ``a`` the block's maxima of \\|m\\| and of v, the bytes c stand for ``sign(c - 128) ((c - 128) / 127)^2 a`` and
     ``(c / 255)^4 a``, rounded to the nearest on the root's scale; a v above zero never becomes zero.  The step itself uses m and v
     before they are rounded.  A block with an infinity or NaN in m or v has NaN there from then on."""
-    _call(8, _adamw8_op, params, grads, codes, absmax, counter, lr, beta1, beta2, eps, weight_decay, masters, unit_rows,
-          grad_norm, max_norm, grad_scale)
+    _call(8, params, grads, codes, absmax, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm, max_norm,
+          unit_rows)
 
 
 # ---- the values of 8-bit states ------------------------------------------------------------
@@ -432,18 +452,22 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls = [(group, cohort) for group in self.param_groups for cohort in self._cohorts(group)]
-        if not calls:
+        cohorts = [(group, cohort) for group in self.param_groups for cohort in self._cohorts(group)]
+        if not cohorts:
             return loss
         norm = None
         if self.max_norm is not None or self.skip_nonfinite:
-            norm = self.grad_norm = grad_norm([g for _, cohort in calls for g in cohort[1]])
-        for group, (params, grads, first, second, masters, counter) in calls:
-            eight = group["state_bits"] == 8
+            norm = self.grad_norm = grad_norm([g for _, cohort in cohorts for g in cohort[1]])
+        calls = []
+        for group, (params, grads, first, second, masters, counter) in cohorts:
             beta1, beta2 = group["betas"]
-            _call(8 if eight else 32, _adamw8_op if eight else _adamw_op, params, grads, first, second, counter, group["lr"], beta1,
-                  beta2, group["eps"], group["weight_decay"], masters if group["master_weights"] else None, group["unit_rows"],
-                  norm, self.max_norm, grad_scale)
+            calls.append((group["state_bits"], params, grads, first, second, masters if group["master_weights"] else None, counter,
+                          group["lr"], group["weight_decay"], beta1, beta2, group["eps"], grad_scale, norm, self.max_norm or 0.0,
+                          group["unit_rows"]))
+        if len(calls) == 1:
+            _call(*calls[0])
+        else:
+            _call_all(calls)
         return loss
 
     def moments(self, p: Tensor, dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:

@@ -536,6 +536,10 @@ typedef struct {
  */
 int flexsae_adamw_step(const flexsae_adamw_tensor *tensors, int64_t count, const flexsae_adamw_config *config, void *stream);
 
+/* What flexsae_adamw_step refuses before it launches anything, without the step: for programs that make several calls and
+ * none of them where one is refused. */
+int flexsae_adamw_check(const flexsae_adamw_tensor *tensors, int64_t count, const flexsae_adamw_config *config);
+
 /* 8-bit states of rows * cols elements, rows as in state1 above (1 where the blocks are those of the whole tensor). */
 typedef struct {
   const void *codes;

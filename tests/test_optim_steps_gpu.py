@@ -186,3 +186,39 @@ def test_a_capture_that_leaves_a_parameter_behind(bits):
     for x, y in zip(a, b):
         assert torch.equal(x, y)
         assert int(opts[0].state[x]["counter"][0]) == int(opts[1].state[y]["counter"][0])
+
+
+# ---- groups --------------------------------------------------------------------------------
+
+
+def _break(opt, how):
+    group = opt.param_groups[1]
+    if how == "lr":
+        group["lr"] = -1.0
+    elif how == "lr on the device":
+        group["lr"] = torch.ones((), dtype=torch.float64, device=DEV)
+    elif how == "betas":
+        group["betas"] = (0.9, 1.0)
+    elif how == "state":
+        s = opt.state[group["params"][1]]
+        key = "exp_avg" if "exp_avg" in s else "codes"
+        s[key] = s[key][:1]
+    elif how == "unit rows":
+        group["unit_rows"] = True
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["lr", "lr on the device", "betas", "state", "unit rows"])
+def test_a_group_that_is_refused_leaves_the_others_unstepped(bits, how):
+    m = _model()
+    opt = flex.AdamW([{"params": m[:2]}, {"params": m[2:]}], state_bits=bits)
+    _set_grads(m, 0)
+    opt.step()
+    _break(opt, how)
+    before = [p.detach().clone() for p in m]
+    states = [{k: t.clone() for k, t in opt.state[p].items()} for p in m]
+    with pytest.raises(ValueError):
+        opt.step()
+    for p, x, s in zip(m, before, states):
+        assert torch.equal(p, x)
+        assert all(torch.equal(t, opt.state[p][k]) for k, t in s.items())
