@@ -747,8 +747,10 @@ class AdamwCall {
     const c10::DeviceGuard guard(*device_);
     const int status = lib.adamw_step(list_.data(), static_cast<int64_t>(list_.size()), &config_, stream_of(*counter_));
     if (status == FLEXSAE_OK || status == FLEXSAE_ERR_LAUNCH) {
-      for (const auto *changed : {&params_, &s0_, &s1_, &masters_})
+      for (const auto *changed : {&params_, &s0_, &s1_})
         for (const Tensor *t : *changed) t->unsafeGetTensorImpl()->bump_version();
+      for (size_t i = 0; i < masters_.size(); ++i)  // (that of an fp32 parameter is ignored)
+        if (list_[i].master != nullptr) masters_[i]->unsafeGetTensorImpl()->bump_version();
       counter_->unsafeGetTensorImpl()->bump_version();
     }
     return status;

@@ -222,3 +222,21 @@ def test_a_group_that_is_refused_leaves_the_others_unstepped(bits, how):
     for p, x, s in zip(m, before, states):
         assert torch.equal(p, x)
         assert all(torch.equal(t, opt.state[p][k]) for k, t in s.items())
+
+
+# ---- masters of fp32 parameters ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_ignored_master_is_left_alone(bits):
+    """... its version too, and whatever stands there: one of inference mode has none."""
+    p = Problem([(20, 30), (30,), (40,)], [F32, F16, F32], bits, master=True)
+    with torch.inference_mode():
+        p.masters[2] = torch.ones(7, device=DEV)
+    first, version = p.masters[0].clone(), p.masters[0]._version
+    versions = [p.masters[1]._version, *(x._version for x in p.params)]
+    p.step()
+    assert p.masters[0]._version == version and torch.equal(p.masters[0], first)
+    assert bool((p.masters[2] == 1).all())
+    assert all(x._version > v for x, v in zip([p.masters[1], *p.params], versions))
+    assert int(p.counter[0]) == 8
