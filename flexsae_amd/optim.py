@@ -472,7 +472,9 @@ class AdamW(torch.optim.Optimizer):
 
     def moments(self, p: Tensor, dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:
         """The first and second moment of a parameter that has been stepped, in ``dtype``."""
-        s = self.state[p]
+        s = self.state.get(p)
+        if not s:
+            raise KeyError("moments: the parameter has not been stepped")
         if "codes" in s:
             m, v = adamw8_moments([s["codes"]], [s["absmax"]], dtype)
             return m[0], v[0]

@@ -2,7 +2,9 @@
 import ctypes
 
 import pytest
+import torch
 
+import flexsae_amd as flex
 from flexsae_amd import _lib
 from tests.test_optim_host import FAKE, _config, _step, _tensor
 
@@ -27,3 +29,12 @@ def test_a_check_launches_nothing():
         assert lib.flexsae_adamw_check(table, 2, ctypes.byref(_config(state_bits=bits, flags=flags))) == _lib.OK
     assert lib.flexsae_adamw_check(None, 0, ctypes.byref(_config())) == _lib.OK
     assert lib.flexsae_adamw_check(None, 1, ctypes.byref(_config())) == _lib.ERR_INVALID_ARGUMENT
+
+
+def test_asking_for_moments_before_a_step_begins_no_state():
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = flex.AdamW([p])
+    with pytest.raises(KeyError, match="not been stepped"):
+        opt.moments(p)
+    assert not opt.state
+    opt.load_state_dict(opt.state_dict())
