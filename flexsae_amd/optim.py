@@ -131,6 +131,9 @@ def _check_step(bits, params, grads, state0, state1, masters, counter, lrs, weig
         master = next(master_of) if masters and p.dtype != torch.float32 else None
         if master is not None and (master.dtype != torch.float32 or master.shape != p.shape):
             raise ValueError(f"the master of params[{i}] is {master.dtype} {tuple(master.shape)}, expected float32 {tuple(p.shape)}")
+    for t in (*params, *state0, *state1, *masters):
+        if any(n > 1 and step == 0 for n, step in zip(t.shape, t.stride())):
+            raise ValueError(f"a tensor of shape {tuple(t.shape)} and strides {t.stride()} has one memory for several elements")
     if counter.dtype != torch.int64 or counter.numel() != 2 or not counter.is_contiguous():
         raise ValueError("counter: expected int64[2] (adamw_counter)")
     for name, t in (("lr", lr), ("grad_norm", grad_norm)):

@@ -240,3 +240,27 @@ def test_an_ignored_master_is_left_alone(bits):
     assert bool((p.masters[2] == 1).all())
     assert all(x._version > v for x, v in zip([p.masters[1], *p.params], versions))
     assert int(p.counter[0]) == 8
+
+
+# ---- refusals ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_expanded_tensors_are_refused_before_the_step(bits):
+    for which in ("params", "s0", "s1", "masters"):
+        p = Problem([(4, 600), (7,)], F16, bits, master=True)
+        x = getattr(p, which)[0]
+        getattr(p, which)[0] = x[..., :1].expand(x.shape)
+        before = [t.clone() for t in p.tensors()]
+        with pytest.raises(ValueError, match="one memory"):
+            p.step()
+        assert all(torch.equal(x, y) for x, y in zip(before, p.tensors())), which
+    # (gradients are read alone: that of a sum is one number)
+    a, b = (Problem([(4, 600)], F32, bits, seed=3) for _ in range(2))
+    a.grads = [torch.ones((), device=DEV).expand(4, 600)]
+    b.grads = [torch.ones(4, 600, device=DEV)]
+    assert torch.equal(flex.grad_norm(a.grads), flex.grad_norm(b.grads))
+    for p in (a, b):
+        p.step()
+    for x, y in zip(a.tensors(), b.tensors()):
+        assert torch.equal(x, y)
