@@ -496,19 +496,33 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """As torch's, with states kept in their own types (torch's own would turn them into the parameter's).  Parameters of a
         group that have taken the same number of steps share a count again."""
-        saved = state_dict["state"]
-        if any("counter" not in s for s in saved.values()):
-            raise ValueError("load_state_dict: the states are not those of this optimizer")
-        super().load_state_dict({**state_dict, "state": {}})
-        for group, old in zip(self.param_groups, state_dict["param_groups"]):
-            counters = {}
-            for p, key in zip(group["params"], old["params"]):
-                if key not in saved:
-                    continue
-                s = {k: v.detach().to(p.device).clone() if isinstance(v, Tensor) else v for k, v in saved[key].items()}
-                counter = s["counter"]
-                s["counter"] = counters.setdefault((p.device, int(counter[0])), counter)
-                self.state[p] = s
+        loaded = {}
+
+        def take(_, state_dict):  # what the hooks before it have left: the groups are torch's business
+            if any("counter" not in s for s in state_dict["state"].values()):
+                raise ValueError("load_state_dict: the states are not those of this optimizer")
+            loaded.update(state_dict)
+            return {**state_dict, "state": {}}
+
+        def fill(_):
+            saved = loaded["state"]
+            for group, old in zip(self.param_groups, loaded["param_groups"]):
+                counters = {}
+                for p, key in zip(group["params"], old["params"]):
+                    if key not in saved:
+                        continue
+                    s = {k: v.detach().to(p.device).clone() if isinstance(v, Tensor) else v for k, v in saved[key].items()}
+                    counter = s["counter"]
+                    s["counter"] = counters.setdefault((p.device, int(counter[0])), counter)
+                    self.state[p] = s
+
+        before = self.register_load_state_dict_pre_hook(take)  # (the last of them)
+        after = self.register_load_state_dict_post_hook(fill, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            before.remove()
+            after.remove()
 
 
 @torch._disable_dynamo  # (torch.compiler.disable, but for the compiler's import here)

@@ -38,3 +38,50 @@ def test_asking_for_moments_before_a_step_begins_no_state():
         opt.moments(p)
     assert not opt.state
     opt.load_state_dict(opt.state_dict())
+
+
+def _stepped(dtype=torch.bfloat16):
+    """An optimizer as after a step (no GPU)."""
+    params = [torch.nn.Parameter(torch.ones(n, 4, dtype=dtype)) for n in (2, 3)]
+    opt = flex.AdamW(params)
+    counter = torch.tensor([5, 0])
+    for i, p in enumerate(params):
+        opt.state[p] = opt._new_state(p, opt.param_groups[0], counter)
+        opt.state[p]["exp_avg"].fill_(1.0 + 2.0 ** -20 + i)
+    return opt
+
+
+def test_hooks_of_loading_states():
+    one, two = _stepped(), _stepped()
+    seen = []
+
+    def before(opt, state_dict):
+        seen.append("before")
+        state = {k: {**s, "exp_avg": s["exp_avg"] * 2} for k, s in state_dict["state"].items()}
+        return {**state_dict, "state": state}
+
+    def after(opt):
+        seen.append(float(opt.state[opt.param_groups[0]["params"][1]]["exp_avg"][0, 0]))
+
+    two.register_load_state_dict_pre_hook(before)
+    two.register_load_state_dict_post_hook(after)
+    for _ in range(2):
+        two.load_state_dict(one.state_dict())
+    assert seen == ["before", 2 * (2 + 2.0 ** -20)] * 2
+    first, second = two.param_groups[0]["params"]
+    assert float(two.state[first]["exp_avg"][0, 0]) == 2 * (1 + 2.0 ** -20)
+    assert two.state[first]["exp_avg"].dtype == torch.float32 and two.state[first]["master"].dtype == torch.float32
+    assert two.state[first]["counter"] is two.state[second]["counter"] and two.state[first]["counter"].tolist() == [5, 0]
+
+
+def test_a_refused_load_leaves_the_states():
+    one, its = _stepped(), torch.optim.AdamW([torch.nn.Parameter(torch.ones(n, 4)) for n in (2, 3)])
+    for p in its.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    its.step()
+    state, groups = dict(one.state), [dict(g) for g in one.param_groups]
+    with pytest.raises(ValueError, match="not those of this optimizer"):
+        one.load_state_dict(its.state_dict())
+    assert dict(one.state) == state and [dict(g) for g in one.param_groups] == groups
+    one.load_state_dict(_stepped().state_dict())  # (and the next one is loaded)
+    assert one.state[one.param_groups[0]["params"][0]]["counter"].tolist() == [5, 0]
