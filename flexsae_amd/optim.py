@@ -350,6 +350,9 @@ def adamw8_moments(codes: Sequence[Tensor], absmax: Sequence[Tensor], dtype: tor
 # ---- the optimizer -------------------------------------------------------------------------
 
 
+_OPTIONS = ("lr", "betas", "eps", "weight_decay", "state_bits", "unit_rows", "master_weights")  # of a group
+
+
 def _not_captured(device: torch.device, what: str) -> None:
     """Refuses what every replay of a captured step would do again."""
     if device.type == "cuda":
@@ -499,7 +502,8 @@ class AdamW(torch.optim.Optimizer):
         loaded = {}
 
         def take(_, state_dict):  # what the hooks before it have left: the groups are torch's business
-            if any("counter" not in s for s in state_dict["state"].values()):
+            if (any("counter" not in s for s in state_dict["state"].values())
+                    or any(k not in group for group in state_dict["param_groups"] for k in _OPTIONS)):
                 raise ValueError("load_state_dict: the states are not those of this optimizer")
             loaded.update(state_dict)
             return {**state_dict, "state": {}}

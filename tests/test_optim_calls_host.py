@@ -85,3 +85,16 @@ def test_a_refused_load_leaves_the_states():
     assert dict(one.state) == state and [dict(g) for g in one.param_groups] == groups
     one.load_state_dict(_stepped().state_dict())  # (and the next one is loaded)
     assert one.state[one.param_groups[0]["params"][0]]["counter"].tolist() == [5, 0]
+
+
+def test_options_of_another_optimizer_are_refused():
+    """Its states are none yet: its groups would leave this one without options."""
+    its = torch.optim.AdamW([torch.nn.Parameter(torch.ones(n, 4)) for n in (2, 3)])
+    one = _stepped()
+    state, groups = dict(one.state), [dict(g) for g in one.param_groups]
+    with pytest.raises(ValueError, match="not those of this optimizer"):
+        one.load_state_dict(its.state_dict())
+    assert dict(one.state) == state and [dict(g) for g in one.param_groups] == groups
+    fresh = flex.AdamW([torch.nn.Parameter(torch.ones(n, 4)) for n in (2, 3)], lr=0.5, state_bits=8)
+    one.load_state_dict(fresh.state_dict())
+    assert one.param_groups[0]["state_bits"] == 8 and one.param_groups[0]["lr"] == 0.5 and not one.state
