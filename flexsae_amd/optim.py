@@ -283,7 +283,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     grad_norm: ``grad_norm(grads)``; one that is not finite makes the call change nothing, ``counter`` neither.  max_norm: clips
     by it.  grad_scale: the loss scale that the gradients carry.
     Arithmetic is in fp32; a weight without a master is rounded once.  The gradients are left as they are.  With ``eps=0`` an
-    element without any gradient so far stays where it is."""
+    element without any gradient so far stays where it is.  No two of the tensors that a call changes may share memory."""
     _call(32, params, grads, exp_avgs, exp_avg_sqs, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm,
           max_norm, unit_rows)
 
@@ -394,6 +394,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("expected 0 <= betas < 1, eps >= 0 and weight_decay >= 0")
             if not isinstance(group["lr"], Tensor) and not group["lr"] >= 0:
                 raise ValueError(f"lr must not be negative, got {group['lr']}")
+            if len(set(group["params"])) != len(group["params"]):
+                raise ValueError("a parameter stands twice in a group: one step would change it in two places at once")
             if group["unit_rows"] and any(p.dim() < 2 for p in group["params"]):
                 raise ValueError("unit_rows: expected matrices")
         except ValueError:

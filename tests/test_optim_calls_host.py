@@ -98,3 +98,15 @@ def test_options_of_another_optimizer_are_refused():
     fresh = flex.AdamW([torch.nn.Parameter(torch.ones(n, 4)) for n in (2, 3)], lr=0.5, state_bits=8)
     one.load_state_dict(fresh.state_dict())
     assert one.param_groups[0]["state_bits"] == 8 and one.param_groups[0]["lr"] == 0.5 and not one.state
+
+
+def test_a_parameter_twice_in_a_group_is_refused():
+    """(Between groups torch refuses it.)"""
+    p, q = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
+    with pytest.raises(ValueError, match="twice"), pytest.warns(UserWarning):
+        flex.AdamW([p, q, p])
+    opt = flex.AdamW([q])
+    with pytest.raises(ValueError, match="twice"), pytest.warns(UserWarning):
+        opt.add_param_group({"params": [p, p]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [p]})
