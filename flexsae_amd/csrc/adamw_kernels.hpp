@@ -334,7 +334,7 @@ __device__ __forceinline__ Maxima maxima(const float (&m)[N], const float (&v)[N
   for (int j = 0; j < N; ++j) bv = max(bv, __float_as_uint(v[j]));
   if constexpr (N == 4) {
     // After the first exchange even lanes carry m's and odd lanes v's, so that the other exchanges and the inverses serve both:
-    // what a block costs is shared by few elements (24571 x 1538 fp32 150 -> 147 us, 2.1M fp32 11.6 -> 11.0).  With eight the registers
+    // what a block costs is shared by few elements (24571 x 1538 fp32 122 -> 118 us, 2.1M fp32 11.0 -> 10.7).  With eight the registers
     // it takes cost more (302M bf16 512 -> 536 us).
     uint32_t bm = 0;
 #pragma unroll
@@ -434,7 +434,7 @@ __device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N],
   const bool all = !rooted(a.v);
 #pragma unroll
   for (int j = 0; j < N; j += 2) {
-    // (one wavefront in 40 has such an element)
+    // (one such pair of a wavefront in 30 to 50: 128 elements, each with 1.1e-6 of its code of v, and half of that of m's, between)
     const bool near = codes_of_two<false>(m + j, v + j, a, least, s + j, c.w[j / 2]);
     if (__any(near || all)) (void)codes_of_two<true>(m + j, v + j, a, least, s + j, c.w[j / 2]);
   }
@@ -615,13 +615,13 @@ __device__ __forceinline__ float row_sum(float x, float (*place)[16], int turn) 
   return x;
 }
 
-// (blocks of eight wavefronts and more: registers for two of them on a compute unit)
+// (blocks of eight wavefronts and more: registers for sixteen on a compute unit, two blocks of eight or one of sixteen)
 constexpr int rows_threads(int waves) { return waves < 4 ? 256 : waves * kWave; }
 
 // Rows of length one.  LANES (64 at least with more than one) of each of WAVES wavefronts hold a row, UNITS units of elements each,
 // in registers: every tensor is read and written once.  UNITS = 0: a row of any length is walked three times (the two products;
 // the length of the moved row; the step), nothing stored before the last walk.  Bound by memory with states in 32 bits (65536 x 2304
-// bf16 with masters: 749 us, 5.64 TB/s), by arithmetic in 8 (24571 x 1538 fp32: 128 us, 4.7 TB/s: 114 vector instructions an element,
+// bf16 with masters: 749 us, 5.64 TB/s), by arithmetic in 8 (24571 x 1538 fp32: 118 us, 5.1 TB/s: 109 vector instructions an element,
 // among them the seventh stretch of a wavefront for the last two columns, and the block's maxima and inverses of every four elements).
 template <typename T, bool MASTER, bool EIGHT, int WAVES, int LANES, int UNITS>
 __global__ __launch_bounds__(rows_threads(WAVES), WAVES < 8 ? 1 : 4) void adamw_rows_kernel(const AdamwTable a) {
@@ -835,7 +835,9 @@ struct MomentsTable {
 };
 static_assert(sizeof(MomentsTable) <= 4096, "kernel arguments");
 
-// A tile is 2048 elements of the flattened tensor, wherever rows end.  Bound by memory: 302M elements to bf16 in 280 us, 6.5 TB/s.
+// A tile is 2048 elements of the flattened tensor, wherever rows end.  Bound by memory: 302M elements to bf16 in 280 us, 6.5 TB/s;
+// rows that are no multiple of 256 by their places: 41 vector instructions an element instead of 17, and maxima fetched by the lane
+// (24571 x 1538: 49 us, 4.7 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kAdamwThreads) void adamw8_moments_kernel(const MomentsTable a) {
   constexpr int N = 16 / static_cast<int>(sizeof(typename Traits<T>::store_t));

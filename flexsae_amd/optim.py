@@ -1,6 +1,6 @@
-"""The optimiser that dictionaries are trained with: AdamW steps over any number of tensors in one launch, with states in 32 bits
-or in 8, the global norm of the gradients, and rows held at length one; as functions over tensors and as ``AdamW``, an optimizer
-of torch's kind.
+"""The optimiser that dictionaries are trained with: AdamW steps over many tensors in one launch, with states in 32 bits or in 8,
+the global norm of the gradients, and rows held at length one; as functions over tensors and as ``AdamW``, an optimizer of
+torch's kind.
 
 Nothing here synchronises: the number of steps taken, the gradients' norm and whether a step is left out because the norm is not
 finite all stay on the device, so a captured graph replays them too.  The reference has no counterpart (its training loop takes
@@ -71,7 +71,8 @@ def _(grads):
 
 def grad_norm(grads: Sequence[Tensor]) -> Tensor:
     """The 2-norm of all elements of all tensors together: 0-dim fp32, on their device.  Squares are summed in 64 bits in a fixed
-    order (the same bits on every run); infinities and NaN reach the result."""
+    order (the same bits on every run); infinities and NaN reach the result.  It takes no part in autograd: a penalty on it has no
+    gradient."""
     if isinstance(grads, Tensor) or len(grads) == 0:
         raise ValueError("grad_norm: expected a list of at least one tensor")
     native = _native(grads[0])
@@ -267,7 +268,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                counter: Tensor, *, lr: Union[_Reals, Tensor] = 1e-3, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
                weight_decay: _Reals = 0.0, masters: Optional[Sequence[Tensor]] = None, unit_rows: bool = False,
                grad_norm: Optional[Tensor] = None, max_norm: Optional[float] = None, grad_scale: float = 1.0) -> None:
-    """One AdamW step of all ``params``, in place, in one launch for up to 66 of them; ``t = counter[0] + 1``::
+    """One AdamW step of all ``params``, in place; ``t = counter[0] + 1``::
 
         g = c * grad              c = min(1, max_norm / (grad_norm / grad_scale + 1e-6)) / grad_scale
         m = beta1 * m + (1 - beta1) * g
@@ -279,11 +280,14 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     lr, weight_decay: a number, or one for each parameter; lr also a 0-dim fp32 tensor, read when the kernel runs.
     masters: fp32 weights that 16-bit params are the rounded copies of (an fp32 parameter's entry is ignored).
     unit_rows: matrices whose rows (along the last dimension) are held at length one: the part of g along the row is left out
-    before, and the row divided by its length after.  A row of zeros stays one.
+    before, and the row divided by its length after.  A row of zeros stays one.  (Lengths between 1e-16 and 1e18: their squares are
+    summed in fp32.)
     grad_norm: ``grad_norm(grads)``; one that is not finite makes the call change nothing, ``counter`` neither.  max_norm: clips
-    by it.  grad_scale: the loss scale that the gradients carry.
-    Arithmetic is in fp32; a weight without a master is rounded once.  The gradients are left as they are.  With ``eps=0`` an
-    element without any gradient so far stays where it is.  No two of the tensors that a call changes may share memory."""
+    by it (None or 0: does not).  grad_scale: the loss scale that the gradients carry.
+    Arithmetic is in fp32; a weight without a master is rounded once.  The gradients are left as they are.  sqrt(v) is taken as
+    2^-63 where it is less, which shows where eps is as small: with ``eps=0`` an element without any gradient so far stays where it
+    is.  A launch takes up to 66 tensors; with unit_rows, of those that follow each other and go through the same kernel (by type,
+    master and number of columns).  No two of the tensors that a call changes may share memory."""
     _call(32, params, grads, exp_avgs, exp_avg_sqs, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm,
           max_norm, unit_rows)
 
@@ -296,7 +300,8 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], codes: Sequen
     fp32 maxima of every block of 256 elements (of a row with unit_rows, else of the flattened parameter) in ``absmax``.  With
     ``a`` the block's maxima of \\|m\\| and of v, the bytes c stand for ``sign(c - 128) ((c - 128) / 127)^2 a`` and
     ``(c / 255)^4 a``, rounded to the nearest on the root's scale; a v above zero never becomes zero.  The step itself uses m and v
-    before they are rounded.  A block with an infinity or NaN in m or v has NaN there from then on."""
+    before they are rounded.  A block with an infinity or NaN in m, or in v (the square of a gradient above 1.8e19 is
+    one), has NaN there from then on, and in its weights from the next step on."""
     _call(8, params, grads, codes, absmax, masters, counter, lr, weight_decay, beta1, beta2, eps, grad_scale, grad_norm, max_norm,
           unit_rows)
 

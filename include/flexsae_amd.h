@@ -530,7 +530,8 @@ typedef struct {
  *   m = b1 m + (1-b1) g, v = b2 v + (1-b2) g^2, w = (1 - lr wd) w - lr (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
  * 8-bit states, blocks of 256: codes[0] = c stands for sign(c-128) ((c-128)/127)^2 max|m|, codes[1] = c for (c/255)^4 max v
  * (at least 1 for a v above zero); the update uses m and v before they are rounded to their codes.  A maximum below the
- * smallest normal number is kept as zero; infinities and NaN make their block NaN.
+ * smallest normal number is kept as zero; one that is infinite or NaN is kept as NaN, of m and of v each for itself.
+ * sqrt(v) is taken as 2^-63 where it is less.
  * Calls that share a counter have to be ordered (one stream).  After a call that returns FLEXSAE_ERR_LAUNCH some of the
  * tensors may have been stepped.
  */

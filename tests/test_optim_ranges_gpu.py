@@ -108,3 +108,15 @@ def test_codes_of_values_below_the_normal_numbers(dtype, master, cols):
         codes.view(-1)[::3] = 1 if top > 1e-34 else codes.min()
         p.checked_step()
         assert bool((p.s0[0][..., 1] >= 1).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,cols", [(F32, 300), (BF16, 40), (F32, 20001)])
+def test_rows_of_very_small_and_very_large_lengths(bits, dtype, cols):
+    p = Problem([(4, cols)], dtype, bits, unit=True, seed=5)
+    w = p.params[0]
+    w[1] = (w[1].float() * 1e-16).to(dtype)
+    w[2] = (w[2].float() * 1e18).to(dtype)
+    p.checked_step(wd=0.0)
+    # (rounding a row of length one to 16 bits moves its length by less than the rounding of a number)
+    assert float((p.params[0].double().norm(dim=1) - 1).abs().max()) < (1e-5 if dtype == F32 else 2.0 ** -8)
