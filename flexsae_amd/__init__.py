@@ -8,6 +8,7 @@ as hand-written HIP kernels for AMD MI355X (gfx950), behind the reference packag
 Public names mirror reference torch-ext/flex_sae/__init__.py:5-18.  The ``triton_*`` names are
 kept so that existing callers need no edit; nothing here uses Triton.
 """
+from .lm import distillation_loss, embedding_lookup, layer_norm, layer_norm_stats
 from .ops import (check_index_flag, hier_stage_bytes, hierarchical_sae_sgd_step, set_dense_latents,
                   set_fused_training,
                   set_hier_min_slice_cols, set_hier_scratch_bytes, set_hier_stage_bytes, set_hot_latents,
@@ -53,4 +54,8 @@ __all__ = [
     "adamw8_state",
     "adamw_counter",
     "AdamW",
+    "layer_norm",
+    "layer_norm_stats",
+    "embedding_lookup",
+    "distillation_loss",
 ]

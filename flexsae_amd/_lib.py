@@ -26,6 +26,7 @@ ERR_SCRATCH_LIMIT = -6
 F32, BF16, F16 = 0, 1, 2
 
 FLAG_INDEX_RANGE = 1
+FLAG_TOKEN_RANGE = 2
 BWD_OUTPUTS_PREZEROED = 1
 BWD_REUSE_PAIR_LIST = 2
 BWD_SWEEP_ONLY = 4
@@ -43,6 +44,7 @@ BWD_RAGGED_ROWS = 16384
 TOPK_BWD_FP32_RESIDUAL = 256
 TOPK_BWD_AS_LARGE = 32768
 ADAMW_UNIT_ROWS = 1
+DISTILL_BY_ROW = 1
 
 
 class Shape(ctypes.Structure):
@@ -83,6 +85,28 @@ class Adamw8State(ctypes.Structure):
 
     _fields_ = [("codes", ctypes.c_void_p), ("absmax", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
                 ("exp_avg_sq", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
+
+
+class Norm(ctypes.Structure):
+    """Mirror of ``flexsae_norm``."""
+
+    _fields_ = [("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("dy_stride", ctypes.c_int64),
+                ("eps", ctypes.c_float), ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32)]
+
+
+class Lookup(ctypes.Structure):
+    """Mirror of ``flexsae_lookup``."""
+
+    _fields_ = [("n", ctypes.c_int64), ("vocab", ctypes.c_int64), ("cols", ctypes.c_int64), ("weight_stride", ctypes.c_int64),
+                ("dout_stride", ctypes.c_int64), ("factor", ctypes.c_float), ("dtype", ctypes.c_int32),
+                ("scale_dtype", ctypes.c_int32)]
+
+
+class Distill(ctypes.Structure):
+    """Mirror of ``flexsae_distill``."""
+
+    _fields_ = [("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("k", ctypes.c_int64), ("logits_stride", ctypes.c_int64),
+                ("temperature", ctypes.c_float), ("dtype", ctypes.c_int32), ("top_dtype", ctypes.c_int32), ("flags", ctypes.c_int32)]
 
 
 class FlexSAELibraryError(RuntimeError):
@@ -136,6 +160,15 @@ SIGNATURES = {
     "flexsae_grad_norm": (_int, [ctypes.POINTER(Grad), _i64, _p, _p, _sz, _p]),
     "flexsae_adamw_step": (_int, [ctypes.POINTER(AdamwTensor), _i64, ctypes.POINTER(AdamwConfig), _p]),
     "flexsae_adamw_check": (_int, [ctypes.POINTER(AdamwTensor), _i64, ctypes.POINTER(AdamwConfig)]),
+    "flexsae_layer_norm_fwd": (_int, [ctypes.POINTER(Norm), _p, _p, _p, _p, _p, _p, _p]),
+    "flexsae_layer_norm_bwd_workspace_bytes": (_sz, [ctypes.POINTER(Norm)]),
+    "flexsae_layer_norm_bwd": (_int, [ctypes.POINTER(Norm), _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "flexsae_lookup_fwd": (_int, [ctypes.POINTER(Lookup), _p, _p, _p, _p, _p, _p]),
+    "flexsae_lookup_bwd_workspace_bytes": (_sz, [ctypes.POINTER(Lookup)]),
+    "flexsae_lookup_bwd": (_int, [ctypes.POINTER(Lookup), _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "flexsae_distill_workspace_bytes": (_sz, [ctypes.POINTER(Distill)]),
+    "flexsae_distill_fwd": (_int, [ctypes.POINTER(Distill), _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _p]),
+    "flexsae_distill_bwd": (_int, [ctypes.POINTER(Distill), _p, _p, _p, _p, _p, _p, _int, _p, _p]),
     "flexsae_adamw8_moments": (_int, [ctypes.POINTER(Adamw8State), _i64, _int, _p]),
 }
 

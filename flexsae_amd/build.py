@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libflexsae_amd.so")
 EAGER_PATH = os.path.join(HERE, "_eager.so")
-HIP_SOURCES = ["flexsae_amd.hip", "optimizer.hip"]  # the losses; the optimiser
+HIP_SOURCES = ["flexsae_amd.hip", "optimizer.hip", "lm.hip"]  # the losses; the optimiser; around a dictionary in a model
 
 # gfx950 only: some kernels use more LDS per workgroup than the 64 KiB of earlier gfx9 parts
 # (csr_sort_long_kernel 65 600 bytes, the hot-latent variant of the training-step kernel more), the

@@ -11,10 +11,13 @@
 #include <dlfcn.h>
 
 #include <atomic>
+#include <cmath>
+#include <optional>
 #include <vector>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -39,7 +42,9 @@ using torch::autograd::variable_list;
   X(abi_version) X(fwd_workspace_bytes) X(topk_fwd_best_workspace_bytes) X(topk_fwd) X(hier_fwd)                        \
   X(topk_bwd_from_indices_workspace_bytes) X(topk_bwd_from_indices) X(hier_bwd_workspace_bytes) X(hier_bwd)             \
   X(hier_fwd_bwd_workspace_bytes_flags) X(hier_step) X(finish_grads)                                                    \
-  X(grad_norm_workspace_bytes) X(grad_norm) X(adamw_step) X(adamw_check) X(adamw8_moments)
+  X(grad_norm_workspace_bytes) X(grad_norm) X(adamw_step) X(adamw_check) X(adamw8_moments)                              \
+  X(layer_norm_fwd) X(layer_norm_bwd_workspace_bytes) X(layer_norm_bwd) X(lookup_fwd) X(lookup_bwd_workspace_bytes)     \
+  X(lookup_bwd) X(distill_workspace_bytes) X(distill_fwd) X(distill_bwd)
 struct Library {
 #define X(name) decltype(&flexsae_##name) name = nullptr;
   FLEXSAE_ENTRIES(X)
@@ -846,6 +851,9 @@ PyObject *py_adamw8_moments(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- around a dictionary in a model ----------------------------------------------------------
+#include "eager_lm.hpp"
+
 // set_flag(device, flag)
 PyObject *py_set_flag(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -893,6 +901,7 @@ PyMethodDef methods[] = {FLEXSAE_METHOD(init),       FLEXSAE_METHOD(set_flag),  
                          FLEXSAE_METHOD(topk_loss),  FLEXSAE_METHOD(hier_loss),   FLEXSAE_METHOD(hier_sliced),
                          FLEXSAE_METHOD(hier_late),  FLEXSAE_METHOD(hier_sgd),    FLEXSAE_METHOD(grad_norm),
                          FLEXSAE_METHOD(adamw),      FLEXSAE_METHOD(adamw_all),   FLEXSAE_METHOD(adamw8_moments),
+                         FLEXSAE_METHOD(layer_norm), FLEXSAE_METHOD(embedding_lookup), FLEXSAE_METHOD(distillation_loss),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_eager", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -69,7 +69,7 @@ def _flag_for(device: torch.device) -> Tensor:
 
 def check_index_flag(device=None) -> None:
     """Synchronise and raise IndexError if any fused call since the last check saw an index
-    outside ``[0, F)``; clears the flag."""
+    outside ``[0, F)``, or a token outside ``[0, V)`` that is not -1; clears the flag."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     flag = _flag_for(dev)
     bits = int(flag.item())
@@ -77,6 +77,8 @@ def check_index_flag(device=None) -> None:
         flag.zero_()
         if bits & _lib.FLAG_INDEX_RANGE:
             raise IndexError("flexsae_amd: an entry of `indices` was outside [0, F)")
+        if bits & _lib.FLAG_TOKEN_RANGE:
+            raise IndexError("flexsae_amd: a token or an entry of `top_indices` was outside [0, V) and not -1")
         raise RuntimeError(f"flexsae_amd: device status flag {bits:#x}")
 
 

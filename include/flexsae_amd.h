@@ -51,7 +51,11 @@ typedef enum {
 
 typedef enum { FLEXSAE_F32 = 0, FLEXSAE_BF16 = 1, FLEXSAE_F16 = 2 } flexsae_dtype;
 
-enum { FLEXSAE_FLAG_INDEX_RANGE = 1 };
+enum {
+  FLEXSAE_FLAG_INDEX_RANGE = 1,
+  FLEXSAE_FLAG_TOKEN_RANGE = 2 /* flexsae_lookup_fwd, flexsae_distill_fwd: a token or vocabulary index below -1 or at or */
+                               /* beyond the vocabulary; it counts as none, as -1 does                                    */
+};
 
 /* flags for the backward entry points */
 enum {
@@ -551,6 +555,97 @@ typedef struct {
 
 /* The values that 8-bit states stand for, in `dtype`. */
 int flexsae_adamw8_moments(const flexsae_adamw8_state *states, int64_t count, int dtype, void *stream);
+
+/*
+ * Around a dictionary that is trained inside a language model: layer norm, rows of a table by token, distillation from a
+ * teacher's top logits.  Rows may lie at any stride (in elements; 0: the same row again) and begin at any element; what these
+ * entry points write is contiguous, and nothing that they write may overlap what they read.  (No reference counterpart.)
+ */
+typedef struct {
+  int64_t rows, cols;          /* cols >= 1 */
+  int64_t x_stride, dy_stride; /* between rows of x and of dy */
+  float eps;                   /* not negative */
+  int32_t dtype;               /* flexsae_dtype of x, y, dy, dx */
+  int32_t weight_dtype, bias_dtype;
+} flexsae_norm;
+
+/*
+ * y = (x - mean) * rstd * weight + bias by rows, rstd = 1 / sqrt(mean((x - mean)^2) + eps), in fp32, rounded once.
+ * weight[cols], bias[cols]: NULL for none.  mean[rows], rstd[rows]: fp32, NULL where not wanted.
+ */
+int flexsae_layer_norm_fwd(const flexsae_norm *norm, const void *x, const void *weight, const void *bias, void *y, float *mean,
+                           float *rstd, void *stream);
+
+size_t flexsae_layer_norm_bwd_workspace_bytes(const flexsae_norm *norm);
+
+/*
+ * Gradients from dy and the forward's mean and rstd: dx, dweight (weight_dtype), dbias (bias_dtype), each NULL where not wanted;
+ * column sums in fp32 in an order that the sizes fix.  The workspace may be NULL without dweight and dbias.
+ */
+int flexsae_layer_norm_bwd(const flexsae_norm *norm, const void *x, const void *dy, const void *weight, const float *mean,
+                           const float *rstd, void *dx, void *dweight, void *dbias, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
+typedef struct {
+  int64_t n, vocab, cols;             /* tokens, rows of the table, columns; vocab < 2^31 */
+  int64_t weight_stride, dout_stride; /* between rows of weight and of dout */
+  float factor;                       /* finite */
+  int32_t dtype;                      /* flexsae_dtype of weight, out, dout, dweight */
+  int32_t scale_dtype;                /* of scale and dscale */
+} flexsae_lookup;
+
+/*
+ * out[i] = factor * scale[i] * weight[tokens[i]], in fp32, rounded once; scale[n]: NULL for ones.  A token of -1 gives a row of
+ * zeros; so does any other outside [0, vocab), and sets FLEXSAE_FLAG_TOKEN_RANGE.
+ */
+int flexsae_lookup_fwd(const flexsae_lookup *lookup, const int64_t *tokens, const void *weight, const void *scale, void *out,
+                       int *status_flag, void *stream);
+
+size_t flexsae_lookup_bwd_workspace_bytes(const flexsae_lookup *lookup);
+
+/*
+ * dweight[vocab][cols] (every row is written, zeros for tokens that do not occur) by sorted tokens, summed in fp32 in an order
+ * that the sizes and tokens fix; dscale[n].  Either is NULL where not wanted (weight is read for dscale only).  Rows of dout whose
+ * token is none are not read.
+ */
+int flexsae_lookup_bwd(const flexsae_lookup *lookup, const int64_t *tokens, const void *weight, const void *scale,
+                       const void *dout, void *dweight, void *dscale, void *workspace, size_t workspace_bytes, void *stream);
+
+enum {
+  FLEXSAE_DISTILL_BY_ROW = 1 /* the losses of the rows, not their mean: loss[rows], and grad[rows] in the backward */
+};
+
+typedef struct {
+  int64_t rows, vocab, k; /* each >= 1 and < 2^31 */
+  int64_t logits_stride;  /* between rows of logits */
+  float temperature;      /* T > 0 */
+  int32_t dtype;          /* flexsae_dtype of logits and dlogits */
+  int32_t top_dtype;      /* of top */
+  int32_t flags;
+} flexsae_distill;
+
+size_t flexsae_distill_workspace_bytes(const flexsae_distill *distill);
+
+/* fp32 numbers of `stats`, which a forward fills for the backward (aligned to 16 bytes): 4 (rows + 1). */
+/*
+ * loss = T^2 sum over rows of a sum over j of p[j] (log p[j] - log q[index[j]]), p = softmax(top / T) over a row's stored places,
+ * q = softmax(logits / T), a the row's weight divided by the sum of all (BY_ROW: the weight); row_weights[rows] (fp32): NULL for ones.
+ * top[rows][k], index[rows][k]: a place with an index of -1 holds no logit (any other outside [0, vocab) neither, and sets
+ * FLEXSAE_FLAG_TOKEN_RANGE); an entry may be stored more than once.  A row of weight zero, or without a stored logit above minus
+ * infinity, counts as zero; its logits do not matter.  Where all weights are zero the mean is zero.
+ * dlogits[rows][vocab] (contiguous), or NULL: the gradient for an upstream gradient of one.
+ */
+int flexsae_distill_fwd(const flexsae_distill *distill, const void *logits, const void *top, const int64_t *index,
+                        const float *row_weights, float *loss, float *stats, void *dlogits, void *workspace,
+                        size_t workspace_bytes, int *status_flag, void *stream);
+
+/*
+ * dlogits for the upstream gradient grad[0] (BY_ROW: grad[rows]), from what the forward left in `stats`.  skip_if_one: dlogits holds
+ * the gradient for an upstream gradient of one, and is left as it is where grad[0] is one (not with BY_ROW).
+ */
+int flexsae_distill_bwd(const flexsae_distill *distill, const void *logits, const void *top, const int64_t *index,
+                        const float *row_weights, const float *stats, const float *grad, int skip_if_one, void *dlogits,
+                        void *stream);
 
 #ifdef __cplusplus
 }
