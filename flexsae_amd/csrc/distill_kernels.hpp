@@ -27,7 +27,7 @@ struct DistillArgs {
   const int64_t *index;
   const float *row_weights;  // or NULL
   float2 *parts;             // [rows][splits]: maximum and sum of a part of a row
-  float4 *stats;             // [rows]: m, ln s, the teacher's maximum, 1 / sum of its exponentials (0: the row is not used);
+  float4 *stats;             // [rows]: m, s, the teacher's maximum, 1 / sum of its exponentials (0: the row is not used);
                              // [rows].x: one over the sum of the weights
   float *row_loss;           // [rows]
   float *loss;
@@ -45,10 +45,42 @@ struct DistillArgs {
 // exp(x / T) by the base-2 exponential; c = log2(e) / T.
 __device__ __forceinline__ float exp_of(float x, float c) { return __builtin_amdgcn_exp2f(x * c); }
 
+// exp((x - m) / T) of a row.  (Of the difference, which is exact where it matters: one operation less, 2^(c x - c m), would have
+// the rounding of c m in every exponent.)
+struct RowExp {
+  float m, c;
+  __device__ __forceinline__ RowExp(float m, float inv_t) : m(m), c(kLog2e * inv_t) {}
+  __device__ __forceinline__ float of(float x) const { return exp_of(x - m, c); }
+};
+
 // The maximum and sum of two parts.  (A maximum is never minus infinity: it begins as the least finite number.)
 __device__ __forceinline__ float2 join(float2 a, float2 b, float c) {
   const float m = fmaxf(a.x, b.x);
   return make_float2(m, a.y * exp_of(a.x - m, c) + b.y * exp_of(b.x - m, c));
+}
+
+// Takes the elements [from, end) of a row, THREADS units at a time, to `with` (first column, elements, how many of them are in the
+// row), with kAhead units of a thread on their way at once.
+template <typename T, int THREADS, typename F>
+__device__ __forceinline__ void walk(const elem_t<T> *in, int64_t from, int64_t end, F with) {
+  constexpr int N = kUnitOf<T>, kAhead = 4;
+  constexpr int64_t kStep = THREADS * N;
+  int64_t at = from + static_cast<int64_t>(threadIdx.x) * N;
+  float x[N];
+  for (; at + (kAhead - 1) * kStep + N <= end; at += kAhead * kStep) {
+    words_t v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = load_words<T>(in + at + u * kStep);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      unpack<T>(v[u], x);
+      with(at + u * kStep, x, int64_t{N});
+    }
+  }
+  for (; at < end; at += kStep) {
+    unpack<T>(load_upto<T>(in + at, end - at), x);
+    with(at, x, end - at);
+  }
 }
 
 template <int N>
@@ -92,7 +124,7 @@ __device__ __forceinline__ float mean_factor(const DistillArgs &a) {
 // Statistics of a part of a row: block = row * splits + part.
 template <typename T>
 __global__ __launch_bounds__(kDistillThreads) void distill_parts_kernel(const DistillArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   __shared__ float2 sh[kDistillThreads / kWave];
   const int64_t block = block_index(), row = block / a.splits, split = block - row * a.splits;
@@ -101,17 +133,12 @@ __global__ __launch_bounds__(kDistillThreads) void distill_parts_kernel(const Di
   const int64_t end = (split + 1) * a.part < a.vocab ? (split + 1) * a.part : a.vocab;
   const float c = kLog2e * a.inv_t;
   float2 ms = make_float2(-FLT_MAX, 0.f);
-  for (int64_t at = split * a.part + static_cast<int64_t>(threadIdx.x) * N; at < end; at += kDistillThreads * N) {
-    float x[N];
-    const int64_t left = end - at;
-    unpack_raw<T, N>(load_upto<T, N>(in + at, left), x);
-    if (left < N) {
+  walk<T, kDistillThreads>(in, split * a.part, end, [&](int64_t, float (&x)[N], int64_t left) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i >= left) x[i] = -INFINITY;
-    }
+    for (int i = 0; i < N; ++i)
+      if (i >= left) x[i] = -INFINITY;
     take<N>(ms, x, c);
-  }
+  });
   ms = wave_join(ms, c);
   if (lane_id() == 0) sh[wave_index()] = ms;
   __syncthreads();
@@ -124,7 +151,7 @@ __global__ __launch_bounds__(kDistillThreads) void distill_parts_kernel(const Di
 // The teacher's side of a row and its loss, by one wavefront that has the row's statistics; fills stats[row] and the row's loss.
 template <typename T>
 __device__ __forceinline__ void finish_row(const DistillArgs &a, int64_t row, float2 ms) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   const S *const in = static_cast<const S *>(a.logits) + row * a.stride;
   const int lane = lane_id();
   const float weight = row_weight(a, row);
@@ -163,7 +190,7 @@ __device__ __forceinline__ void finish_row(const DistillArgs &a, int64_t row, fl
     loss = group_sum<kWave>(loss);
   }
   if (lane != 0) return;
-  a.stats[row] = make_float4(ms.x, log_s, t.x, used ? 1.f / t.y : 0.f);
+  a.stats[row] = make_float4(ms.x, ms.y, t.x, used ? 1.f / t.y : 0.f);
   a.row_loss[row] = used ? a.t * a.t * weight * loss : 0.f;
 }
 
@@ -195,8 +222,8 @@ __global__ __launch_bounds__(1024) void distill_mean_kernel(const DistillArgs a)
 // The entries of a part of a row that the teacher has stored: gradients in the place of those that `dlogits` holds without the
 // teacher.  Run by the whole block, behind a barrier.  An entry that is stored twice is written by the first of its places.
 template <typename T, int THREADS>
-__device__ __forceinline__ void stored_entries(const DistillArgs &a, int64_t row, int64_t from, int64_t end, float4 st, float coef) {
-  using S = typename Traits<T>::store_t;
+__device__ __forceinline__ void stored_entries(const DistillArgs &a, int64_t row, int64_t from, int64_t end, float4 st, const RowExp &e, float coef) {
+  using S = elem_t<T>;
   const S *const in = static_cast<const S *>(a.logits) + row * a.stride;
   S *const out = static_cast<S *>(a.dlogits) + row * a.vocab;
   const int64_t *const index = a.index + row * a.k;
@@ -209,18 +236,16 @@ __device__ __forceinline__ void stored_entries(const DistillArgs &a, int64_t row
     for (int64_t j = 0; j < a.k && first; ++j) {
       if (index[j] != i) continue;
       first = j >= k;
-      p += exp_of(load_scalar(a.top, a.top_dtype, row * a.k + j) - st.z, c) * st.w;
+      p += exp_of(load_scalar(a.top, a.top_dtype, row * a.k + j) - st.z, c);
     }
-    if (!first) continue;
-    const float q = __builtin_amdgcn_exp2f((Traits<T>::up(in[i]) - st.x) * c - st.y * kLog2e);
-    out[i] = Traits<T>::down(coef * (q - p));
+    if (first) out[i] = Traits<T>::down(coef / st.y * e.of(Traits<T>::up(in[i])) - coef * (p * st.w));
   }
 }
 
 // Gradient of a part of a row: block = row * splits + part.
 template <typename T>
 __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const DistillArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   if (a.skip_if_one && a.grad[0] == 1.f) return;
   const int64_t block = block_index(), row = block / a.splits, split = block - row * a.splits;
@@ -232,23 +257,214 @@ __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const Dis
   const float upstream = a.grad == nullptr ? 1.f : a.grad[a.by_row ? row : 0];
   const float coef = a.t * row_weight(a, row) * mean_factor(a) * upstream;
   const bool used = st.w != 0.f;
-  const float c = kLog2e * a.inv_t, shift = st.y * kLog2e;
-  for (int64_t at = from + static_cast<int64_t>(threadIdx.x) * N; at < end; at += kDistillThreads * N) {
-    float x[N];
-    const int64_t left = end - at;
-    if (used) {
-      unpack_raw<T, N>(load_upto<T, N>(in + at, left), x);
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = coef * __builtin_amdgcn_exp2f((x[i] - st.x) * c - shift);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = 0.f;
-    }
-    store_upto<T, N>(out + at, pack<T, N>(x), left);
+  if (!used) {
+    for (int64_t at = from + static_cast<int64_t>(threadIdx.x) * N; at < end; at += kDistillThreads * N)
+      store_upto<T>(out + at, words_t(0u), end - at);
+    return;
   }
-  if (!used) return;
+  const RowExp e(st.x, a.inv_t);
+  const float each = coef / st.y;
+  walk<T, kDistillThreads>(in, from, end, [&](int64_t at, float (&x)[N], int64_t left) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = each * e.of(x[i]);
+    store_upto<T>(out + at, pack<T>(x), left);
+  });
   __syncthreads();
-  stored_entries<T, kDistillThreads>(a, row, from, end, st, coef);
+  stored_entries<T, kDistillThreads>(a, row, from, end, st, e, coef);
+}
+
+// ---- a row in the registers of one block ------------------------------------------------------
+
+// Words of minus infinities.
+template <typename T>
+constexpr uint32_t kMinusInfinities = Traits<T>::dtype == FLEXSAE_F32 ? 0xff800000u : Traits<T>::dtype == FLEXSAE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+
+// The largest of what a lane has seen, without converting it: 16-bit floats that are not negative are ordered as their bits, and
+// negative ones the other way round.  (A NaN that is passed over shows in the sum.)
+template <typename T>
+struct LargestBits {
+  typedef int16_t pair_t __attribute__((ext_vector_type(2)));
+  pair_t most = -32768, least = 32767;
+  __device__ __forceinline__ void take(words_t v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pair_t p;
+      const uint32_t w = v[i];
+      __builtin_memcpy(&p, &w, 4);
+      most = __builtin_elementwise_max(most, p);
+      least = __builtin_elementwise_min(least, p);
+    }
+  }
+  __device__ __forceinline__ float value() const {
+    const int16_t hi = most.x > most.y ? most.x : most.y, lo = least.x < least.y ? least.x : least.y;
+    return Traits<T>::up(static_cast<uint16_t>(hi >= 0 ? hi : lo));
+  }
+};
+template <>
+struct LargestBits<float> {
+  float most = -INFINITY;
+  __device__ __forceinline__ void take(words_t v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = fmaxf(most, __uint_as_float(v[i]));
+  }
+  __device__ __forceinline__ float value() const { return most; }
+};
+
+// A block's threads share out the places of the teacher, one a thread.
+struct Stored {
+  int index;  // -1: none
+  float top;
+};
+__device__ __forceinline__ Stored load_stored(const DistillArgs &a, int64_t row) {
+  Stored t = {-1, 0.f};
+  const int k = static_cast<int>(threadIdx.x);
+  if (row >= a.rows || k >= a.k) return t;
+  const int64_t i = a.index[row * a.k + k];
+  t.top = load_scalar(a.top, a.top_dtype, row * a.k + k);
+  if (i >= 0 && i < a.vocab) t.index = static_cast<int>(i);
+  else if (a.flag && i != -1) atomicOr(a.flag, FLEXSAE_FLAG_TOKEN_RANGE);
+  return t;
+}
+
+// A row that is not used: a gradient of zeros, and no loss.
+template <typename T, int THREADS, bool GRAD>
+__device__ __forceinline__ void unused_row(const DistillArgs &a, int64_t row) {
+  constexpr int N = kUnitOf<T>;
+  if (threadIdx.x == 0) {
+    a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    a.row_loss[row] = 0.f;
+  }
+  if constexpr (!GRAD) return;
+  elem_t<T> *const out = static_cast<elem_t<T> *>(a.dlogits) + row * a.vocab;
+  for (int64_t at = static_cast<int64_t>(threadIdx.x) * N; at < a.vocab; at += THREADS * N) store_upto<T>(out + at, words_t(0u), a.vocab - at);
+}
+
+template <typename T, int THREADS, int UNITS>
+__global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs a) {
+  using S = elem_t<T>;
+  constexpr int N = kUnitOf<T>, kWaves = THREADS / kWave;
+  __shared__ float2 maxima[kWaves];  // of logits and teacher
+  __shared__ float2 sums[kWaves];    // of both exponentials
+  // the teacher's places: entry, exponential, the student's logit; the two logits
+  // apart; those of a thread's columns in a chain
+  __shared__ int stored[THREADS], chain[THREADS], head[THREADS];
+  __shared__ float stored_p[THREADS], stored_z[THREADS], apart[THREADS];
+  const int64_t row = block_index();
+  if (row >= a.rows) return;
+  const float weight = row_weight(a, row);
+  if (weight == 0.f) {
+    (void)load_stored(a, row);
+    return unused_row<T, THREADS, true>(a, row);
+  }
+  // whole units, and behind them up to N - 1 elements, one of a thread
+  const uint32_t cols = static_cast<uint32_t>(a.vocab), whole = cols - cols % N, first = threadIdx.x * N, last = whole + threadIdx.x;
+  const S *const in = static_cast<const S *>(a.logits) + row * a.stride;
+  S *const out = static_cast<S *>(a.dlogits) + row * a.vocab;
+  const int places = static_cast<int>(a.k), k = static_cast<int>(threadIdx.x);
+  words_t held[UNITS];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const uint32_t at = first + u * THREADS * N;
+    held[u] = load_words<T>(in + (at < whole ? at : 0u));
+  }
+  // (behind the row's loads: what waits for these does not hold those up)
+  const int64_t place = row * a.k + (k < places ? k : places - 1);
+  S last_one = in[last < cols ? last : 0u];
+  int64_t index = a.index[place];
+  const uint32_t t_bits = load_scalar_bits(a.top, a.top_dtype, place);
+  const float tail = last < cols ? Traits<T>::up(last_one) : -INFINITY, t = scalar_from_bits(t_bits, a.top_dtype);
+  if (k >= places) index = -1;
+  if (index < -1 || index >= a.vocab) {
+    if (a.flag) atomicOr(a.flag, FLEXSAE_FLAG_TOKEN_RANGE);
+    index = -1;
+  }
+  const S z_one = in[index < 0 ? 0 : index];
+  head[k] = -1;
+  stored[k] = static_cast<int>(index);
+  float top = wave_max(index < 0 ? -INFINITY : t == t ? t : INFINITY);  // (a NaN makes the row's loss one)
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u)
+    if ((u + 1) * THREADS * N > whole) held[u] = first + u * THREADS * N < whole ? held[u] : words_t(kMinusInfinities<T>);
+  LargestBits<T> largest;
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) largest.take(held[u]);
+  float m = wave_max(fmaxf(largest.value(), tail));
+  if (lane_id() == 0) maxima[wave_index()] = make_float2(m, top);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    m = fmaxf(m, maxima[w].x);
+    top = fmaxf(top, maxima[w].y);
+  }
+  if (top == -INFINITY) return unused_row<T, THREADS, true>(a, row);
+  const RowExp e(m, a.inv_t);
+  const float p = index < 0 ? 0.f : exp_of(t - top, kLog2e * a.inv_t);
+  stored_p[k] = p;
+  if (p != 0.f) {
+    chain[k] = atomicExch(&head[static_cast<uint32_t>(index) < whole ? static_cast<uint32_t>(index) / N % THREADS : static_cast<uint32_t>(index) - whole], k);
+  }
+  float sum = e.of(tail);
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    float x[N];
+    unpack<T>(held[u], x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += e.of(x[i]);
+  }
+  // (the compiler would keep the exponentials, which take twice the registers of the row, instead of taking them again)
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) asm volatile("" : "+v"(held[u]));
+  const float z = Traits<T>::up(z_one);
+  stored_z[k] = z;
+  apart[k] = ((t - top) - (z - m)) * a.inv_t;
+  sum = group_sum<kWave>(sum);
+  float sum_top = group_sum<kWave>(p);
+  if (lane_id() == 0) sums[wave_index()] = make_float2(sum, sum_top);
+  __syncthreads();
+  sum = sum_top = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    sum += sums[w].x;
+    sum_top += sums[w].y;
+  }
+  const float inv_top = 1.f / sum_top, log_s = logf(sum);
+  if (wave_index() == 0) {
+    const float logs = logf(sum_top) - log_s;
+    float loss = 0.f;
+    for (int j = k; j < places; j += kWave)
+      if (stored_p[j] != 0.f) loss = fmaf(stored_p[j] * inv_top, apart[j] - logs, loss);
+    loss = group_sum<kWave>(loss);
+    if (k == 0) {
+      a.stats[row] = make_float4(m, sum, top, inv_top);
+      a.row_loss[row] = a.t * a.t * weight * loss;
+    }
+  }
+  const float coef = a.t * weight * mean_factor(a), each = coef / sum;
+  auto gradient = [&](float x) { return each * e.of(x); };
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const uint32_t at = first + u * THREADS * N;
+    float x[N];
+    unpack<T>(held[u], x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = gradient(x[i]);
+    store_whole<T>(out + at, pack<T>(x), at < whole);
+  }
+  if (last < cols) out[last] = Traits<T>::down(gradient(tail));
+  // the stored entries among the thread's columns, in whose places the gradients above have been stored by this very thread
+  for (int j = head[k]; j >= 0; j = chain[j]) {
+    float all = 0.f;
+    int from = -1;
+    for (;;) {  // an entry that is stored more than once: its places in their order
+      int least = THREADS;
+      for (int i = head[k]; i >= 0; i = chain[i])
+        if (stored[i] == stored[j] && i > from && i < least) least = i;
+      if (least == THREADS) break;
+      all += stored_p[least];
+      from = least;
+    }
+    out[stored[j]] = Traits<T>::down(gradient(stored_z[j]) - coef * (all * inv_top));
+  }
 }
 
 }  // namespace flexsae

@@ -127,7 +127,7 @@ __device__ __forceinline__ float2 row_moments(const float (&x)[UNITS][N], int64_
 
 template <typename T, int LANES, int UNITS>
 __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_fwd_kernel(const NormArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   __shared__ float2 sh[2][kNormMostWaves];
   const NormShare<LANES> share;
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_f
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
-      unpack_raw<T, N>(load_upto<T, N>(in + c, a.cols - c), x[u]);
+      unpack<T>(load_upto<T>(in + c, a.cols - c), x[u]);
     }
     const float2 moments = row_moments<LANES, UNITS, N>(x, a.cols, share, sh, static_cast<int>(i & 1));
     const float mean = moments.x, rstd = 1.f / sqrtf(moments.y + a.eps);
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_f
         if (a.bias) v += b[u][k];
         x[u][k] = v;
       }
-      store_upto<T, N>(out + c, pack<T, N>(x[u]), a.cols - c);
+      store_upto<T>(out + c, pack<T>(x[u]), a.cols - c);
     }
     if (share.me == 0) {
       if (a.mean) a.mean[row] = mean;
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_f
 // Rows that no block holds: walked three times, a block a row.
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   __shared__ float2 sh[2][kNormMostWaves];
   const int64_t row = block_index();
@@ -183,13 +183,13 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArg
   float x[N], w[N], b[N];
   float sum = 0.f, squares = 0.f;
   for (int64_t c = static_cast<int64_t>(threadIdx.x) * N; c < a.cols; c += step) {
-    unpack_raw<T, N>(load_upto<T, N>(in + c, a.cols - c), x);
+    unpack<T>(load_upto<T>(in + c, a.cols - c), x);
 #pragma unroll
     for (int i = 0; i < N; ++i) sum += x[i];
   }
   const float mean = row_sums<0>(sum, 0.f, sh, 0).x / static_cast<float>(a.cols);
   for (int64_t c = static_cast<int64_t>(threadIdx.x) * N; c < a.cols; c += step) {
-    unpack_raw<T, N>(load_upto<T, N>(in + c, a.cols - c), x);
+    unpack<T>(load_upto<T>(in + c, a.cols - c), x);
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (c + i < a.cols) squares = fmaf(x[i] - mean, x[i] - mean, squares);
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArg
   const float rstd = 1.f / sqrtf(row_sums<0>(squares, 0.f, sh, 1).x / static_cast<float>(a.cols) + a.eps);
   S *const out = static_cast<S *>(a.y) + row * a.cols;
   for (int64_t c = static_cast<int64_t>(threadIdx.x) * N; c < a.cols; c += step) {
-    unpack_raw<T, N>(load_upto<T, N>(in + c, a.cols - c), x);
+    unpack<T>(load_upto<T>(in + c, a.cols - c), x);
     if (a.weight) load_typed<N>(a.weight, a.weight_dtype, c, a.cols - c, w);
     if (a.bias) load_typed<N>(a.bias, a.bias_dtype, c, a.cols - c, b);
 #pragma unroll
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArg
       if (a.bias) v += b[i];
       x[i] = v;
     }
-    store_upto<T, N>(out + c, pack<T, N>(x), a.cols - c);
+    store_upto<T>(out + c, pack<T>(x), a.cols - c);
   }
   if (threadIdx.x == 0) {
     if (a.mean) a.mean[row] = mean;
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArg
 // groups of lanes share a block.
 template <typename T, int LANES, int UNITS>
 __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_bwd_kernel(const NormArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   __shared__ float2 sh[2][kNormMostWaves];
   const NormShare<LANES> share;
@@ -242,19 +242,19 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_b
     const S *const in = static_cast<const S *>(a.x) + row * a.x_stride;
     const S *const grad = static_cast<const S *>(a.dy) + row * a.dy_stride;
     const float mean = a.mean[row], rstd = a.rstd[row];
-    raw_vec_t<T, N> xr[UNITS], gr[UNITS];
+    words_t xr[UNITS], gr[UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
-      xr[u] = load_upto<T, N>(in + c, a.cols - c);
-      gr[u] = load_upto<T, N>(grad + c, a.cols - c);
+      xr[u] = load_upto<T>(in + c, a.cols - c);
+      gr[u] = load_upto<T>(grad + c, a.cols - c);
     }
     float c1 = 0.f, c2 = 0.f;
     float x[UNITS][N], g[UNITS][N];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      unpack_raw<T, N>(xr[u], x[u]);
-      unpack_raw<T, N>(gr[u], g[u]);
+      unpack<T>(xr[u], x[u]);
+      unpack<T>(gr[u], g[u]);
 #pragma unroll
       for (int i = 0; i < N; ++i) {  // (behind the row's end all gradients are zeros)
         const float unit = (x[u][i] - mean) * rstd;
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_b
       const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
 #pragma unroll
       for (int i = 0; i < N; ++i) x[u][i] = rstd * (g[u][i] - c1 - x[u][i] * c2);
-      store_upto<T, N>(out + c, pack<T, N>(x[u]), a.cols - c);
+      store_upto<T>(out + c, pack<T>(x[u]), a.cols - c);
     }
   }
   if (a.partial == nullptr) return;
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_b
 // Rows that no block holds: dx by walking the row twice, and the column sums by a kernel of their own.
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(const NormArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   __shared__ float2 sh[2][kNormMostWaves];
   const int64_t row = block_index();
@@ -330,8 +330,8 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(const NormArg
 #pragma unroll
   for (int i = 0; i < N; ++i) w[i] = 1.f;
   auto load = [&](int64_t c) {
-    unpack_raw<T, N>(load_upto<T, N>(in + c, a.cols - c), x);
-    unpack_raw<T, N>(load_upto<T, N>(grad + c, a.cols - c), g);
+    unpack<T>(load_upto<T>(in + c, a.cols - c), x);
+    unpack<T>(load_upto<T>(grad + c, a.cols - c), g);
     if (a.weight) load_typed<N>(a.weight, a.weight_dtype, c, a.cols - c, w);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -356,14 +356,14 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(const NormArg
     load(c);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = rstd * (g[i] - c1 - x[i] * c2);
-    store_upto<T, N>(out + c, pack<T, N>(x), a.cols - c);
+    store_upto<T>(out + c, pack<T>(x), a.cols - c);
   }
 }
 
 // Column sums of the rows b, b + gridDim.y, ... of block (., b); a thread has N columns.
 template <typename T>
 __global__ __launch_bounds__(kNormThreads) void layer_norm_columns_kernel(const NormArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   const int64_t c = (static_cast<int64_t>(blockIdx.x) * kNormThreads + threadIdx.x) * N;
   if (c >= a.cols) return;
@@ -372,8 +372,8 @@ __global__ __launch_bounds__(kNormThreads) void layer_norm_columns_kernel(const 
   for (int i = 0; i < N; ++i) dw[i] = db[i] = 0.f;
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     float x[N], g[N];
-    unpack_raw<T, N>(load_upto<T, N>(static_cast<const S *>(a.x) + row * a.x_stride + c, a.cols - c), x);
-    unpack_raw<T, N>(load_upto<T, N>(static_cast<const S *>(a.dy) + row * a.dy_stride + c, a.cols - c), g);
+    unpack<T>(load_upto<T>(static_cast<const S *>(a.x) + row * a.x_stride + c, a.cols - c), x);
+    unpack<T>(load_upto<T>(static_cast<const S *>(a.dy) + row * a.dy_stride + c, a.cols - c), g);
     const float mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
     for (int i = 0; i < N; ++i) {

@@ -203,7 +203,7 @@ int check_lookup(const flexsae_lookup *l) {
 using LookupKernel = void (*)(const LookupArgs);
 struct LookupPlan {
   LookupKernel fwd, pieces, pieces_dots, bwd, bwd_dots, dots;
-  int64_t groups, tiles;  // of a block, of a row
+  int64_t groups, tiles, width;  // of a block, of a row, columns of whole tiles
 };
 
 template <typename T, int LANES, int UNITS>
@@ -211,7 +211,8 @@ LookupPlan lookup_shared(int64_t cols) {
   return {lookup_fwd_kernel<T, LANES, UNITS>,           lookup_pieces_kernel<T, LANES, UNITS, false>,
           lookup_pieces_kernel<T, LANES, UNITS, true>,  lookup_bwd_kernel<T, LANES, UNITS, false>,
           lookup_bwd_kernel<T, LANES, UNITS, true>,     lookup_dots_kernel<T, LANES, UNITS>,
-          kLookupThreads / LANES,                       ceil_div(cols, int64_t{LANES} * UNITS * kUnitOf<T>)};
+          kLookupThreads / LANES,                       ceil_div(cols, int64_t{LANES} * UNITS * kUnitOf<T>),
+          ceil_div(cols, int64_t{LANES} * UNITS * kUnitOf<T>) * LANES * UNITS * kUnitOf<T>};
 }
 
 template <typename T>
@@ -262,7 +263,7 @@ LookupSpace lookup_space(const flexsae_lookup &l, const LookupPlan &plan) {
   s.map = take(n * 4);
   s.csr_bytes = l.n > 0 ? flexsae_csr_workspace_bytes(l.n, 1, l.vocab) : 0;
   s.csr = take(s.csr_bytes);
-  s.pieces = take(l.n > kLookupChunk ? static_cast<size_t>(ceil_div(l.n, kLookupChunk)) * 2 * static_cast<size_t>(l.cols) * 4 : 0);
+  s.pieces = take(l.n > kLookupChunk ? static_cast<size_t>(ceil_div(l.n, kLookupChunk)) * 2 * static_cast<size_t>(plan.width) * 4 : 0);
   s.dots = take(n * static_cast<size_t>(plan.tiles) * 4);
   return s;
 }
@@ -410,15 +411,33 @@ DistillArgs distill_args(const flexsae_distill &d, const void *logits, const voi
 }
 
 using DistillKernel = void (*)(const DistillArgs);
+// A row in the registers of a block of so many threads: where it fits there, and each of the teacher's places has a thread.
+struct DistillHeld {
+  DistillKernel kernel = nullptr;
+  int threads = 0;
+};
 struct DistillKernels {
   DistillKernel parts, rows, grad;
+  DistillHeld held;
 };
 template <typename T>
-DistillKernels distill_kernels() {
-  return {distill_parts_kernel<T>, distill_rows_kernel<T>, distill_grad_kernel<T>};
+DistillHeld distill_held(int64_t vocab, int64_t k) {
+  const int64_t units = ceil_div(vocab, kUnitOf<T>);
+  if (vocab < kUnitOf<T>) return {};
+  if (units <= 256 * 4 && k <= 256) return {distill_held_kernel<T, 256, 4>, 256};
+  if (units <= 256 * 16 && k <= 256) return {distill_held_kernel<T, 256, 16>, 256};
+  if (units <= 512 * 16 && k <= 512) return {distill_held_kernel<T, 512, 16>, 512};
+  if (units <= 1024 * 16 && k <= 1024) return {distill_held_kernel<T, 1024, 16>, 1024};
+  return {};
 }
-DistillKernels distill_kernels(int dtype) {
-  return dtype == FLEXSAE_F32 ? distill_kernels<float>() : dtype == FLEXSAE_BF16 ? distill_kernels<bf16_t>() : distill_kernels<f16_t>();
+template <typename T>
+DistillKernels distill_kernels(int64_t vocab, int64_t k) {
+  return {distill_parts_kernel<T>, distill_rows_kernel<T>, distill_grad_kernel<T>, distill_held<T>(vocab, k)};
+}
+DistillKernels distill_kernels(const flexsae_distill &d) {
+  return d.dtype == FLEXSAE_F32    ? distill_kernels<float>(d.vocab, d.k)
+         : d.dtype == FLEXSAE_BF16 ? distill_kernels<bf16_t>(d.vocab, d.k)
+                                   : distill_kernels<f16_t>(d.vocab, d.k);
 }
 
 }  // namespace
@@ -445,10 +464,20 @@ int flexsae_distill_fwd(const flexsae_distill *d, const void *logits, const void
   a.dlogits = dlogits;
   a.flag = status_flag;
   const hipStream_t s = as_stream(stream);
-  const DistillKernels k = distill_kernels(d->dtype);
+  const DistillKernels k = distill_kernels(*d);
+  const auto finish = [&]() {
+    if (a.by_row) return static_cast<int>(FLEXSAE_OK);
+    distill_mean_kernel<<<1, 1024, 0, s>>>(a);
+    return launch_status();
+  };
   if (!a.by_row && row_weights) {
     distill_weights_kernel<<<1, 1024, 0, s>>>(a);
     if (const int rc = launch_status()) return rc;
+  }
+  if (dlogits && k.held.kernel && (a.rows >= kComputeUnits || k.held.threads == 256)) {
+    k.held.kernel<<<grid_of(a.rows), k.held.threads, 0, s>>>(a);
+    if (const int rc = launch_status()) return rc;
+    return finish();
   }
   k.parts<<<grid_of(a.rows * a.splits), kDistillThreads, 0, s>>>(a);
   if (const int rc = launch_status()) return rc;
@@ -458,9 +487,7 @@ int flexsae_distill_fwd(const flexsae_distill *d, const void *logits, const void
     k.grad<<<grid_of(a.rows * a.splits), kDistillThreads, 0, s>>>(a);
     if (const int rc = launch_status()) return rc;
   }
-  if (a.by_row) return FLEXSAE_OK;
-  distill_mean_kernel<<<1, 1024, 0, s>>>(a);
-  return launch_status();
+  return finish();
 }
 
 int flexsae_distill_bwd(const flexsae_distill *d, const void *logits, const void *top, const int64_t *index, const float *row_weights,
@@ -474,7 +501,7 @@ int flexsae_distill_bwd(const flexsae_distill *d, const void *logits, const void
   a.grad = grad;
   a.dlogits = dlogits;
   a.skip_if_one = skip_if_one != 0;
-  distill_kernels(d->dtype).grad<<<grid_of(a.rows * a.splits), kDistillThreads, 0, as_stream(stream)>>>(a);
+  distill_kernels(*d).grad<<<grid_of(a.rows * a.splits), kDistillThreads, 0, as_stream(stream)>>>(a);
   return launch_status();
 }
 

@@ -24,7 +24,7 @@ struct LookupArgs {
   const void *dout;
   void *out;  // backward: dW
   const uint32_t *begin, *map;  // of the sorted places
-  float *pieces;      // [chunks][2][cols]: the end of a token that began before the stretch, and the beginning of one that ends behind it
+  float *pieces;      // [chunks][2][columns of whole tiles]: the end of a token that began before the stretch, and the beginning of one that ends behind it
   float *dots;        // [n][tiles] shares of ds, or NULL
   void *dscale;
   int *flag;
@@ -49,41 +49,43 @@ struct LookupPlace {
     tile = task - item * tiles;
     first = tile * (LANES * UNITS * N) + (static_cast<int>(threadIdx.x) % LANES) * N;
   }
+  // columns of whole tiles, which rows of fp32 sums have
+  __device__ __forceinline__ int64_t width(int64_t tiles) const { return tiles * (LANES * UNITS * N); }
   __device__ __forceinline__ int64_t column(int u) const { return first + static_cast<int64_t>(u) * LANES * N; }
 };
 
 template <typename T, int LANES, int UNITS>
 __global__ __launch_bounds__(kLookupThreads) void lookup_fwd_kernel(const LookupArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   const LookupPlace<T, LANES, UNITS> at(a.tiles);
   if (at.item >= a.n) return;
   const int64_t token = a.tokens[at.item], row = row_of(token, a.vocab);
   if (a.flag && at.first == 0 && (token < -1 || token >= a.vocab)) atomicOr(a.flag, FLEXSAE_FLAG_TOKEN_RANGE);
   S *const out = static_cast<S *>(a.out) + at.item * a.cols;
-  raw_vec_t<T, N> v[UNITS];
+  words_t v[UNITS];
   if (row < 0) {
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       v[u] = 0;
-      store_upto<T, N>(out + at.column(u), v[u], a.cols - at.column(u));
+      store_upto<T>(out + at.column(u), v[u], a.cols - at.column(u));
     }
     return;
   }
   const S *const in = static_cast<const S *>(a.weight) + row * a.weight_stride;
   const float scale = a.scale ? a.factor * load_scalar(a.scale, a.scale_dtype, at.item) : a.factor;
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) v[u] = load_upto<T, N>(in + at.column(u), a.cols - at.column(u));
+  for (int u = 0; u < UNITS; ++u) v[u] = load_upto<T>(in + at.column(u), a.cols - at.column(u));
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
     if (scale != 1.f) {
       float x[N];
-      unpack_raw<T, N>(v[u], x);
+      unpack<T>(v[u], x);
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] *= scale;
-      v[u] = pack<T, N>(x);
+      v[u] = pack<T>(x);
     }
-    store_upto<T, N>(out + at.column(u), v[u], a.cols - at.column(u));
+    store_upto<T>(out + at.column(u), v[u], a.cols - at.column(u));
   }
 }
 
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_fwd_kernel(const Lookup
 template <typename T, int LANES, int UNITS, bool DOTS>
 __device__ __forceinline__ void add_places(const LookupArgs &a, const LookupPlace<T, LANES, UNITS> &at, uint32_t from, uint32_t to,
                                            bool check, const float (&w)[UNITS][kUnitOf<T>], float (&sum)[UNITS][kUnitOf<T>]) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   for (uint32_t p = from; p < to; ++p) {
     const int64_t n = a.map[p];
@@ -103,7 +105,7 @@ __device__ __forceinline__ void add_places(const LookupArgs &a, const LookupPlac
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       float x[N];
-      unpack_raw<T, N>(load_upto<T, N>(in + at.column(u), a.cols - at.column(u)), x);
+      unpack<T>(load_upto<T>(in + at.column(u), a.cols - at.column(u)), x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         sum[u][i] = fmaf(scale, x[i], sum[u][i]);
@@ -123,7 +125,7 @@ __device__ __forceinline__ void load_row(const LookupArgs &a, const LookupPlace<
   constexpr int N = kUnitOf<T>;
   const auto *const in = static_cast<const typename Traits<T>::store_t *>(a.weight) + row * a.weight_stride;
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) unpack_raw<T, N>(load_upto<T, N>(in + at.column(u), a.cols - at.column(u)), w[u]);
+  for (int u = 0; u < UNITS; ++u) unpack<T>(load_upto<T>(in + at.column(u), a.cols - at.column(u)), w[u]);
 }
 
 template <int UNITS, int N>
@@ -152,9 +154,11 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_pieces_kernel(const Loo
     clear(sum);
     if constexpr (DOTS) load_row(a, at, token, w);
     add_places<T, LANES, UNITS, DOTS>(a, at, b > lo ? b : lo, e < hi ? e : hi, token == 0, w, sum);
-    float *const out = a.pieces + (at.item * 2 + which) * a.cols;
+    float *const out = a.pieces + (at.item * 2 + which) * at.width(a.tiles);
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) store_upto<float, N>(out + at.column(u), pack<float, N>(sum[u]), a.cols - at.column(u));
+    for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+      for (int h = 0; h < N; h += 4) *reinterpret_cast<float4 *>(out + at.column(u) + h) = make_float4(sum[u][h], sum[u][h + 1], sum[u][h + 2], sum[u][h + 3]);
   };
   const int64_t first = token_at(lo), last = token_at(hi - 1);
   const uint32_t first_begin = a.begin[first], first_end = a.begin[first + 1];
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_pieces_kernel(const Loo
 
 template <typename T, int LANES, int UNITS, bool DOTS>
 __global__ __launch_bounds__(kLookupThreads) void lookup_bwd_kernel(const LookupArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   const LookupPlace<T, LANES, UNITS> at(a.tiles);
   if (at.item >= a.vocab) return;
@@ -176,14 +180,17 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_bwd_kernel(const Lookup
   if (to - from > kLookupChunk) {
     for (uint32_t chunk = from / kLookupChunk; chunk <= (to - 1) / kLookupChunk; ++chunk) {
       const int which = from > chunk * kLookupChunk;
-      const float *const piece = a.pieces + (static_cast<int64_t>(chunk) * 2 + which) * a.cols;
+      const float *const piece = a.pieces + (static_cast<int64_t>(chunk) * 2 + which) * at.width(a.tiles);
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        float x[N];
-        unpack_raw<float, N>(load_upto<float, N>(piece + at.column(u), a.cols - at.column(u)), x);
+      for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[u][i] += x[i];
-      }
+        for (int h = 0; h < N; h += 4) {
+          const float4 x = *reinterpret_cast<const float4 *>(piece + at.column(u) + h);
+          sum[u][h] += x.x;
+          sum[u][h + 1] += x.y;
+          sum[u][h + 2] += x.z;
+          sum[u][h + 3] += x.w;
+        }
     }
   } else if (to > from) {
     float w[UNITS][N];
@@ -192,13 +199,13 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_bwd_kernel(const Lookup
   }
   S *const out = static_cast<S *>(a.out) + at.item * a.cols;
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) store_upto<T, N>(out + at.column(u), pack<T, N>(sum[u]), a.cols - at.column(u));
+  for (int u = 0; u < UNITS; ++u) store_upto<T>(out + at.column(u), pack<T>(sum[u]), a.cols - at.column(u));
 }
 
 // Shares of ds by rows of dout, where no gradient of the table is wanted.
 template <typename T, int LANES, int UNITS>
 __global__ __launch_bounds__(kLookupThreads) void lookup_dots_kernel(const LookupArgs a) {
-  using S = typename Traits<T>::store_t;
+  using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   const LookupPlace<T, LANES, UNITS> at(a.tiles);
   if (at.item >= a.n) return;
@@ -210,8 +217,8 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_dots_kernel(const Looku
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
     float x[N], g[N];
-    unpack_raw<T, N>(load_upto<T, N>(in + at.column(u), a.cols - at.column(u)), x);
-    unpack_raw<T, N>(load_upto<T, N>(grad + at.column(u), a.cols - at.column(u)), g);
+    unpack<T>(load_upto<T>(in + at.column(u), a.cols - at.column(u)), x);
+    unpack<T>(load_upto<T>(grad + at.column(u), a.cols - at.column(u)), g);
 #pragma unroll
     for (int i = 0; i < N; ++i) dot = fmaf(x[i], g[i], dot);
   }

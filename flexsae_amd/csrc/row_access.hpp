@@ -9,67 +9,123 @@ namespace flexsae {
 template <typename T>
 constexpr int kUnitOf = 16 / static_cast<int>(sizeof(typename Traits<T>::store_t));  // elements of 16 bytes, one access of a lane
 
-// Vectors that are aligned to their elements only: rows of an odd number of 16-bit elements begin at odd addresses.  (The HSA ABI
-// runs kernels with unaligned access on, and the compiler forms the same 16-byte accesses.)
-template <typename S, int N>
-using loose_vec_t = S __attribute__((ext_vector_type(N), aligned(sizeof(S))));
+// What a lane reads or writes at once, as four words.
+typedef uint32_t words_t __attribute__((ext_vector_type(4)));
 
-// The N elements at p of which the first `left` are there; zeros (or `fill`'s bits) for the rest.
-template <typename T, int N, bool NT = false>
-__device__ __forceinline__ raw_vec_t<T, N> load_upto(const typename Traits<T>::store_t *p, int64_t left,
-                                                     typename Traits<T>::store_t fill = 0) {
-  using S = typename Traits<T>::store_t;
-  raw_vec_t<T, N> v;
-  if (left >= N) {
-    const auto *q = reinterpret_cast<const loose_vec_t<S, N> *>(p);
-    if constexpr (NT) v = __builtin_nontemporal_load(q);
-    else v = *q;
-    return v;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = i < left ? p[i] : fill;
-  return v;
+// The same in memory, aligned to its elements only: rows of an odd number of 16-bit elements begin at odd addresses.  (The HSA ABI
+// runs kernels with unaligned access on, and the compiler forms the same 16-byte accesses.)
+template <typename T>
+struct LooseWords;
+template <>
+struct LooseWords<float> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <>
+struct LooseWords<bf16_t> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <>
+struct LooseWords<f16_t> : LooseWords<bf16_t> {};
+
+template <typename T>
+using elem_t = typename Traits<T>::store_t;
+
+template <typename T>
+__device__ __forceinline__ uint32_t bits_of(elem_t<T> v) {
+  if constexpr (sizeof(v) == 4) return __float_as_uint(v);
+  else return v;
+}
+template <typename T>
+__device__ __forceinline__ elem_t<T> from_bits(uint32_t v) {
+  if constexpr (sizeof(elem_t<T>) == 4) return __uint_as_float(v);
+  else return static_cast<uint16_t>(v);
 }
 
-template <typename T, int N>
-__device__ __forceinline__ raw_vec_t<T, N> pack(const float (&x)[N]) {
-  raw_vec_t<T, N> v;
-  if constexpr (Traits<T>::dtype == FLEXSAE_BF16) {
-    vec_t<uint32_t, N / 2> w;
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) w[i] = f32x2_to_bf16x2_bits(x[2 * i], x[2 * i + 1]);
-    __builtin_memcpy(&v, &w, sizeof v);
+template <typename T>
+__device__ __forceinline__ words_t load_words(const elem_t<T> *p) {
+  return *reinterpret_cast<const typename LooseWords<T>::type *>(p);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_whole(elem_t<T> *p, words_t v, bool there) {
+  if (there) *reinterpret_cast<typename LooseWords<T>::type *>(p) = v;
+}
+
+// The first `left` of the elements at p, zeros for the rest.
+template <typename T>
+__device__ __forceinline__ words_t load_upto(const elem_t<T> *p, int64_t left) {
+  constexpr int N = kUnitOf<T>, kPer = N / 4;
+  words_t v = 0u;
+  if (left >= N) {
+    v = *reinterpret_cast<const typename LooseWords<T>::type *>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = Traits<T>::down(x[i]);
+    for (int i = 0; i < N - 1; ++i)
+      if (i < left) v[i / kPer] |= bits_of<T>(p[i]) << (i % kPer * 16);
   }
   return v;
 }
 
-template <typename T, int N, bool NT = false>
-__device__ __forceinline__ void store_upto(typename Traits<T>::store_t *p, const raw_vec_t<T, N> &v, int64_t left) {
-  using S = typename Traits<T>::store_t;
+template <typename T>
+__device__ __forceinline__ void store_upto(elem_t<T> *p, words_t v, int64_t left) {
+  constexpr int N = kUnitOf<T>, kPer = N / 4;
   if (left >= N) {
-    auto *q = reinterpret_cast<loose_vec_t<S, N> *>(p);
-    const loose_vec_t<S, N> w = v;
-    if constexpr (NT) __builtin_nontemporal_store(w, q);
-    else *q = w;
-    return;
-  }
+    *reinterpret_cast<typename LooseWords<T>::type *>(p) = v;
+  } else {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < left) p[i] = v[i];
+    for (int i = 0; i < N - 1; ++i)
+      if (i < left) p[i] = from_bits<T>(v[i / kPer] >> (i % kPer * 16));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(words_t v, float (&x)[kUnitOf<T>]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Traits<T>::dtype == FLEXSAE_F32) {
+      x[i] = __uint_as_float(v[i]);
+    } else if constexpr (Traits<T>::dtype == FLEXSAE_BF16) {
+      x[2 * i] = __uint_as_float(v[i] << 16);
+      x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    } else {
+      x[2 * i] = f16_bits_to_f32(static_cast<uint16_t>(v[i]));
+      x[2 * i + 1] = f16_bits_to_f32(static_cast<uint16_t>(v[i] >> 16));
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ words_t pack(const float (&x)[kUnitOf<T>]) {
+  words_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Traits<T>::dtype == FLEXSAE_F32) v[i] = __float_as_uint(x[i]);
+    else if constexpr (Traits<T>::dtype == FLEXSAE_BF16) v[i] = f32x2_to_bf16x2_bits(x[2 * i], x[2 * i + 1]);
+    else v[i] = static_cast<uint32_t>(f32_to_f16_bits(x[2 * i])) | static_cast<uint32_t>(f32_to_f16_bits(x[2 * i + 1])) << 16;
+  }
+  return v;
 }
 
 // N elements of a type that is known at run time, as fp32; zeros behind `left`.
 template <int N>
 __device__ __forceinline__ void load_typed(const void *base, int dtype, int64_t off, int64_t left, float (&o)[N]) {
+  static_assert(N == 4 || N == 8, "units of 16 bytes");
   if (dtype == FLEXSAE_F32) {
-    unpack_raw<float, N>(load_upto<float, N>(static_cast<const float *>(base) + off, left), o);
+#pragma unroll
+    for (int h = 0; h < N; h += 4) {
+      float x[4];
+      unpack<float>(load_upto<float>(static_cast<const float *>(base) + off + h, left - h), x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[h + i] = x[i];
+    }
   } else {
-    const auto v = load_upto<bf16_t, N>(static_cast<const uint16_t *>(base) + off, left);
-    if (dtype == FLEXSAE_BF16) unpack_raw<bf16_t, N>(v, o);
-    else unpack_raw<f16_t, N>(v, o);
+    // (of a unit of four elements the second half is not there)
+    const words_t v = load_upto<bf16_t>(static_cast<const uint16_t *>(base) + off, N == 8 ? left : left < 4 ? left : 4);
+    float x[8];
+    if (dtype == FLEXSAE_BF16) unpack<bf16_t>(v, x);
+    else unpack<f16_t>(v, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = x[i];
   }
 }
 
@@ -93,6 +149,19 @@ __device__ __forceinline__ float group_sum(float v) {
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
   }
   return v;
+}
+
+// The largest over a wavefront, in all lanes.
+__device__ __forceinline__ float wave_max(float v) {
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  v = fmaxf(v, dpp_move<0x140>(v));
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // Blocks beyond the first kGridRow go into further rows of the grid (threads of a grid are counted in 32 bits along an axis).

@@ -351,7 +351,7 @@ def _check_distill(z, top, index, weights=None, T=1.0, by_row=False, grad=1.0):
     ref.within(loss, want["loss"], tol["loss"] + ref.U * want["loss"].abs() + 1e-38, "loss")
     ref.within(dz, want["dz"], ref.rounded(want["dz"], z.dtype, tol["dz"]), "dz")
     alone = flex.distillation_loss(z, top, index, temperature=T, row_weights=weights, reduction="none" if by_row else "mean")
-    assert torch.equal(alone, loss.detach()) or (alone.isnan() & loss.isnan()).any()
+    ref.within(alone, want["loss"], tol["loss"] + ref.U * want["loss"].abs() + 1e-38, "loss alone")
     return loss.detach(), dz
 
 
@@ -362,6 +362,18 @@ def test_distill(n, v, k, dtype):
     z, top, index = _distill_inputs(n, v, k, dtype, seed=n + v + k)
     scale = 1024.0 if dtype == torch.float16 else 1.0
     _check_distill(z, top, index, grad=scale)
+
+
+@pytest.mark.parametrize("n,v,k", [(3, 4, 1), (3, 8, 2), (300, 4097, 256), (5, 8193, 257), (260, 16385, 300), (258, 32771, 9),
+                                   (256, 65535, 512), (300, 65536, 40), (257, 131071, 700), (260, 131080, 20), (260, 3000, 1500)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+def test_distill_of_rows_in_registers_and_beyond(n, v, k, dtype):
+    z, top, index = _distill_inputs(n, v, k, dtype, seed=n + v)
+    index[:, k // 2:] = torch.where(torch.rand(n, k - k // 2, generator=_gen(1)).to(DEV) < 0.1, index[:, :1], index[:, k // 2:])
+    weights = torch.rand(n, generator=_gen(2)).to(DEV)
+    weights[1] = 0.0
+    index[2] = -1
+    _check_distill(z, top, index, weights, T=0.8, grad=1.0 if dtype != torch.float16 else 4096.0)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
@@ -410,7 +422,11 @@ def test_distill_masked_logits():
         away = torch.rand(8, 900, generator=_gen(2)).to(DEV) < 0.5
         away.scatter_(1, index, False)
         _check_distill(z.masked_fill(away, -math.inf), top, index, grad=64.0)
-        _check_distill(z.masked_fill(away, torch.finfo(dtype).min), top, index, grad=64.0)
+        for low in (torch.finfo(dtype).min, torch.finfo(dtype).min / 2, -1000.0):
+            _check_distill(z.masked_fill(away, low), top, index, grad=64.0)
+            every = z.clone()
+            every[3] = low  # nothing else: even
+            _check_distill(every, top, index, T=0.25, grad=64.0)
     z, top, index = _distill_inputs(4, 300, 5, torch.float32, seed=7)
     lost = z.clone()
     lost[1, index[1, 0]] = -math.inf
@@ -568,6 +584,14 @@ def _pass(fn, tensors, grad):
     return [out.detach(), *torch.autograd.grad(out, leaves, grad)]
 
 
+def _same(name, a, b):
+    """The ops take the gradient of a mean from other partial sums than the one that is made along with the loss: both within the
+    bounds of the formula, so within twice the rounding of each other (and 1e-5 for the sums, of 1e3 terms in a lane at most)."""
+    if name not in ("mean", "scaled"):
+        return all(torch.equal(p, q) for p, q in zip(a, b))
+    return all(bool(((p.double() - q.double()).abs() <= (2 * ref.half(p.dtype) + 1e-5) * q.double().abs()).all()) for p, q in zip(a, b))
+
+
 def test_the_same_bits_on_every_run_and_through_the_ops():
     for name, fn, tensors, grad in _calls():
         first = _pass(fn, tensors, grad)
@@ -575,7 +599,7 @@ def test_the_same_bits_on_every_run_and_through_the_ops():
             assert all(torch.equal(a, b) for a, b in zip(first, _pass(fn, tensors, grad))), name
         flex.set_index_checking(True)  # (calls then go through the ops)
         try:
-            assert all(torch.equal(a, b) for a, b in zip(first, _pass(fn, tensors, grad))), name
+            assert _same(name, first, _pass(fn, tensors, grad)), name
         finally:
             flex.set_index_checking(False)
 
@@ -657,7 +681,7 @@ def test_compiled_calls():
         want = _pass(fn, tensors, grad)
         compiled = torch.compile(fn, backend="aot_eager", fullgraph=True)
         got = _pass(compiled, tensors, grad)
-        assert all(torch.equal(a, b) for a, b in zip(want, got)), name
+        assert _same(name, want, got), name
 
 
 def test_large_offsets():
