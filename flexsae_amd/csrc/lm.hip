@@ -200,24 +200,36 @@ int check_lookup(const flexsae_lookup *l) {
   return FLEXSAE_OK;
 }
 
+constexpr int kLookupRows = 4;          // rows of a group of lanes ...
+constexpr int64_t kLookupMany = 8192;  // ... where there are this many blocks without
 using LookupKernel = void (*)(const LookupArgs);
 struct LookupPlan {
-  LookupKernel fwd, pieces, pieces_dots, bwd, bwd_dots, dots;
+  LookupKernel fwd, fwd_rows, pieces, pieces_dots, bwd, bwd_dots, bwd_rows, bwd_rows_dots, dots;
   int64_t groups, tiles, width;  // of a block, of a row, columns of whole tiles
 };
 
-template <typename T, int LANES, int UNITS>
+template <typename T, int LANES, int UNITS, bool WHOLE = true>
 LookupPlan lookup_shared(int64_t cols) {
-  return {lookup_fwd_kernel<T, LANES, UNITS>,           lookup_pieces_kernel<T, LANES, UNITS, false>,
-          lookup_pieces_kernel<T, LANES, UNITS, true>,  lookup_bwd_kernel<T, LANES, UNITS, false>,
-          lookup_bwd_kernel<T, LANES, UNITS, true>,     lookup_dots_kernel<T, LANES, UNITS>,
-          kLookupThreads / LANES,                       ceil_div(cols, int64_t{LANES} * UNITS * kUnitOf<T>),
-          ceil_div(cols, int64_t{LANES} * UNITS * kUnitOf<T>) * LANES * UNITS * kUnitOf<T>};
+  constexpr int64_t kTile = int64_t{LANES} * UNITS * kUnitOf<T>;
+  const int64_t tiles = ceil_div(cols, kTile);
+  return {lookup_fwd_kernel<T, LANES, UNITS, WHOLE, 1>,
+          lookup_fwd_kernel<T, LANES, UNITS, WHOLE, kLookupRows>,
+          lookup_pieces_kernel<T, LANES, UNITS, WHOLE, false>,
+          lookup_pieces_kernel<T, LANES, UNITS, WHOLE, true>,
+          lookup_bwd_kernel<T, LANES, UNITS, WHOLE, false, 1>,
+          lookup_bwd_kernel<T, LANES, UNITS, WHOLE, true, 1>,
+          lookup_bwd_kernel<T, LANES, UNITS, WHOLE, false, kLookupRows>,
+          lookup_bwd_kernel<T, LANES, UNITS, WHOLE, true, kLookupRows>,
+          lookup_dots_kernel<T, LANES, UNITS, WHOLE>,
+          kLookupThreads / LANES,
+          tiles,
+          tiles * kTile};
 }
 
 template <typename T>
 LookupPlan lookup_plan(int64_t cols) {
   const int64_t units = ceil_div(cols, kUnitOf<T>);
+  if (cols < kUnitOf<T>) return lookup_shared<T, 16, 1, false>(cols);
   if (units <= 16) return lookup_shared<T, 16, 1>(cols);
   if (units <= 32) return lookup_shared<T, 32, 1>(cols);
   return lookup_shared<T, 64, 1>(cols);
@@ -245,7 +257,12 @@ LookupArgs lookup_args(const flexsae_lookup &l, const LookupPlan &plan, const in
   return a;
 }
 
-bool too_many(int64_t items, const LookupPlan &plan) { return items > kMostBlocks / plan.tiles; }
+// (tasks of groups of lanes are counted in 32 bits)
+bool too_many(int64_t items, const LookupPlan &plan) { return items >= ((int64_t{1} << 32) - kLookupThreads) / plan.tiles; }
+bool many(int64_t items, const LookupPlan &plan) { return items * plan.tiles >= kLookupMany * plan.groups; }
+int64_t lookup_blocks(int64_t items, bool rows, const LookupPlan &plan) {
+  return ceil_div(ceil_div(items, rows ? kLookupRows : 1) * plan.tiles, plan.groups);
+}
 
 // Where the parts of a backward's workspace lie.
 struct LookupSpace {
@@ -284,7 +301,8 @@ int flexsae_lookup_fwd(const flexsae_lookup *l, const int64_t *tokens, const voi
   LookupArgs a = lookup_args(*l, plan, tokens, weight, scale);
   a.out = out;
   a.flag = status_flag;
-  plan.fwd<<<grid_of(ceil_div(l->n * plan.tiles, plan.groups)), kLookupThreads, 0, as_stream(stream)>>>(a);
+  const bool rows = many(l->n, plan);
+  (rows ? plan.fwd_rows : plan.fwd)<<<grid_of(lookup_blocks(l->n, rows, plan)), kLookupThreads, 0, as_stream(stream)>>>(a);
   return launch_status();
 }
 
@@ -326,7 +344,9 @@ int flexsae_lookup_bwd(const flexsae_lookup *l, const int64_t *tokens, const voi
         if (const int rc = launch_status()) return rc;
       }
     }
-    (dscale ? plan.bwd_dots : plan.bwd)<<<grid_of(ceil_div(l->vocab * plan.tiles, plan.groups)), kLookupThreads, 0, s>>>(a);
+    const bool rows = many(l->vocab, plan);
+    (rows ? dscale ? plan.bwd_rows_dots : plan.bwd_rows : dscale ? plan.bwd_dots : plan.bwd)<<<
+        grid_of(lookup_blocks(l->vocab, rows, plan)), kLookupThreads, 0, s>>>(a);
     if (const int rc = launch_status()) return rc;
   } else if (l->n > 0) {
     plan.dots<<<grid_of(ceil_div(l->n * plan.tiles, plan.groups)), kLookupThreads, 0, s>>>(a);
