@@ -41,6 +41,53 @@ struct NormShare {
   }
 };
 
+// A lane's units of a row.  WHOLE: rows have N elements and more; where one ends inside a unit, the lane has its last N elements
+// instead, the first `again` of which the lane before has too: both compute and store the same, and sums leave them out.  Else a row
+// is a part of one unit.
+template <typename T, int UNITS, bool WHOLE>
+struct RowUnits {
+  static constexpr int N = kUnitOf<T>;
+  int cols, column[UNITS], again[UNITS];
+  __device__ __forceinline__ RowUnits(int me, int lanes, int64_t row_cols) : cols(static_cast<int>(row_cols)) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int at = (u * lanes + me) * N;
+      column[u] = !WHOLE ? at : at >= cols ? 0 : at + N > cols ? cols - N : at;
+      again[u] = at >= cols ? N : at - column[u];
+    }
+  }
+  __device__ __forceinline__ words_t load(const elem_t<T> *row, int u) const {
+    if constexpr (WHOLE) return load_words<T>(row + column[u]);
+    else return load_upto<T>(row + column[u], cols - column[u]);
+  }
+  __device__ __forceinline__ void store(elem_t<T> *row, int u, words_t v) const {
+    if constexpr (WHOLE) store_whole<T>(row + column[u], v, again[u] < N);
+    else store_upto<T>(row + column[u], v, cols - column[u]);
+  }
+  // f(i) for each element of unit u that is in the row and that no other lane has
+  template <typename F>
+  __device__ __forceinline__ void once(int u, F f) const {
+    if (WHOLE && again[u] == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (WHOLE ? i >= again[u] : column[u] + i < cols) f(i);
+    }
+  }
+  // the same of all elements that are in the row
+  template <typename F>
+  __device__ __forceinline__ void each(int u, F f) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (WHOLE ? again[u] < N : column[u] + i < cols) f(i);
+  }
+  __device__ __forceinline__ void typed(const void *base, int dtype, int u, float (&o)[N]) const {
+    load_typed<N>(base, dtype, column[u], WHOLE ? N : cols - column[u], o);
+  }
+};
+
 // Sum over the lanes of a row of two numbers at once; `turn` alternates between calls of a block (its part of `sh` is read until
 // the next barrier).
 template <int LANES>
@@ -53,107 +100,86 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2 (*sh)[kNormM
     if (waves == 1) return mine;
     if (lane_id() == 0) sh[turn][wave_index()] = mine;
     __syncthreads();
-    float2 all = make_float2(0.f, 0.f);
-    for (int w = 0; w < waves; ++w) {
-      all.x += sh[turn][w].x;
-      all.y += sh[turn][w].y;
-    }
-    return all;
+    // (a wavefront's sums in a lane of each 16, and one read of the LDS instead of one after another)
+    const int w = lane_id() % kNormMostWaves;
+    const float2 theirs = w < waves ? sh[turn][w] : make_float2(0.f, 0.f);
+    return make_float2(group_sum<kNormMostWaves>(theirs.x), group_sum<kNormMostWaves>(theirs.y));
   }
 }
 
-// Mean of a row and its mean square about it, from what the wavefronts hold: UNITS units of N elements a lane, of which the first
-// `left[u]` are in the row.
-template <int LANES, int UNITS, int N>
-__device__ __forceinline__ float2 row_moments(const float (&x)[UNITS][N], int64_t cols, const NormShare<LANES> &sh_of,
-                                              float2 (*sh)[kNormMostWaves], int turn) {
-  float sum = 0.f;
+// Mean of a row and its mean square about it, from what the wavefronts hold.
+template <typename T, int LANES, int UNITS, bool WHOLE>
+__device__ __forceinline__ float2 row_moments(const float (&x)[UNITS][kUnitOf<T>], const RowUnits<T, UNITS, WHOLE> &units,
+                                              const NormShare<LANES> &share, float2 (*sh)[kNormMostWaves], int turn) {
+  constexpr int kGroup = LANES == 0 ? kWave : LANES, kSpan = kWave * kUnitOf<T>;
+  const int cols = units.cols;
+  float sum = 0.f, squares = 0.f;
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-    for (int i = 0; i < N; ++i) sum += x[u][i];  // (zeros behind the row's end)
-  constexpr int kGroup = LANES == 0 ? kWave : LANES;
+  for (int u = 0; u < UNITS; ++u) units.once(u, [&](int i) { sum += x[u][i]; });
   sum = group_sum<kGroup>(sum);
-  int64_t held = cols;
-  if constexpr (LANES == 0) {
-    held = 0;
+  auto held_by = [&](int wave) {  // elements
+    int n = 0;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int64_t rest = cols - (static_cast<int64_t>(u) * sh_of.lanes + wave_index() * kWave) * N;
-      held += rest < 0 ? 0 : rest > kWave * N ? kWave * N : rest;
+      const int rest = cols - (u * share.lanes + wave * kWave) * kUnitOf<T>;
+      n += rest < 0 ? 0 : rest > kSpan ? kSpan : rest;
     }
-  }
-  const float mean = held > 0 ? sum / static_cast<float>(held) : 0.f;
-  float squares = 0.f;
+    return static_cast<float>(n);
+  };
+  const float held = LANES == 0 ? held_by(wave_index()) : static_cast<float>(cols);
+  const float mean = held > 0.f ? sum / held : 0.f;
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    const int64_t left = cols - (static_cast<int64_t>(u) * sh_of.lanes + sh_of.me) * N;
-    if (left >= N) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) squares = fmaf(x[u][i] - mean, x[u][i] - mean, squares);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < left) squares = fmaf(x[u][i] - mean, x[u][i] - mean, squares);
-    }
-  }
+  for (int u = 0; u < UNITS; ++u) units.once(u, [&](int i) { squares = fmaf(x[u][i] - mean, x[u][i] - mean, squares); });
   squares = group_sum<kGroup>(squares);
-  if constexpr (LANES != 0) {
-    return make_float2(mean, squares / static_cast<float>(cols));
-  } else {
-    const int waves = sh_of.lanes / kWave;
-    if (waves == 1) return make_float2(mean, squares / static_cast<float>(cols));
-    if (lane_id() == 0) sh[turn][wave_index()] = make_float2(mean, squares);
-    __syncthreads();
-    auto held_by = [&](int w) {
-      int64_t n = 0;
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int64_t rest = cols - (static_cast<int64_t>(u) * sh_of.lanes + w * kWave) * N;
-        n += rest < 0 ? 0 : rest > kWave * N ? kWave * N : rest;
-      }
-      return static_cast<float>(n);
-    };
-    float all = 0.f, m2 = 0.f;
-    for (int w = 0; w < waves; ++w) all += held_by(w) * sh[turn][w].x;
-    all /= static_cast<float>(cols);
-    for (int w = 0; w < waves; ++w) {
-      const float d = sh[turn][w].x - all;
-      m2 += sh[turn][w].y + held_by(w) * d * d;
-    }
-    return make_float2(all, m2 / static_cast<float>(cols));
-  }
+  const int waves = LANES == 0 ? share.lanes / kWave : 1;
+  if (waves == 1) return make_float2(mean, squares / static_cast<float>(cols));
+  if (lane_id() == 0) sh[turn][wave_index()] = make_float2(mean, squares);
+  __syncthreads();
+  // (as in row_sums)
+  const int w = lane_id() % kNormMostWaves;
+  const float2 theirs = w < waves ? sh[turn][w] : make_float2(0.f, 0.f);
+  const float n = w < waves ? held_by(w) : 0.f;
+  const float all = group_sum<kNormMostWaves>(n * theirs.x) / static_cast<float>(cols), d = theirs.x - all;
+  return make_float2(all, group_sum<kNormMostWaves>(theirs.y + n * d * d) / static_cast<float>(cols));
 }
 
-template <typename T, int LANES, int UNITS>
+// Consecutive rows by a group of lanes, the next one's elements on their way while a row is worked on; weight and bias stay in
+// registers.
+template <typename T, int LANES, int UNITS, bool WHOLE>
 __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_fwd_kernel(const NormArgs a) {
   using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   __shared__ float2 sh[2][kNormMostWaves];
   const NormShare<LANES> share;
+  const RowUnits<T, UNITS, WHOLE> units(share.me, share.lanes, a.cols);
+  const int64_t first = block_index() * a.per_block * share.groups + share.group;
+  if (first >= a.rows) return;  // (of all lanes of a row at once)
+  auto source = [&](int64_t row) { return static_cast<const S *>(a.x) + (row < a.rows ? row : first) * a.x_stride; };
+  words_t raw[UNITS];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) raw[u] = units.load(source(first), u);
   float w[UNITS][N], b[UNITS][N];
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
-    const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
-    if (a.weight) load_typed<N>(a.weight, a.weight_dtype, c, a.cols - c, w[u]);
-    if (a.bias) load_typed<N>(a.bias, a.bias_dtype, c, a.cols - c, b[u]);
+    if (a.weight) units.typed(a.weight, a.weight_dtype, u, w[u]);
+    if (a.bias) units.typed(a.bias, a.bias_dtype, u, b[u]);
   }
   for (int64_t i = 0; i < a.per_block; ++i) {
-    const int64_t row = (block_index() * a.per_block + i) * share.groups + share.group;
-    if (row >= a.rows) return;  // (of all lanes of a row at once)
-    const S *const in = static_cast<const S *>(a.x) + row * a.x_stride;
+    const int64_t row = first + i * share.groups;
+    if (row >= a.rows) return;
     float x[UNITS][N];
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
-      unpack<T>(load_upto<T>(in + c, a.cols - c), x[u]);
+    for (int u = 0; u < UNITS; ++u) unpack<T>(raw[u], x[u]);
+    if (i + 1 < a.per_block) {
+      const S *const in = source(row + share.groups);
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) raw[u] = units.load(in, u);
     }
-    const float2 moments = row_moments<LANES, UNITS, N>(x, a.cols, share, sh, static_cast<int>(i & 1));
+    const float2 moments = row_moments<T, LANES>(x, units, share, sh, static_cast<int>(i & 1));
     const float mean = moments.x, rstd = 1.f / sqrtf(moments.y + a.eps);
     S *const out = static_cast<S *>(a.y) + row * a.cols;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         float v = (x[u][k] - mean) * rstd;
@@ -161,7 +187,7 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_f
         if (a.bias) v += b[u][k];
         x[u][k] = v;
       }
-      store_upto<T>(out + c, pack<T>(x[u]), a.cols - c);
+      units.store(out, u, pack<T>(x[u]));
     }
     if (share.me == 0) {
       if (a.mean) a.mean[row] = mean;
@@ -218,54 +244,63 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const NormArg
 // Blocks go over the rows, each keeping the column sums of its own in registers, and leave one row of partial sums each.  (Atomics
 // into one row of sums would make their order, and so the last bits, a matter of chance.)  Dynamic LDS: 2 groups cols floats where
 // groups of lanes share a block.
-template <typename T, int LANES, int UNITS>
+template <typename T, int LANES, int UNITS, bool WHOLE>
 __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_bwd_kernel(const NormArgs a) {
   using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
   __shared__ float2 sh[2][kNormMostWaves];
   const NormShare<LANES> share;
+  const RowUnits<T, UNITS, WHOLE> units(share.me, share.lanes, a.cols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * share.groups;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * share.groups + share.group;
+  words_t xr[UNITS], gr[UNITS];
+  float mean = 0.f, rstd = 0.f;
+  auto load = [&](int64_t r) {
+    r = r < a.rows ? r : 0;
+    const S *const in = static_cast<const S *>(a.x) + r * a.x_stride;
+    const S *const grad = static_cast<const S *>(a.dy) + r * a.dy_stride;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      xr[u] = units.load(in, u);
+      gr[u] = units.load(grad, u);
+    }
+    mean = a.mean[r];
+    rstd = a.rstd[r];
+  };
+  load(row);
   float w[UNITS][N], dw[UNITS][N], db[UNITS][N];
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
-    const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       w[u][i] = 1.f;
       dw[u][i] = 0.f;
       db[u][i] = 0.f;
     }
-    if (a.weight) load_typed<N>(a.weight, a.weight_dtype, c, a.cols - c, w[u]);
+    if (a.weight) units.typed(a.weight, a.weight_dtype, u, w[u]);
   }
-  int turn = 0;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * share.groups;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * share.groups + share.group; row < a.rows; row += step, turn ^= 1) {
-    const S *const in = static_cast<const S *>(a.x) + row * a.x_stride;
-    const S *const grad = static_cast<const S *>(a.dy) + row * a.dy_stride;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    words_t xr[UNITS], gr[UNITS];
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
-      xr[u] = load_upto<T>(in + c, a.cols - c);
-      gr[u] = load_upto<T>(grad + c, a.cols - c);
-    }
+  for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
     float c1 = 0.f, c2 = 0.f;
     float x[UNITS][N], g[UNITS][N];
+    const float r = rstd;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       unpack<T>(xr[u], x[u]);
       unpack<T>(gr[u], g[u]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {  // (behind the row's end all gradients are zeros)
-        const float unit = (x[u][i] - mean) * rstd;
+      for (int i = 0; i < N; ++i) {
+        const float unit = (x[u][i] - mean) * r;
         dw[u][i] = fmaf(g[u][i], unit, dw[u][i]);
         db[u][i] += g[u][i];
         g[u][i] *= w[u][i];
-        c1 += g[u][i];
-        c2 = fmaf(g[u][i], unit, c2);
         x[u][i] = unit;
       }
+      units.once(u, [&](int i) {
+        c1 += g[u][i];
+        c2 = fmaf(g[u][i], x[u][i], c2);
+      });
     }
+    load(row + step);
     if (a.y == nullptr) continue;
     const float2 sums = row_sums<LANES>(c1, c2, sh, turn);
     c1 = sums.x / static_cast<float>(a.cols);
@@ -273,38 +308,26 @@ __global__ __launch_bounds__(LANES == 0 ? 1024 : kNormThreads) void layer_norm_b
     S *const out = static_cast<S *>(a.y) + row * a.cols;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[u][i] = rstd * (g[u][i] - c1 - x[u][i] * c2);
-      store_upto<T>(out + c, pack<T>(x[u]), a.cols - c);
+      for (int i = 0; i < N; ++i) x[u][i] = r * (g[u][i] - c1 - x[u][i] * c2);
+      units.store(out, u, pack<T>(x[u]));
     }
   }
   if (a.partial == nullptr) return;
   float *const out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+  auto put = [&](float *to) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u)
+      units.each(u, [&](int i) {
+        to[units.column[u] + i] = dw[u][i];
+        to[a.cols + units.column[u] + i] = db[u][i];
+      });
+  };
   if constexpr (LANES == 0) {
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (c + i < a.cols) {
-          out[c + i] = dw[u][i];
-          out[a.cols + c + i] = db[u][i];
-        }
-    }
+    put(out);
   } else {
     extern __shared__ float sums[];  // [groups][2][cols]
-    float *const mine = sums + static_cast<int64_t>(share.group) * 2 * a.cols;
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int64_t c = (static_cast<int64_t>(u) * share.lanes + share.me) * N;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (c + i < a.cols) {
-          mine[c + i] = dw[u][i];
-          mine[a.cols + c + i] = db[u][i];
-        }
-    }
+    put(sums + static_cast<int64_t>(share.group) * 2 * a.cols);
     __syncthreads();
     for (int64_t c = threadIdx.x; c < 2 * a.cols; c += kNormThreads) {
       float s = 0.f;
@@ -401,6 +424,7 @@ __global__ __launch_bounds__(1024) void layer_norm_finish_kernel(const float *__
   const int wv = wave_index();
   float s = 0.f;
   if (c < cols)
+#pragma unroll 8
     for (int64_t p = wv; p < parts; p += kNormMostWaves) s += partial[(p * 2 + blockIdx.y) * cols + c];
   sh[wv][lane_id()] = s;
   __syncthreads();

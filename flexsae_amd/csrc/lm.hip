@@ -55,13 +55,14 @@ struct NormPlan {
   bool held = true;  // false: rows that no block holds
 };
 
-template <typename T, int LANES, int UNITS>
+template <typename T, int LANES, int UNITS, bool WHOLE = true>
 NormPlan norm_shared(bool backward) {
-  return {backward ? layer_norm_bwd_kernel<T, LANES, UNITS> : layer_norm_fwd_kernel<T, LANES, UNITS>, kNormThreads, kNormThreads / LANES};
+  return {backward ? layer_norm_bwd_kernel<T, LANES, UNITS, WHOLE> : layer_norm_fwd_kernel<T, LANES, UNITS, WHOLE>, kNormThreads,
+          kNormThreads / LANES};
 }
 template <typename T, int UNITS>
 NormPlan norm_block(int64_t units, bool backward) {
-  return {backward ? layer_norm_bwd_kernel<T, 0, UNITS> : layer_norm_fwd_kernel<T, 0, UNITS>,
+  return {backward ? layer_norm_bwd_kernel<T, 0, UNITS, true> : layer_norm_fwd_kernel<T, 0, UNITS, true>,
           static_cast<int>(ceil_div(units, kWave * UNITS)) * kWave, 1};
 }
 
@@ -70,12 +71,13 @@ NormPlan norm_plan(int64_t cols, bool backward) {
   constexpr int64_t N = kUnitOf<T>;
   constexpr int kEight = 8 / N, kSixteen = 16 / N;  // units of 8 and 16 elements
   const int64_t units = ceil_div(cols, N);
+  if (cols < N) return norm_shared<T, 16, 1, false>(backward);
   if (units <= 16) return norm_shared<T, 16, 1>(backward);
   if (units <= 32) return norm_shared<T, 32, 1>(backward);
   if (units <= 64) return norm_shared<T, 64, 1>(backward);
   if (units <= 64 * kEight) return norm_shared<T, 64, kEight>(backward);
   if (units <= 64 * kSixteen) return norm_shared<T, 64, kSixteen>(backward);
-  if (units <= 8 * 64 * kEight) return norm_block<T, kEight>(units, backward);
+  if (units <= (backward ? kNormMostWaves : 8) * 64 * kEight) return norm_block<T, kEight>(units, backward);
   if (units <= kNormMostWaves * 64 * kSixteen) return norm_block<T, kSixteen>(units, backward);
   return {backward ? layer_norm_bwd_long_kernel<T> : layer_norm_fwd_long_kernel<T>, 1024, 1, false};
 }
@@ -126,7 +128,12 @@ int flexsae_layer_norm_fwd(const flexsae_norm *n, const void *x, const void *wei
   a.mean = mean;
   a.rstd = rstd;
   const NormPlan plan = norm_plan(*n, false);
-  const int64_t blocks = ceil_div(n->rows, plan.groups);
+  if (plan.held) {
+    // rows of a block one after another, where there are blocks enough for eight rounds of them
+    const int64_t rounds = n->rows / (plan.groups * kComputeUnits * (2048 / plan.threads) * 8);
+    a.per_block = rounds < 1 ? 1 : rounds > 8 ? 8 : rounds;
+  }
+  const int64_t blocks = ceil_div(n->rows, plan.groups * a.per_block);
   plan.kernel<<<grid_of(blocks), plan.threads, 0, as_stream(stream)>>>(a);
   return launch_status();
 }
