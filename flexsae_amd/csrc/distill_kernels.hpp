@@ -451,19 +451,22 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
     store_whole<T>(out + at, pack<T>(x), at < whole);
   }
   if (last < cols) out[last] = Traits<T>::down(gradient(tail));
-  // the stored entries among the thread's columns, in whose places the gradients above have been stored by this very thread
+  // The stored entries among the thread's columns, in whose places the gradients above have been stored by this very thread.  One that
+  // is stored more than once is summed in 52 bits of the largest, whose sum no order changes, and its places leave the chain.
   for (int j = head[k]; j >= 0; j = chain[j]) {
-    float all = 0.f;
-    int from = -1;
-    for (;;) {  // an entry that is stored more than once: its places in their order
-      int least = THREADS;
-      for (int i = head[k]; i >= 0; i = chain[i])
-        if (stored[i] == stored[j] && i > from && i < least) least = i;
-      if (least == THREADS) break;
-      all += stored_p[least];
-      from = least;
+    const int entry = stored[j];
+    float all = stored_p[j];
+    int64_t more = 0;
+    for (int before = j, i = chain[j]; i >= 0; i = chain[i]) {
+      if (stored[i] != entry) {
+        before = i;
+        continue;
+      }
+      more += static_cast<int64_t>(stored_p[i] * 0x1p52f);
+      chain[before] = chain[i];
     }
-    out[stored[j]] = Traits<T>::down(gradient(stored_z[j]) - coef * (all * inv_top));
+    if (more != 0) all = static_cast<float>(static_cast<int64_t>(all * 0x1p52f) + more) * 0x1p-52f;
+    out[entry] = Traits<T>::down(gradient(stored_z[j]) - coef * (all * inv_top));
   }
 }
 

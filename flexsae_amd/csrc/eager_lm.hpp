@@ -47,7 +47,7 @@ bool take_optional(PyObject *o, Tensor &out) {
 
 // ---- layer norm ----------------------------------------------------------------------------
 bool usable_norm(const Tensor &x, const Tensor &weight, const Tensor &bias) {
-  if (!plain_tensor(x) || x.dim() < 1 || x.size(-1) < 1 || dtype_of(x.scalar_type()) < 0) return false;
+  if (!plain_tensor(x) || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) >= (int64_t{1} << 27) || dtype_of(x.scalar_type()) < 0) return false;
   for (const Tensor *t : {&weight, &bias})
     if (t->defined() && (!plain_beside(*t, x) || t->dim() != 1 || t->size(0) != x.size(-1) || dtype_of(t->scalar_type()) < 0)) return false;
   return true;

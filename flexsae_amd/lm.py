@@ -88,6 +88,8 @@ def _check_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps
         _float(name, t)
         if tuple(t.shape) != (x.shape[-1],):
             raise ValueError(f"layer_norm: {name} is {tuple(t.shape)}, rows have {x.shape[-1]} columns")
+    if x.shape[-1] >= 2 ** 27 or x.numel() // x.shape[-1] >= 2 ** 32:
+        raise ValueError("sizes beyond the kernels' index range: need fewer than 2^32 rows of fewer than 2^27 columns")
     if not (eps >= 0 and math.isfinite(eps)):
         raise ValueError(f"layer_norm: eps must be finite and not negative, got {eps}")
     _on_one_gpu(("x", x), ("weight", weight), ("bias", bias))

@@ -562,7 +562,7 @@ int flexsae_adamw8_moments(const flexsae_adamw8_state *states, int64_t count, in
  * entry points write is contiguous, and nothing that they write may overlap what they read.  (No reference counterpart.)
  */
 typedef struct {
-  int64_t rows, cols;          /* cols >= 1 */
+  int64_t rows, cols;          /* rows < 2^32, 1 <= cols < 2^27 */
   int64_t x_stride, dy_stride; /* between rows of x and of dy */
   float eps;                   /* not negative */
   int32_t dtype;               /* flexsae_dtype of x, y, dy, dx */

@@ -461,6 +461,17 @@ def test_distill_entries_stored_twice():
     index[:, 20:] = index[:, :20].flip(1)
     index[3] = index[3, 0]
     _check_distill(z, top, index)
+    # rows in registers: all places of a row the same, two in turn, and many entries of one thread
+    for k in (200, 1000):
+        z, top, index = _distill_inputs(260, 9000, k, torch.float32, seed=14)
+        index[0], index[1], index[2] = 8999, torch.arange(k, device=DEV) % 2, torch.arange(k, device=DEV) % 4
+        index[3] = torch.arange(k, device=DEV) % 8 * 4096 // 4
+        top[4:8] = -1e4
+        top[4:8, -1] = 1.0
+        index[4:8, :-1] = 0  # (places without weight, as of padding)
+        first = _check_distill(z, top, index)
+        again = _check_distill(z, top, index)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
 def test_distill_indices_outside_the_vocabulary():
