@@ -8,6 +8,13 @@
 // vocabulary holds no logit.  A row of weight zero, or without a stored logit above minus infinity, is not read: it counts as zero
 // and has a gradient of zeros.
 //
+// Three ways.  With the gradient of a mean a row is read once, into the registers of one block (distill_held_kernel): maximum, sum
+// and gradient from there.  8192 rows of 131072 bf16: 855 us, 5.0 TB/s of reads and writes where a copy by the library reaches 4.8;
+// statistics and gradient by passes of their own take 1440, and one block a row that reads it twice 1270: a second read comes no
+// faster from the Infinity Cache.  At this size a block fills its compute unit, whose memory rests while it takes the sum.
+// Few long rows, rows that no block holds and losses without a gradient go by parts of rows (121 us for 537 MB), joined by a wavefront a
+// row; and gradients for an upstream gradient that the forward did not know by parts of rows again (46 us for 102 MB read and written).
+//
 // The row's statistics are its maximum m and s = sum of exp((z - m) / T), in one pass: a running maximum per lane, sums rescaled
 // when it moves.  Exponents are of differences from the maximum, so that large logits cost no digits.
 #pragma once
@@ -61,7 +68,7 @@ __device__ __forceinline__ float2 join(float2 a, float2 b, float c) {
 
 // Takes the elements [from, end) of a row, THREADS units at a time, to `with` (first column, elements, how many of them are in the
 // row), with kAhead units of a thread on their way at once.
-template <typename T, int THREADS, typename F>
+template <typename T, int THREADS, bool NT, typename F>
 __device__ __forceinline__ void walk(const elem_t<T> *in, int64_t from, int64_t end, F with) {
   constexpr int N = kUnitOf<T>, kAhead = 4;
   constexpr int64_t kStep = THREADS * N;
@@ -70,7 +77,7 @@ __device__ __forceinline__ void walk(const elem_t<T> *in, int64_t from, int64_t 
   for (; at + (kAhead - 1) * kStep + N <= end; at += kAhead * kStep) {
     words_t v[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) v[u] = load_words<T>(in + at + u * kStep);
+    for (int u = 0; u < kAhead; ++u) v[u] = load_words<T, NT>(in + at + u * kStep);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       unpack<T>(v[u], x);
@@ -133,7 +140,7 @@ __global__ __launch_bounds__(kDistillThreads) void distill_parts_kernel(const Di
   const int64_t end = (split + 1) * a.part < a.vocab ? (split + 1) * a.part : a.vocab;
   const float c = kLog2e * a.inv_t;
   float2 ms = make_float2(-FLT_MAX, 0.f);
-  walk<T, kDistillThreads>(in, split * a.part, end, [&](int64_t, float (&x)[N], int64_t left) {
+  walk<T, kDistillThreads, true>(in, split * a.part, end, [&](int64_t, float (&x)[N], int64_t left) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (i >= left) x[i] = -INFINITY;
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const Dis
   }
   const RowExp e(st.x, a.inv_t);
   const float each = coef / st.y;
-  walk<T, kDistillThreads>(in, from, end, [&](int64_t at, float (&x)[N], int64_t left) {
+  walk<T, kDistillThreads, false>(in, from, end, [&](int64_t at, float (&x)[N], int64_t left) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = each * e.of(x[i]);
     store_upto<T>(out + at, pack<T>(x), left);
@@ -310,35 +317,22 @@ struct LargestBits<float> {
   __device__ __forceinline__ float value() const { return most; }
 };
 
-// A block's threads share out the places of the teacher, one a thread.
-struct Stored {
-  int index;  // -1: none
-  float top;
-};
-__device__ __forceinline__ Stored load_stored(const DistillArgs &a, int64_t row) {
-  Stored t = {-1, 0.f};
-  const int k = static_cast<int>(threadIdx.x);
-  if (row >= a.rows || k >= a.k) return t;
-  const int64_t i = a.index[row * a.k + k];
-  t.top = load_scalar(a.top, a.top_dtype, row * a.k + k);
-  if (i >= 0 && i < a.vocab) t.index = static_cast<int>(i);
-  else if (a.flag && i != -1) atomicOr(a.flag, FLEXSAE_FLAG_TOKEN_RANGE);
-  return t;
-}
-
 // A row that is not used: a gradient of zeros, and no loss.
-template <typename T, int THREADS, bool GRAD>
+template <typename T, int THREADS>
 __device__ __forceinline__ void unused_row(const DistillArgs &a, int64_t row) {
   constexpr int N = kUnitOf<T>;
   if (threadIdx.x == 0) {
     a.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
     a.row_loss[row] = 0.f;
   }
-  if constexpr (!GRAD) return;
   elem_t<T> *const out = static_cast<elem_t<T> *>(a.dlogits) + row * a.vocab;
   for (int64_t at = static_cast<int64_t>(threadIdx.x) * N; at < a.vocab; at += THREADS * N) store_upto<T>(out + at, words_t(0u), a.vocab - at);
 }
 
+// Loads are unconditional (lanes behind the row's end read its first elements, and put them aside): one that waits for its own
+// condition waits for those before it, which made the whole of this kernel 1.2 times as long.  The stored entries are put in their
+// places by the threads whose columns they are, so that no barrier waits for the stores; a search for entries that are stored twice, by
+// each against all, was 5 us a row.
 template <typename T, int THREADS, int UNITS>
 __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs a) {
   using S = elem_t<T>;
@@ -352,10 +346,7 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
   const int64_t row = block_index();
   if (row >= a.rows) return;
   const float weight = row_weight(a, row);
-  if (weight == 0.f) {
-    (void)load_stored(a, row);
-    return unused_row<T, THREADS, true>(a, row);
-  }
+  if (weight == 0.f) return unused_row<T, THREADS>(a, row);
   // whole units, and behind them up to N - 1 elements, one of a thread
   const uint32_t cols = static_cast<uint32_t>(a.vocab), whole = cols - cols % N, first = threadIdx.x * N, last = whole + threadIdx.x;
   const S *const in = static_cast<const S *>(a.logits) + row * a.stride;
@@ -396,7 +387,7 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
     m = fmaxf(m, maxima[w].x);
     top = fmaxf(top, maxima[w].y);
   }
-  if (top == -INFINITY) return unused_row<T, THREADS, true>(a, row);
+  if (top == -INFINITY) return unused_row<T, THREADS>(a, row);
   const RowExp e(m, a.inv_t);
   const float p = index < 0 ? 0.f : exp_of(t - top, kLog2e * a.inv_t);
   stored_p[k] = p;

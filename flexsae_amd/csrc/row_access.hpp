@@ -41,14 +41,20 @@ __device__ __forceinline__ elem_t<T> from_bits(uint32_t v) {
   else return static_cast<uint16_t>(v);
 }
 
-template <typename T>
+// NT: streaming, for what is read or written once and not soon again.
+template <typename T, bool NT = false>
 __device__ __forceinline__ words_t load_words(const elem_t<T> *p) {
-  return *reinterpret_cast<const typename LooseWords<T>::type *>(p);
+  const auto *q = reinterpret_cast<const typename LooseWords<T>::type *>(p);
+  if constexpr (NT) return __builtin_nontemporal_load(q);
+  else return *q;
 }
 
-template <typename T>
+template <typename T, bool NT = false>
 __device__ __forceinline__ void store_whole(elem_t<T> *p, words_t v, bool there) {
-  if (there) *reinterpret_cast<typename LooseWords<T>::type *>(p) = v;
+  using L = typename LooseWords<T>::type;
+  if (!there) return;
+  if constexpr (NT) __builtin_nontemporal_store(static_cast<L>(v), reinterpret_cast<L *>(p));
+  else *reinterpret_cast<L *>(p) = v;
 }
 
 // The first `left` of the elements at p, zeros for the rest.
