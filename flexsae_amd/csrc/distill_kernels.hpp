@@ -346,7 +346,13 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
   const int64_t row = block_index();
   if (row >= a.rows) return;
   const float weight = row_weight(a, row);
-  if (weight == 0.f) return unused_row<T, THREADS>(a, row);
+  if (weight == 0.f) {
+    if (static_cast<int64_t>(threadIdx.x) < a.k && a.flag) {
+      const int64_t i = a.index[row * a.k + threadIdx.x];
+      if (i < -1 || i >= a.vocab) atomicOr(a.flag, FLEXSAE_FLAG_TOKEN_RANGE);
+    }
+    return unused_row<T, THREADS>(a, row);
+  }
   // whole units, and behind them up to N - 1 elements, one of a thread
   const uint32_t cols = static_cast<uint32_t>(a.vocab), whole = cols - cols % N, first = threadIdx.x * N, last = whole + threadIdx.x;
   const S *const in = static_cast<const S *>(a.logits) + row * a.stride;

@@ -482,6 +482,12 @@ def test_distill_indices_outside_the_vocabulary():
         flex.check_index_flag()
     _check_distill(z, top, index.clamp(-1, 59).int())
     flex.check_index_flag()
+    weights = torch.ones(5, device=DEV)
+    weights[0] = weights[1] = weights[2] = 0.0  # (also of rows that are not used)
+    for leaf in (z, z.clone().requires_grad_()):
+        flex.distillation_loss(leaf, top, index, row_weights=weights)
+        with pytest.raises(IndexError, match="token"):
+            flex.check_index_flag()
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
