@@ -178,6 +178,15 @@ bool capturing(const Tensor &t) {
   const c10::DeviceGuard guard(t.device());
   return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
 }
+// The graph that the tensor's current stream is captured into: 0 for none, else a number of its own.
+int64_t capture_of(const Tensor &t) {
+  const c10::DeviceGuard guard(t.device());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const hipError_t rc = hipStreamGetCaptureInfo(c10::hip::getCurrentHIPStream(t.device().index()).stream(), &status, &id);
+  TORCH_CHECK(rc == hipSuccess, "hipStreamGetCaptureInfo: ", hipGetErrorString(rc));
+  return status == hipStreamCaptureStatusNone ? 0 : static_cast<int64_t>(id) + 1;
+}
 const int64_t *index_ptr(const Tensor &t) { return t.const_data_ptr<int64_t>(); }
 float *f32(const Tensor &t) { return t.data_ptr<float>(); }
 

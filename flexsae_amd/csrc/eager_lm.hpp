@@ -296,7 +296,10 @@ struct Distill : torch::autograd::Function<Distill> {
     ctx->saved_data["t"] = temperature;
     ctx->saved_data["by_row"] = by_row;
     // no saved tensor: the backward completes it in place and hands the very buffer on
-    if (early) ctx->saved_data["dlogits"] = dlogits;
+    if (early) {
+      ctx->saved_data["dlogits"] = dlogits;
+      ctx->saved_data["capture"] = capture_of(logits);
+    }
     return loss;
   }
 
@@ -326,8 +329,10 @@ struct Distill : torch::autograd::Function<Distill> {
       dlogits = at->second.toTensor();
       ctx->saved_data.erase("dlogits");  // the buffer now belongs to whoever receives the gradient
     }
+    // (not one of another graph, or of none: what a replay writes there would be another's, or what it finds there no gradient for
+    // an upstream gradient of one any more)
     const bool early = dlogits.defined() && dlogits.device() == logits.device() && dlogits.sizes() == logits.sizes() &&
-                       dlogits.scalar_type() == logits.scalar_type();
+                       dlogits.scalar_type() == logits.scalar_type() && ctx->saved_data["capture"].toInt() == capture_of(logits);
     if (!early) dlogits = make(logits, logits.sizes(), logits.scalar_type());
     const flexsae_distill d = distill_of(logits, z.stride, t.top, temperature, by_row);
     check(lib.distill_bwd(&d, z.t.const_data_ptr(), t.top.const_data_ptr(), index_ptr(t.index), weights_ptr(t), f32(stats), f32(grad),
