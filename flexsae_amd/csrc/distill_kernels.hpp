@@ -280,6 +280,10 @@ __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const Dis
   stored_entries<T, kDistillThreads>(a, row, from, end, st, e, coef);
 }
 
+// For sums of probabilities that no order changes: p 2^up as a whole number, of p below 2^(52 - up); 2^11 of them fit.
+__device__ __forceinline__ int exponent_of(float p) { return __builtin_amdgcn_frexp_expf(p); }
+__device__ __forceinline__ int64_t scaled(float p, int up) { return static_cast<int64_t>(ldexpf(p, up)); }
+
 // ---- a row in the registers of one block ------------------------------------------------------
 
 // Words of minus infinities.
@@ -448,21 +452,31 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
     store_whole<T>(out + at, pack<T>(x), at < whole);
   }
   if (last < cols) out[last] = Traits<T>::down(gradient(tail));
-  // The stored entries among the thread's columns, in whose places the gradients above have been stored by this very thread.  One that
-  // is stored more than once is summed in 52 bits of the largest, whose sum no order changes, and its places leave the chain.
+  // The stored entries among the thread's columns, in whose places the gradients above have been stored by this very thread.  What an
+  // entry's places have is summed in 52 bits of the largest of them, exact numbers of which no order changes the sum (the chain's order is
+  // that of the exchanges above), and its places leave the chain.
   for (int j = head[k]; j >= 0; j = chain[j]) {
     const int entry = stored[j];
-    float all = stored_p[j];
-    int64_t more = 0;
-    for (int before = j, i = chain[j]; i >= 0; i = chain[i]) {
-      if (stored[i] != entry) {
-        before = i;
-        continue;
+    float all = stored_p[j], most = all;
+    bool more = false;
+    for (int i = chain[j]; i >= 0; i = chain[i])
+      if (stored[i] == entry) {
+        most = fmaxf(most, stored_p[i]);
+        more = true;
       }
-      more += static_cast<int64_t>(stored_p[i] * 0x1p52f);
-      chain[before] = chain[i];
+    if (more) {
+      const int up = 52 - exponent_of(most);
+      int64_t sum_up = scaled(all, up);
+      for (int before = j, i = chain[j]; i >= 0; i = chain[i]) {
+        if (stored[i] != entry) {
+          before = i;
+          continue;
+        }
+        sum_up += scaled(stored_p[i], up);
+        chain[before] = chain[i];
+      }
+      all = ldexpf(static_cast<float>(sum_up), -up);
     }
-    if (more != 0) all = static_cast<float>(static_cast<int64_t>(all * 0x1p52f) + more) * 0x1p-52f;
     out[entry] = Traits<T>::down(gradient(stored_z[j]) - coef * (all * inv_top));
   }
 }

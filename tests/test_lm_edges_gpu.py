@@ -1,6 +1,4 @@
 """Layer norm, lookup and distillation where calls, values and captures are out of the ordinary (bounds of tests/lm_reference.py)."""
-import math
-
 import pytest
 import torch
 
@@ -69,3 +67,29 @@ def test_an_eager_backward_of_a_captured_forward(dtype):
     want, tol = ref.distill(z, top, index, None, 1.0, False, torch.ones(()))
     ref.within(dz, want["dz"], ref.rounded(want["dz"], dtype, tol["dz"]), "dz")
     del graph
+
+
+# ---- distillation's values -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=NAMES[:2])  # (the range of fp16 does not hold such gradients)
+@pytest.mark.parametrize("n,v,k", [(70, 5000, 12), (260, 9000, 200), (260, 40000, 900), (5, 700, 1500)])
+@pytest.mark.parametrize("by_row", [False, True])
+def test_entries_stored_twice_with_small_probabilities(n, v, k, dtype, by_row):
+    """Places of one entry far below the row's largest add up as others do, and to the same bits on every run; the student's own
+    probability of it vanishes, so that they are all of its gradient."""
+    z, top, index = _distill_inputs(n, v, k, dtype, seed=n + k, top_dtype=torch.float32)
+    index = 18 + index % (v - 18)
+    index[:, 0] = 0
+    top[:, 0] = 1.0
+    for row in range(4):  # below 2^-52 of the largest, about there, and between there and 2^-28
+        place = torch.arange(1, 9, device=DEV) * ((k - 1) // 8)
+        index[row, place] = 17
+        top[row, place] = torch.linspace(-39.0, -40.0, 8, device=DEV) + 8.0 * row
+    index[4, 1:] = 17  # all but one
+    top[4, 1:] = -45.0 + torch.rand(k - 1, generator=_gen(3)).to(DEV)
+    z[:, 17] = -200.0
+    first = _check_distill(z, top, index, by_row=by_row)[1]
+    assert (first[:5, 17] < 0).all()
+    for _ in range(4):
+        assert torch.equal(first, _check_distill(z, top, index, by_row=by_row)[1])
