@@ -401,7 +401,8 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
   const RowExp e(m, a.inv_t);
   const float p = index < 0 ? 0.f : exp_of(t - top, kLog2e * a.inv_t);
   stored_p[k] = p;
-  if (p != 0.f) {
+  // (a place without a share is left out, but not of a teacher that has none to give, whose shares are all NaN)
+  if (index >= 0 && (p != 0.f || top == INFINITY)) {
     chain[k] = atomicExch(&head[static_cast<uint32_t>(index) < whole ? static_cast<uint32_t>(index) / N % THREADS : static_cast<uint32_t>(index) - whole], k);
   }
   float sum = e.of(tail);

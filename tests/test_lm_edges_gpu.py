@@ -1,4 +1,6 @@
 """Layer norm, lookup and distillation where calls, values and captures are out of the ordinary (bounds of tests/lm_reference.py)."""
+import math
+
 import pytest
 import torch
 
@@ -93,3 +95,18 @@ def test_entries_stored_twice_with_small_probabilities(n, v, k, dtype, by_row):
     assert (first[:5, 17] < 0).all()
     for _ in range(4):
         assert torch.equal(first, _check_distill(z, top, index, by_row=by_row)[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("lost", [math.nan, math.inf])
+@pytest.mark.parametrize("by_row", [False, True])
+def test_a_teacher_without_a_distribution(lost, by_row, dtype):
+    """A stored logit that is NaN or infinite leaves none of the row's stored entries a probability: their gradients are NaN, those of
+    the other entries and rows what they are."""
+    for n, v, k in ((12, 900, 7), (260, 9000, 300)):
+        z, top, index = _distill_inputs(n, v, k, dtype, seed=v)
+        index[:, 0] = 5
+        top[2, 0], top[7, k - 1] = lost, lost
+        loss, dz = _check_distill(z, top, index, by_row=by_row)
+        assert dz[2, index[2]].isnan().all() and not dz[3].isnan().any()
+        assert loss[[2, 7]].isnan().all() if by_row else loss.isnan()
