@@ -35,8 +35,8 @@ struct DistillArgs {
   const float *row_weights;  // or NULL
   float2 *parts;             // [rows][splits]: maximum and sum of a part of a row
   float4 *stats;             // [rows]: m, s, the teacher's maximum, 1 / sum of its exponentials (0: the row is not used);
-                             // [rows].x: one over the sum of the weights
-  float *row_loss;           // [rows]
+                             // [rows]: one over the sum of the weights, in 64 bits
+  float *row_loss;           // [rows], times their weights' shares
   float *loss;
   const float *grad;  // upstream gradient: one number, or one of every row; NULL: one
   void *dlogits;
@@ -118,14 +118,18 @@ __global__ __launch_bounds__(1024) void distill_weights_kernel(const DistillArgs
   if (threadIdx.x != 0) return;
   s = 0.;
   for (int w = 0; w < 1024 / kWave; ++w) s += sh[w];
-  a.stats[a.rows].x = s == 0. ? 0.f : static_cast<float>(1. / s);  // (the mean of no rows is zero)
+  *reinterpret_cast<double *>(a.stats + a.rows) = s == 0. ? 0. : 1. / s;  // (the mean of no rows is zero)
 }
 
-// Weight of a row with regard to the mean.
+// Weight of a row, and its share of a mean.  (Of weights by 64 bits: their sum, and one over it, may be beyond the normal numbers of
+// fp32 where they are not.)
 __device__ __forceinline__ float row_weight(const DistillArgs &a, int64_t row) { return a.row_weights ? a.row_weights[row] : 1.f; }
+__device__ __forceinline__ float weight_share(const DistillArgs &a, float weight) {
+  return a.by_row || !a.row_weights ? weight : static_cast<float>(weight * *reinterpret_cast<const double *>(a.stats + a.rows));
+}
+// ... times this: where there are no weights the rows share it evenly
 __device__ __forceinline__ float mean_factor(const DistillArgs &a) {
-  if (a.by_row) return 1.f;
-  return a.row_weights ? a.stats[a.rows].x : 1.f / static_cast<float>(a.rows);
+  return a.by_row || a.row_weights ? 1.f : 1.f / static_cast<float>(a.rows);
 }
 
 // Statistics of a part of a row: block = row * splits + part.
@@ -198,7 +202,7 @@ __device__ __forceinline__ void finish_row(const DistillArgs &a, int64_t row, fl
   }
   if (lane != 0) return;
   a.stats[row] = make_float4(ms.x, ms.y, t.x, used ? 1.f / t.y : 0.f);
-  a.row_loss[row] = used ? a.t * a.t * weight * loss : 0.f;
+  a.row_loss[row] = used ? a.t * a.t * weight_share(a, weight) * loss : 0.f;
 }
 
 // Rows whose parts are there: a wavefront a row.
@@ -262,7 +266,7 @@ __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const Dis
   const S *const in = static_cast<const S *>(a.logits) + row * a.stride;
   S *const out = static_cast<S *>(a.dlogits) + row * a.vocab;
   const float upstream = a.grad == nullptr ? 1.f : a.grad[a.by_row ? row : 0];
-  const float coef = a.t * row_weight(a, row) * mean_factor(a) * upstream;
+  const float coef = a.t * weight_share(a, row_weight(a, row)) * mean_factor(a) * upstream;
   const bool used = st.w != 0.f;
   if (!used) {
     for (int64_t at = from + static_cast<int64_t>(threadIdx.x) * N; at < end; at += kDistillThreads * N)
@@ -429,7 +433,7 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
     sum += sums[w].x;
     sum_top += sums[w].y;
   }
-  const float inv_top = 1.f / sum_top, log_s = logf(sum);
+  const float inv_top = 1.f / sum_top, log_s = logf(sum), share = weight_share(a, weight);
   if (wave_index() == 0) {
     const float logs = logf(sum_top) - log_s;
     float loss = 0.f;
@@ -438,10 +442,10 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(const DistillArgs
     loss = group_sum<kWave>(loss);
     if (k == 0) {
       a.stats[row] = make_float4(m, sum, top, inv_top);
-      a.row_loss[row] = a.t * a.t * weight * loss;
+      a.row_loss[row] = a.t * a.t * share * loss;
     }
   }
-  const float coef = a.t * weight * mean_factor(a), each = coef / sum;
+  const float coef = a.t * share * mean_factor(a), each = coef / sum;
   auto gradient = [&](float x) { return each * e.of(x); };
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {

@@ -110,3 +110,17 @@ def test_a_teacher_without_a_distribution(lost, by_row, dtype):
         loss, dz = _check_distill(z, top, index, by_row=by_row)
         assert dz[2, index[2]].isnan().all() and not dz[3].isnan().any()
         assert loss[[2, 7]].isnan().all() if by_row else loss.isnan()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -140, 2.0 ** -130, 2.0 ** 118, 2.0 ** 126])
+def test_row_weights_of_any_size(size):
+    """Of a mean only the ratios of the weights count, also where their sum, or one over it, is beyond the normal numbers of fp32."""
+    n = 600
+    weights = (1.0 + torch.randint(0, 2, (n,), generator=_gen(5)) * (torch.arange(n) > 2)).to(DEV)
+    weights[3] = 0.0
+    for dtype in DTYPES:
+        z, top, index = _distill_inputs(n, 700, 9, dtype, seed=50)
+        scale = 1.0 if dtype != torch.float16 else 4096.0
+        loss, dz = _check_distill(z, top, index, weights, grad=scale)
+        again, dz2 = _check_distill(z, top, index, weights * size, grad=scale)
+        assert torch.equal(loss, again) and torch.equal(dz, dz2)
