@@ -317,7 +317,8 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: Union[None, float, T
     if isinstance(scale, (int, float)):
         factor, scale = float(scale), None
     elif scale is not None and scale.shape != tokens.shape:
-        scale = scale.expand(tokens.shape)
+        _float("scale", scale)
+        scale = scale.to(torch.float32).expand(tokens.shape)  # (shares of its gradient are added up before they are rounded)
     tokens = _indices("tokens", tokens)
     native = _native(weight)
     if native is not None:

@@ -124,3 +124,32 @@ def test_row_weights_of_any_size(size):
         loss, dz = _check_distill(z, top, index, weights, grad=scale)
         again, dz2 = _check_distill(z, top, index, weights * size, grad=scale)
         assert torch.equal(loss, again) and torch.equal(dz, dz2)
+
+
+# ---- lookup --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+def test_the_gradient_of_a_broadcast_scale_is_rounded_once(dtype):
+    """Shares of tokens that nearly cancel, each of which a 16-bit type would round by more than is left of their sum."""
+    n = 256
+    w = torch.ones(3, 40, device=DEV, dtype=dtype)
+    tokens = torch.arange(n, device=DEV) % 3
+    dout = torch.zeros(n, 40, device=DEV, dtype=dtype)
+    dout[:, 0] = torch.where(torch.arange(n, device=DEV) % 2 == 0, 1.0, -1.0).to(dtype)
+    dout[::2, 1] = torch.finfo(dtype).eps * 0.375
+    for shape in ((), (1,), (16, 1), (1, 16)):
+        cube = tokens if len(shape) < 2 else tokens.view(16, 16)
+        scale = torch.full(shape, 1.5, device=DEV, dtype=dtype, requires_grad=True)
+        out = flex.embedding_lookup(cube, w, scale)
+        assert out.dtype == dtype and out.eq(1.5).all()
+        out.backward(dout.view(*cube.shape, 40))
+        assert scale.grad.dtype == dtype and scale.grad.shape == scale.shape
+        want, _ = ref.lookup(tokens, w, torch.full((n,), 1.5), 1.0, dout)
+        shares = want["ds"].view(cube.shape)
+        for axis, size in enumerate(shape if len(shape) == 2 else ()):
+            if size == 1:
+                shares = shares.sum(axis, keepdim=True)
+        shares = shares.sum().view(shape) if len(shape) < 2 else shares
+        many = n // scale.numel()  # (shares of at most 1 + 2^-8, added up in any order)
+        ref.within(scale.grad, shares, ref.rounded(shares, dtype, many * (many + 4) * ref.U), str(shape))
