@@ -75,10 +75,11 @@ def check_index_flag(device=None) -> None:
     bits = int(flag.item())
     if bits:
         flag.zero_()
-        if bits & _lib.FLAG_INDEX_RANGE:
-            raise IndexError("flexsae_amd: an entry of `indices` was outside [0, F)")
-        if bits & _lib.FLAG_TOKEN_RANGE:
-            raise IndexError("flexsae_amd: a token or an entry of `top_indices` was outside [0, V) and not -1")
+        seen = [text for bit, text in ((_lib.FLAG_INDEX_RANGE, "an entry of `indices` was outside [0, F)"),
+                                       (_lib.FLAG_TOKEN_RANGE, "a token or an entry of `top_indices` was outside [0, V) and not -1"))
+                if bits & bit]
+        if seen:
+            raise IndexError("flexsae_amd: " + "; ".join(seen))
         raise RuntimeError(f"flexsae_amd: device status flag {bits:#x}")
 
 

@@ -153,3 +153,16 @@ def test_the_gradient_of_a_broadcast_scale_is_rounded_once(dtype):
         shares = shares.sum().view(shape) if len(shape) < 2 else shares
         many = n // scale.numel()  # (shares of at most 1 + 2^-8, added up in any order)
         ref.within(scale.grad, shares, ref.rounded(shares, dtype, many * (many + 4) * ref.U), str(shape))
+
+
+# ---- the flag ------------------------------------------------------------------------------
+
+
+def test_the_flag_names_all_that_was_out_of_range():
+    w = torch.randn(10, 24, device=DEV)
+    flex.embedding_lookup(torch.tensor([3, 10], device=DEV), w)
+    flex.triton_topk_sae_loss(torch.tensor([[1, 10]], device=DEV), w, torch.ones(1, 2, device=DEV), torch.zeros(24, device=DEV),
+                              torch.zeros(1, 24, device=DEV))
+    with pytest.raises(IndexError, match=r"(?s)`indices`.*token"):
+        flex.check_index_flag()
+    flex.check_index_flag()
