@@ -146,9 +146,22 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_fwd_kernel(const Lookup
   }
 }
 
+// Brings the places of tokens that are rows, among the group's `count`, to its first lanes, in their order; -> how many there are.
+template <int LANES>
+__device__ __forceinline__ int rows_first(const LookupArgs &a, int count, uint32_t &place) {
+  const int me = static_cast<int>(threadIdx.x) % LANES, first = lane_id() - me;
+  const bool there = me < count && row_of(a.tokens[place], a.vocab) >= 0;
+  const uint64_t group = (__ballot(there) >> first) & (LANES == kWave ? ~uint64_t{0} : (uint64_t{1} << LANES) - 1);
+  const int kept = __popcll(group), before = __popcll(group & ((uint64_t{1} << me) - 1));
+  const int to = there ? before : kept + me - before;
+  place = static_cast<uint32_t>(__builtin_amdgcn_ds_permute((first + to) * 4, static_cast<int>(place)));
+  return kept;
+}
+
 // Adds the rows of dout at sorted places [from, to), all of one token, to `sum`; w: the token's row (used with dots).  check: the
-// places may be of tokens that are no row (they are filed under row 0).  Places and scales of LANES tokens are read at once, a lane
-// each, and AHEAD rows are on their way together: a walk that waits for each place and then for its row takes 3 latencies a row.
+// places may be of tokens that are no row (they are filed under row 0), whose rows of dout are not read.  Places and scales of LANES
+// tokens are read at once, a lane each, and AHEAD rows are on their way together: a walk that waits for each place and then for its row
+// takes 3 latencies a row.
 template <typename T, int LANES, int UNITS, bool WHOLE, bool DOTS, int AHEAD>
 __device__ __forceinline__ void add_places(const LookupArgs &a, const LookupPlace<T, LANES, UNITS, WHOLE> &at, uint32_t from, uint32_t to,
                                            bool check, const float (&w)[UNITS][kUnitOf<T>], float (&sum)[UNITS][kUnitOf<T>]) {
@@ -156,29 +169,27 @@ __device__ __forceinline__ void add_places(const LookupArgs &a, const LookupPlac
   constexpr int N = kUnitOf<T>;
   const int me = static_cast<int>(threadIdx.x) % LANES;
   for (uint32_t base = from; base < to; base += LANES) {
-    const int count = static_cast<int>(to - base < LANES ? to - base : LANES);
+    int count = static_cast<int>(to - base < LANES ? to - base : LANES);
     uint32_t n_mine = a.map[base + (me < count ? me : 0)];
-    const bool there = !check || row_of(a.tokens[n_mine], a.vocab) >= 0;
+    if (check) count = rows_first<LANES>(a, count, n_mine);
     const float scale_mine = a.scale ? a.factor * load_scalar(a.scale, a.scale_dtype, n_mine) : a.factor;
     auto together = [&](auto ahead, int j) {
       constexpr int A = decltype(ahead)::value;
       words_t v[A][UNITS];
       uint32_t n[A];
       float scale[A];
-      bool use[A];
 #pragma unroll
       for (int r = 0; r < A; ++r) {
         const int lane = j + r < count ? j + r : j;  // (a row that is there stands in for one behind the last)
         n[r] = static_cast<uint32_t>(of_lane<LANES>(static_cast<int>(n_mine), lane));
         scale[r] = of_lane<LANES>(scale_mine, lane);
-        use[r] = j + r < count && (!check || of_lane<LANES>(static_cast<int>(there), lane) != 0);
         const S *const in = static_cast<const S *>(a.dout) + n[r] * a.dout_stride;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) v[r][u] = at.load(in, u);
       }
 #pragma unroll
       for (int r = 0; r < A; ++r) {
-        if (!use[r]) continue;
+        if (A != AHEAD && j + r >= count) continue;
         float dot = 0.f;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {

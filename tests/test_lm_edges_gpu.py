@@ -1,10 +1,12 @@
 """Layer norm, lookup and distillation where calls, values and captures are out of the ordinary (bounds of tests/lm_reference.py)."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 import flexsae_amd as flex
+from flexsae_amd import _lib
 from tests import lm_reference as ref
 from tests.test_lm_gpu import DEV, DTYPES, NAMES, _check_distill, _check_lookup, _distill_inputs, _gen, _lookup_inputs
 
@@ -153,6 +155,45 @@ def test_the_gradient_of_a_broadcast_scale_is_rounded_once(dtype):
         shares = shares.sum().view(shape) if len(shape) < 2 else shares
         many = n // scale.numel()  # (shares of at most 1 + 2^-8, added up in any order)
         ref.within(scale.grad, shares, ref.rounded(shares, dtype, many * (many + 4) * ref.U), str(shape))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("n,d", [(15, 3), (64, 100), (300, 130), (1000, 40), (700, 1537), (5000, 600)])
+def test_tokens_that_are_no_row_among_those_of_row_zero(n, d, dtype):
+    """They are filed under row 0: in every order, few and many, alone in a stretch of sorted places and beside it; with a row that
+    the gradient is wanted for among them or none."""
+    for kind, (rows, none) in enumerate([(1, 0.5), (3, 0.9), (2, 0.02), (1, 0.99), (5, 1.0)]):
+        tokens, w, scale, dout = _lookup_inputs(n, rows, d, dtype, seed=n + kind, pad=0.0)
+        away = torch.rand(n, generator=_gen(kind)).to(DEV) < none
+        away[n // 2:n // 2 + 100] = True
+        tokens[away] = torch.where(torch.arange(n, device=DEV) % 3 == 0, -1, -1 - rows)[away]
+        dout[away] = math.nan
+        scale[away] = math.inf
+        _check_lookup(tokens, w, scale, dout)
+        _check_lookup(tokens, w, None, dout)
+    with pytest.raises(IndexError, match="token"):
+        flex.check_index_flag()
+
+
+def test_rows_of_the_gradient_behind_the_last_token_are_not_needed():
+    """A padded batch whose upstream gradient ends with its tokens, by the library's entry point, which promises not to read rows of
+    tokens that are none."""
+    n, there, d = 1000, 421, 256
+    tokens, w, scale, dout = _lookup_inputs(n, 7, d, torch.float32, seed=3, pad=0.1)
+    tokens[there:] = -1
+    short = dout[:there].clone()
+    dweight, dscale = torch.full_like(w, 7.0), torch.full_like(scale, 7.0)
+    lib = _lib.load()
+    lookup = ctypes.byref(_lib.Lookup(n, 7, d, d, d, 1.0, _lib.F32, _lib.F32))
+    nbytes = lib.flexsae_lookup_bwd_workspace_bytes(lookup)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+    at = lambda t: ctypes.c_void_p(t.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.flexsae_lookup_bwd(lookup, at(tokens), at(w), at(scale), at(short), at(dweight), at(dscale), at(workspace), nbytes,
+                                  stream) == _lib.OK
+    want, tol = ref.lookup(tokens, w, scale, 1.0, dout)
+    ref.within(dweight, want["dw"], ref.rounded(want["dw"], torch.float32, tol["dw"]), "dw")
+    ref.within(dscale, want["ds"], ref.rounded(want["ds"], torch.float32, tol["ds"]), "ds")
 
 
 # ---- the flag ------------------------------------------------------------------------------
