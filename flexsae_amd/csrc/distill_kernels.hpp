@@ -42,7 +42,7 @@ struct DistillArgs {
   void *dlogits;
   int *flag;
   int64_t rows, vocab, k, stride, part;  // part: columns of a part of a row, whole units
-  int splits;
+  int splits, slots;  // slots: of the table of stored entries
   float inv_t, t;
   int top_dtype;
   bool by_row;       // losses of rows, not their mean
@@ -230,31 +230,92 @@ __global__ __launch_bounds__(1024) void distill_mean_kernel(const DistillArgs a)
   a.loss[0] = static_cast<float>(s * static_cast<double>(mean_factor(a)));
 }
 
-// The entries of a part of a row that the teacher has stored: gradients in the place of those that `dlogits` holds without the
-// teacher.  Run by the whole block, behind a barrier.  An entry that is stored twice is written by the first of its places.
-template <typename T, int THREADS>
-__device__ __forceinline__ void stored_entries(const DistillArgs &a, int64_t row, int64_t from, int64_t end, float4 st, const RowExp &e, float coef) {
-  using S = elem_t<T>;
-  const S *const in = static_cast<const S *>(a.logits) + row * a.stride;
-  S *const out = static_cast<S *>(a.dlogits) + row * a.vocab;
-  const int64_t *const index = a.index + row * a.k;
-  const float c = kLog2e * a.inv_t;
-  for (int64_t k = threadIdx.x; k < a.k; k += THREADS) {
-    const int64_t i = index[k];
-    if (i < from || i >= end) continue;
-    float p = 0.f;
-    bool first = true;
-    for (int64_t j = 0; j < a.k && first; ++j) {
-      if (index[j] != i) continue;
-      first = j >= k;
-      p += exp_of(load_scalar(a.top, a.top_dtype, row * a.k + j) - st.z, c);
-    }
-    if (first) out[i] = Traits<T>::down(coef / st.y * e.of(Traits<T>::up(in[i])) - coef * (p * st.w));
+// For sums of probabilities that no order changes: p 2^up as a whole number.
+__device__ __forceinline__ int exponent_of(float p) { return __builtin_amdgcn_frexp_expf(p); }
+__device__ __forceinline__ int64_t scaled(float p, int up) { return static_cast<int64_t>(ldexpf(p, up)); }
+
+// The entries of a part of a row that the teacher has stored, each once, with the sum of their places' probabilities, in a table in the
+// LDS.  A place finds its entry's slot by a hash where the table has twice as many as there are places; else a slot is an entry, of as many
+// entries at a time, and the places are read again for the next ones.  A search of each place among all the others would grow with the
+// square of their number (us of a backward, 1000 x 32000 fp16, with it and now: 64 places 61 and 48, 256 179 and 50, 1000 2009 and 68;
+// 32000 are 2300).  The sums are those of whole numbers, as many bits of the entry's largest as leave room for all places.
+constexpr int64_t kStoredMost = 2048;  // places that a hash finds the slots of
+constexpr int kStoredBytes = 16;       // of a slot
+
+// U: of the teacher's logits.  (A type that is known at run time alone is a branch in loops that lanes leave one after another; the
+// compiler kept its condition as a mask of the lanes that were left in one of them, and used it for all lanes in the next.)
+template <typename U, int THREADS>
+struct StoredEntries {
+  int *key;         // the entry, or -1
+  uint32_t *most;   // bits of the largest
+  uint64_t *sum;
+  int slots;        // a power of two
+  int bits;
+  __device__ __forceinline__ StoredEntries(void *lds, int slots, int64_t k)
+      : key(reinterpret_cast<int *>(static_cast<uint64_t *>(lds) + slots)), most(reinterpret_cast<uint32_t *>(key + slots)),
+        sum(static_cast<uint64_t *>(lds)), slots(slots) {
+    const int rest = 31 + __builtin_clz(static_cast<unsigned>(k));  // (fewer than 2^(63 - rest) places)
+    bits = rest < 52 ? rest : 52;
   }
-}
+  __device__ __forceinline__ int slot_of(int entry, bool hashed, int64_t from) const {
+    if (!hashed) {
+      const int slot = static_cast<int>(entry - from);
+      key[slot] = entry;  // (every place writes the same)
+      return slot;
+    }
+    uint32_t slot = static_cast<uint32_t>(entry) * 2654435761u >> 16;
+    for (;; ++slot) {  // (ends: half of the slots stay free)
+      slot &= static_cast<uint32_t>(slots) - 1u;
+      const int there = atomicCAS(&key[slot], -1, entry);
+      if (there == -1 || there == entry) return static_cast<int>(slot);
+    }
+  }
+  // f(entry, probability) for the places of a row whose entries are in [from, end), but for those without a share (of a teacher that
+  // has any to give)
+  template <typename F>
+  __device__ __forceinline__ void places(const DistillArgs &a, int64_t row, int64_t from, int64_t end, float top, F f) const {
+    constexpr int kAhead = 4;
+    const int64_t *const index = a.index + row * a.k;
+    const auto *const logit = static_cast<const elem_t<U> *>(a.top) + row * a.k;
+    const float c = kLog2e * a.inv_t;
+    for (int64_t k = threadIdx.x; k < a.k; k += kAhead * THREADS) {
+      int64_t i[kAhead];
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) i[r] = k + r * THREADS < a.k ? index[k + r * THREADS] : -1;
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) {
+        if (i[r] < from || i[r] >= end) continue;
+        const float p = exp_of(Traits<U>::up(logit[k + r * THREADS]) - top, c);
+        if (p != 0.f || top == INFINITY) f(static_cast<int>(i[r]), p);
+      }
+    }
+  }
+  // By the whole block, behind a barrier where the table was in use.
+  __device__ __forceinline__ void gather(const DistillArgs &a, int64_t row, int64_t from, int64_t end, float top, bool hashed) const {
+    for (int s = threadIdx.x; s < slots; s += THREADS) {
+      key[s] = -1;
+      most[s] = 0u;
+      sum[s] = 0u;
+    }
+    __syncthreads();
+    places(a, row, from, end, top, [&](int entry, float p) { atomicMax(&most[slot_of(entry, hashed, from)], __float_as_uint(p)); });
+    __syncthreads();
+    places(a, row, from, end, top, [&](int entry, float p) {
+      const int slot = slot_of(entry, hashed, from);
+      atomicAdd(reinterpret_cast<unsigned long long *>(&sum[slot]), static_cast<unsigned long long>(scaled(p, up(slot))));
+    });
+  }
+  // f(entry, probability) for the slots in use, behind a barrier.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int s = threadIdx.x; s < slots; s += THREADS)
+      if (key[s] >= 0) f(key[s], ldexpf(static_cast<float>(sum[s]), -up(s)));
+  }
+  __device__ __forceinline__ int up(int slot) const { return bits - exponent_of(__uint_as_float(most[slot])); }
+};
 
 // Gradient of a part of a row: block = row * splits + part.
-template <typename T>
+template <typename T, typename U>
 __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const DistillArgs a) {
   using S = elem_t<T>;
   constexpr int N = kUnitOf<T>;
@@ -273,6 +334,10 @@ __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const Dis
       store_upto<T>(out + at, words_t(0u), end - at);
     return;
   }
+  extern __shared__ __align__(16) uint64_t table[];
+  const StoredEntries<U, kDistillThreads> stored(table, a.slots, a.k);
+  const bool hashed = a.k <= kStoredMost;
+  if (hashed) stored.gather(a, row, from, end, st.z, true);
   const RowExp e(st.x, a.inv_t);
   const float each = coef / st.y;
   walk<T, kDistillThreads, false>(in, from, end, [&](int64_t at, float (&x)[N], int64_t left) {
@@ -280,13 +345,20 @@ __global__ __launch_bounds__(kDistillThreads) void distill_grad_kernel(const Dis
     for (int i = 0; i < N; ++i) x[i] = each * e.of(x[i]);
     store_upto<T>(out + at, pack<T>(x), left);
   });
-  __syncthreads();
-  stored_entries<T, kDistillThreads>(a, row, from, end, st, e, coef);
+  // in the places of gradients without the teacher, which are there behind a barrier
+  const auto put = [&](int i, float p) { out[i] = Traits<T>::down(each * e.of(Traits<T>::up(in[i])) - coef * (p * st.w)); };
+  if (hashed) {
+    __syncthreads();
+    stored.each(put);
+    return;
+  }
+  for (int64_t first = from; first < end; first += a.slots) {
+    __syncthreads();
+    stored.gather(a, row, first, first + a.slots < end ? first + a.slots : end, st.z, false);
+    __syncthreads();
+    stored.each(put);
+  }
 }
-
-// For sums of probabilities that no order changes: p 2^up as a whole number, of p below 2^(52 - up); 2^11 of them fit.
-__device__ __forceinline__ int exponent_of(float p) { return __builtin_amdgcn_frexp_expf(p); }
-__device__ __forceinline__ int64_t scaled(float p, int up) { return static_cast<int64_t>(ldexpf(p, up)); }
 
 // ---- a row in the registers of one block ------------------------------------------------------
 

@@ -418,6 +418,13 @@ int check_tensors(const flexsae_distill *d, const void *logits, const void *top,
   return FLEXSAE_OK;
 }
 
+// Slots of a block's table of stored entries: twice the places, to a power of two, up to what leaves two blocks a compute unit.
+int distill_slots(int64_t k) {
+  int slots = 64;
+  while (slots < 2 * kStoredMost && slots < 2 * k) slots *= 2;
+  return slots;
+}
+
 DistillArgs distill_args(const flexsae_distill &d, const void *logits, const void *top, const int64_t *index, const float *row_weights,
                          float *stats) {
   const DistillSplit split = distill_split(d);
@@ -433,6 +440,7 @@ DistillArgs distill_args(const flexsae_distill &d, const void *logits, const voi
   a.stride = d.logits_stride;
   a.part = split.part;
   a.splits = split.splits;
+  a.slots = distill_slots(d.k);
   a.t = d.temperature;
   a.inv_t = 1.f / d.temperature;
   a.top_dtype = d.top_dtype;
@@ -461,13 +469,16 @@ DistillHeld distill_held(int64_t vocab, int64_t k) {
   return {};
 }
 template <typename T>
-DistillKernels distill_kernels(int64_t vocab, int64_t k) {
-  return {distill_parts_kernel<T>, distill_rows_kernel<T>, distill_grad_kernel<T>, distill_held<T>(vocab, k)};
+DistillKernels distill_kernels_of(const flexsae_distill &d) {
+  const DistillKernel grad = d.top_dtype == FLEXSAE_F32    ? distill_grad_kernel<T, float>
+                             : d.top_dtype == FLEXSAE_BF16 ? distill_grad_kernel<T, bf16_t>
+                                                           : distill_grad_kernel<T, f16_t>;
+  return {distill_parts_kernel<T>, distill_rows_kernel<T>, grad, distill_held<T>(d.vocab, d.k)};
 }
 DistillKernels distill_kernels(const flexsae_distill &d) {
-  return d.dtype == FLEXSAE_F32    ? distill_kernels<float>(d.vocab, d.k)
-         : d.dtype == FLEXSAE_BF16 ? distill_kernels<bf16_t>(d.vocab, d.k)
-                                   : distill_kernels<f16_t>(d.vocab, d.k);
+  return d.dtype == FLEXSAE_F32    ? distill_kernels_of<float>(d)
+         : d.dtype == FLEXSAE_BF16 ? distill_kernels_of<bf16_t>(d)
+                                   : distill_kernels_of<f16_t>(d);
 }
 
 }  // namespace
@@ -514,7 +525,7 @@ int flexsae_distill_fwd(const flexsae_distill *d, const void *logits, const void
   k.rows<<<grid_of(ceil_div(a.rows, kDistillThreads / kWave)), kDistillThreads, 0, s>>>(a);
   if (const int rc = launch_status()) return rc;
   if (dlogits) {
-    k.grad<<<grid_of(a.rows * a.splits), kDistillThreads, 0, s>>>(a);
+    k.grad<<<grid_of(a.rows * a.splits), kDistillThreads, a.slots * kStoredBytes, s>>>(a);
     if (const int rc = launch_status()) return rc;
   }
   return finish();
@@ -531,7 +542,7 @@ int flexsae_distill_bwd(const flexsae_distill *d, const void *logits, const void
   a.grad = grad;
   a.dlogits = dlogits;
   a.skip_if_one = skip_if_one != 0;
-  distill_kernels(*d).grad<<<grid_of(a.rows * a.splits), kDistillThreads, 0, as_stream(stream)>>>(a);
+  distill_kernels(*d).grad<<<grid_of(a.rows * a.splits), kDistillThreads, a.slots * kStoredBytes, as_stream(stream)>>>(a);
   return launch_status();
 }
 

@@ -114,6 +114,21 @@ def test_a_teacher_without_a_distribution(lost, by_row, dtype):
         assert loss[[2, 7]].isnan().all() if by_row else loss.isnan()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("n,v,k", [(3, 9001, 1024), (3, 9001, 2048), (3, 9001, 2049), (520, 6001, 2500), (9, 30000, 30000), (2, 300, 5000)])
+def test_many_stored_entries(n, v, k, dtype):
+    """Up to the whole vocabulary and beyond it: all different, some more than once, all the same."""
+    for top_dtype in DTYPES:
+        z, top, index = _distill_inputs(n, v, k, dtype, seed=k, top_dtype=top_dtype)
+        index[0] = torch.arange(k, device=DEV) % v
+        index[1] = torch.where(torch.rand(k, generator=_gen(n + k)).to(DEV) < 0.5, v - 1, index[1])
+        index[-1, k // 3:] = -1
+        scale = 1.0 if dtype != torch.float16 else 4096.0
+        first = _check_distill(z, top, index, grad=0.5 * scale)  # (not the gradient that is made along with the loss)
+        assert all(torch.equal(a, b) for a, b in zip(first, _check_distill(z, top, index, grad=0.5 * scale)))
+        _check_distill(z, top, index, by_row=True, grad=torch.full((n,), scale))
+
+
 @pytest.mark.parametrize("size", [2.0 ** -140, 2.0 ** -130, 2.0 ** 118, 2.0 ** 126])
 def test_row_weights_of_any_size(size):
     """Of a mean only the ratios of the weights count, also where their sum, or one over it, is beyond the normal numbers of fp32."""
