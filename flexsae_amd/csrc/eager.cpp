@@ -410,7 +410,10 @@ struct SlicedLoss : torch::autograd::Function<SlicedLoss> {
     ctx->save_for_backward({indices, weight, vals, bias, target, r.dvals, r.dbias});
     ctx->set_materialize_grads(false);
     // the unit gradient is no saved tensor: the backward scales it in place and hands the very buffer on
-    if (plan.need_dw) ctx->saved_data["dW"] = r.dW;
+    if (plan.need_dw) {
+      ctx->saved_data["dW"] = r.dW;
+      ctx->saved_data["capture"] = capture_of(weight);
+    }
     save_plan(ctx, plan);
     return r.loss;
   }
@@ -420,21 +423,23 @@ struct SlicedLoss : torch::autograd::Function<SlicedLoss> {
     const Tensor &grad = grads[0];
     if (!grad.defined()) return variable_list(6);
     const auto at = ctx->saved_data.find("dW");
-    Tensor dW = at != ctx->saved_data.end() ? at->second.toTensor() : Tensor();
+    // (not one of another graph, or of none, which every replay would scale again, or the forward's write anew; it stays for a
+    // backward that is of the forward's)
+    const bool mine = at != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_of(at->second.toTensor());
+    Tensor dW = mine ? at->second.toTensor() : Tensor();
     const StepPlan plan = saved_plan(ctx);
     if (!plain_backward(grad) || (lists_in_python && !dW.defined()) || !usable_inputs(saved) ||
         !usable_fp32(saved[5], saved[1], saved[2].sizes()) || !usable_fp32(saved[6], saved[1], saved[3].sizes()) ||
         (dW.defined() && dW.device() != saved[1].device())) {
       auto out = backward_in_python(ctx, kSliced, grad, saved, {plan.need_dw, plan.flags}, &dW, 6);
-      if (dW.defined()) ctx->saved_data["dW"] = dW;
-      else ctx->saved_data.erase("dW");
+      if (mine && !dW.defined()) ctx->saved_data.erase("dW");
       return out;
     }
     Tensor dvals = prepared(saved[5]), dbias = prepared(saved[6]);
     if (ctx->needs_input_grad(1)) {
       TORCH_CHECK(plan.need_dw, "the step ran without dW but weight requires a gradient");
-      ctx->saved_data.erase("dW");  // the buffer now belongs to whoever receives the gradient
-      if (!dW.defined()) {          // a second backward through a retained graph: the buffer went with the first one
+      if (mine) ctx->saved_data.erase("dW");  // the buffer now belongs to whoever receives the gradient
+      if (!dW.defined()) {                    // a second backward through a retained graph: the buffer went with the first one
         Step again = hier_step({saved[0], saved[1], saved[2], saved[3], saved[4]}, plan);
         dW = again.dW;
         dvals = again.dvals;

@@ -1133,8 +1133,15 @@ def _train_sliced_setup_context(ctx, inputs, output):
     if ctx.dw_in_place:
         ctx.save_for_backward(indices, weight, vals, bias, target, dvals, dbias)
         ctx.dw_unit = dW if ctx.needs_input_grad[1] else None
+        ctx.captured = torch.cuda.is_current_stream_capturing()
     else:
         ctx.save_for_backward(indices, weight, vals, bias, target, dvals, dbias, dW)
+
+
+def _own_unit_gradient(ctx):
+    """The unit gradient that the forward has left, None where it is gone, or where one of forward and backward is captured and the
+    other is not: every replay would scale it again, or write it anew under whoever has received it."""
+    return ctx.dw_unit if ctx.captured == torch.cuda.is_current_stream_capturing() else None
 
 
 def _train_sliced_backward(ctx, grad_loss, grad_dvals, grad_dbias, grad_dw):
@@ -1153,10 +1160,10 @@ def _train_sliced_backward(ctx, grad_loss, grad_dvals, grad_dbias, grad_dw):
         indices, weight, vals, bias, target, dvals, dbias = ctx.saved_tensors
         dW = None
         if ctx.needs_input_grad[1]:
-            dW = ctx.dw_unit
+            dW = _own_unit_gradient(ctx)
             # Several upstream gradients at once, or a graph of the backward, get gradients of their own: the buffer stays.
             own = torch.is_grad_enabled() or _is_batched(g)
-            if not own:
+            if not own and dW is not None:
                 ctx.dw_unit = None  # the buffer now belongs to whoever receives the gradient
             if dW is None:
                 # a second backward through a retained graph: the buffer went with the first one
@@ -1323,6 +1330,7 @@ class _HierTrainSliced(torch.autograd.Function):
         ctx.dw_in_place = True
         ctx.save_for_backward(indices, weight, vals, bias, target, dvals, dbias)
         ctx.dw_unit = dW if ctx.needs_input_grad[1] else None
+        ctx.captured = torch.cuda.is_current_stream_capturing()
         return loss
 
     @staticmethod
@@ -1332,9 +1340,10 @@ class _HierTrainSliced(torch.autograd.Function):
         indices, weight, vals, bias, target, dvals, dbias = ctx.saved_tensors
         dW = None
         if ctx.needs_input_grad[1]:
-            dW = ctx.dw_unit
-            ctx.dw_unit = None  # the buffer now belongs to whoever receives the gradient
-            if dW is None:  # a second backward through a retained graph: the buffer went with the first one
+            dW = _own_unit_gradient(ctx)
+            if dW is not None:
+                ctx.dw_unit = None  # the buffer now belongs to whoever receives the gradient
+            else:  # a second backward through a retained graph: the buffer went with the first one
                 _, dvals, dbias, dW = _hier_train_sliced_impl(indices, weight, vals, bias, target, True, ctx.hot, ctx.dense)
         dW, dvals, dbias = _finish_grads(grad_loss, weight, dW, dvals, ctx.leaf_dtypes[0], dbias, ctx.leaf_dtypes[1])
         return None, dW, dvals, dbias, None, None, None, None
@@ -1408,6 +1417,7 @@ def _general_backward(kind, grad, saved, needs, numbers, dw_unit):
         return tuple(_HierLateStep.backward(ctx, grad)[:5]), None
     ctx.leaf_dtypes = (saved[2].dtype, saved[3].dtype)
     ctx.need_dw, ctx.dw_in_place, ctx.dw_unit = bool(numbers[0]), True, dw_unit
+    ctx.captured = torch.cuda.is_current_stream_capturing()  # (the unit gradient is given where it may be taken)
     ctx.hot, ctx.dense = bool(numbers[1] & _lib.BWD_HOT_LATENTS), bool(numbers[1] & _lib.BWD_DENSE_LATENTS)
     grads = _HierTrainSliced.backward(ctx, grad) if plain else _train_sliced_backward(ctx, grad, None, None, None)
     return tuple(grads[:5]), ctx.dw_unit

@@ -1,0 +1,55 @@
+"""A hierarchical step whose forward runs before a graph is captured and whose backward is captured: every replay makes the gradients
+for the upstream gradient of its time."""
+import pytest
+import torch
+
+import flexsae_amd as flex
+from flexsae_amd import ops
+from tests.helpers import make_inputs
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def _by_op(idx, W, v, b, t):
+    return ops.hier_train_sliced(idx, W, v, b, t, True, False, False)[0]
+
+
+def _by_functions(idx, W, v, b, t):
+    return ops._HierTrainSliced.apply(idx, W, v, b, t, True, False, False)
+
+
+@pytest.mark.parametrize("fn", [flex.triton_hierarchical_sae_loss, _by_functions, _by_op], ids=["eager", "functions", "op"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_a_captured_backward_of_an_eager_step(fn, dtype, monkeypatch):
+    monkeypatch.setattr(ops, "_late_step", lambda *_: False)
+    idx, W, v, b, t = (x.to(DEV) for x in make_inputs(40, 16, 411, 256, dtype, seed=6))
+    leaves = [x.clone().requires_grad_() for x in (W, v, b)]
+    up = torch.tensor(2.0, device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = {}
+        for value in (2.0, 0.5, 1.0):
+            up.fill_(value)
+            want[value] = torch.autograd.grad(fn(idx, *leaves, t), leaves, up)
+        loss = fn(idx, *leaves, t)
+        torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = torch.autograd.grad(loss, leaves, up, retain_graph=True)
+    for value in (2.0, 2.0, 0.5, 1.0, 2.0):
+        up.fill_(value)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(got, want[value]):
+            assert torch.equal(a, c), value
+    del graph
+    # an eager backward of the same step, whose gradients no replay changes
+    up.fill_(0.5)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        left = torch.autograd.grad(loss, leaves, up)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(left, want[0.5]))

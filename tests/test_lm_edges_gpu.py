@@ -34,7 +34,7 @@ def test_a_captured_backward_of_an_eager_forward(dtype):
         g = torch.ones((), device=DEV)
         torch.autograd.grad(flex.distillation_loss(leaf, top, index), leaf, g)
         loss = flex.distillation_loss(leaf, top, index)
-    graph, (dz,) = _captured(stream, lambda: torch.autograd.grad(loss, leaf, g))
+    graph, (dz,) = _captured(stream, lambda: torch.autograd.grad(loss, leaf, g, retain_graph=True))
     for value in (1.0, 64.0, 1.0, 0.5, 1.0, 1.0):
         g.fill_(value)
         torch.cuda.synchronize()
