@@ -273,6 +273,8 @@ __global__ void csr_fill_kernel(const int64_t *__restrict__ indices, int64_t n_p
   }
 }
 
+constexpr int64_t kSortGridRow = int64_t{1} << 22;  // blocks of a row of the sort's grid
+
 // Sort every group ascending so that the list does not depend on the order in which the
 // count kernel's atomics happened to be served.  One wavefront per latent: groups of up to
 // 64 pairs are rank-sorted in registers (pair ids are distinct); longer ones are appended
@@ -282,7 +284,8 @@ __global__ __launch_bounds__(256) void csr_sort_short_kernel(const uint32_t *__r
                                                              uint32_t *__restrict__ long_count,
                                                              uint32_t *__restrict__ long_list) {
   const int lane = lane_id();
-  const int64_t f = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 6) + wave_in_block();
+  // (threads of a grid are counted in 32 bits along an axis: 2^26 latents and more take further rows of it)
+  const int64_t f = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * (blockDim.x >> 6) + wave_in_block();
   if (f >= F) return;
   const uint32_t s0 = begin[f];
   const uint32_t n = begin[f + 1] - s0;

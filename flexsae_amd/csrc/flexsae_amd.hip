@@ -591,8 +591,9 @@ void csr_build_launch(const int64_t *indices, int64_t B, int64_t K, int64_t F, u
                      sc.block_sums);
   hipLaunchKernelGGL(csr_fill_kernel, dim3(grid_for(n_pairs, 256, 8192)), dim3(256), 0, st, indices,
                      n_pairs, F, begin, sc.rank, map);
+  const int64_t sort_blocks = ceil_div(F, kWavesPerBlock), sort_row = sort_blocks < kSortGridRow ? sort_blocks : kSortGridRow;
   hipLaunchKernelGGL(csr_sort_short_kernel,
-                     dim3(static_cast<unsigned>(ceil_div(F, kWavesPerBlock))), dim3(kBlock), 0, st,
+                     dim3(static_cast<unsigned>(sort_row), static_cast<unsigned>(ceil_div(sort_blocks, sort_row))), dim3(kBlock), 0, st,
                      begin, map, F, sc.lists.ctrl + kLongCount, sc.lists.long_list);
   hipLaunchKernelGGL(csr_sort_long_kernel, dim3(1024), dim3(1024), 0, st, begin, map, sc.lists.ctrl + kLongCount,
                      sc.lists.long_list, static_cast<uint32_t>(B < (1LL << 31) ? B : 0xffffffffLL),

@@ -222,3 +222,22 @@ def test_the_flag_names_all_that_was_out_of_range():
     with pytest.raises(IndexError, match=r"(?s)`indices`.*token"):
         flex.check_index_flag()
     flex.check_index_flag()
+
+
+# ---- long tables ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("v", [(1 << 26) - 3, (1 << 26) + 5, (1 << 27) + 11])
+def test_the_same_bits_for_long_tables(v):
+    """A table's gradient by sorted tokens at its end, where the lists of rows are more than a grid has threads along an axis."""
+    n, d = 200_000, 2
+    g = torch.Generator(DEV).manual_seed(1)
+    w = torch.zeros(v, d, device=DEV, requires_grad=True)
+    low = torch.randint(0, 4000, (n,), generator=g, device=DEV)
+    dout = torch.randn(n, d, generator=g, device=DEV)
+    out = flex.embedding_lookup(low + (v - 4000), w)
+    runs = [torch.autograd.grad(out, w, dout, retain_graph=True)[0] for _ in range(3)]
+    assert all(torch.equal(runs[0], r) for r in runs[1:])
+    few = torch.zeros(4000, d, device=DEV, requires_grad=True)
+    want, = torch.autograd.grad(flex.embedding_lookup(low, few), few, dout)
+    assert torch.equal(runs[0][-4000:], want) and not runs[0][:-4000].any()
