@@ -90,7 +90,7 @@ def _check_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps
             raise ValueError(f"layer_norm: {name} is {tuple(t.shape)}, rows have {x.shape[-1]} columns")
     if x.shape[-1] >= 2 ** 27 or x.numel() // x.shape[-1] >= 2 ** 32:
         raise ValueError("sizes beyond the kernels' index range: need fewer than 2^32 rows of fewer than 2^27 columns")
-    if not (eps >= 0 and math.isfinite(eps)):
+    if not 0 <= eps < math.inf:
         raise ValueError(f"layer_norm: eps must be finite and not negative, got {eps}")
     _on_one_gpu(("x", x), ("weight", weight), ("bias", bias))
 
@@ -223,7 +223,7 @@ def _check_lookup(tokens: Tensor, weight: Tensor, scale: Optional[Tensor], facto
         _float("scale", scale)
         if scale.shape != tokens.shape:
             raise ValueError(f"embedding_lookup: scale is {tuple(scale.shape)}, tokens {tuple(tokens.shape)}")
-    if not math.isfinite(factor):
+    if not -math.inf < factor < math.inf:
         raise ValueError(f"embedding_lookup: scale must be finite, got {factor}")
     _on_one_gpu(("weight", weight), ("tokens", tokens), ("scale", scale))
 
@@ -345,7 +345,7 @@ def _check_distill(logits: Tensor, top: Tensor, index: Tensor, row_weights: Opti
     if row_weights is not None and (row_weights.shape != logits.shape[:-1] or row_weights.dtype != torch.float32):
         raise ValueError(f"distillation_loss: row_weights is {row_weights.dtype} {tuple(row_weights.shape)}, rows "
                          f"{tuple(logits.shape[:-1])}")
-    if not (temperature > 0 and math.isfinite(temperature)):
+    if not 0 < temperature < math.inf:
         raise ValueError(f"distillation_loss: temperature must be positive and finite, got {temperature}")
     if not 1e-18 < temperature < 1e18:
         raise ValueError(f"distillation_loss: temperature must be within 1e-18 and 1e18, got {temperature}")

@@ -241,3 +241,26 @@ def test_the_same_bits_for_long_tables(v):
     few = torch.zeros(4000, d, device=DEV, requires_grad=True)
     want, = torch.autograd.grad(flex.embedding_lookup(low, few), few, dout)
     assert torch.equal(runs[0][-4000:], want) and not runs[0][:-4000].any()
+
+
+# ---- compiled calls ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dynamic", [True, None])
+def test_compiled_calls_of_changing_sizes_and_numbers(dynamic):
+    def chain(x, w, tokens, table, scale, top, index, out, temperature, eps):
+        z = flex.layer_norm(x + flex.embedding_lookup(tokens, table, scale), w, eps=eps) @ out
+        return flex.distillation_loss(z, top, index, row_weights=tokens >= 0, temperature=temperature) + flex.distillation_loss(z, top, index)
+
+    compiled = torch.compile(chain, backend="aot_eager", fullgraph=True, dynamic=dynamic)
+    g = _gen(60)
+    for n, scale, temperature, eps in ((7, 1.5, 1.0, 1e-5), (12, 0.5, 2.0, 1e-6), (33, 3, 0.7, 1e-3), (33, 2, 3, 1e-4)):
+        x, w, table, out, top = (torch.randn(s, generator=g).to(DEV) for s in ((n, 64), (64,), (9, 64), (64, 70), (n, 4)))
+        tokens, index = torch.randint(-1, 9, (n,), generator=g).to(DEV), torch.randint(0, 70, (n, 4), generator=g).to(DEV)
+        leaves = [t.requires_grad_() for t in (x, w, table, out)]
+        results = []
+        for fn in (chain, compiled):
+            loss = fn(x, w, tokens, table, scale, top, index, out, temperature, eps)
+            results.append([loss, *torch.autograd.grad(loss, leaves)])
+        for a, b in zip(*results):  # (the ops take gradients of a mean from other partial sums: rounding errors of sums of 70 terms)
+            assert (a - b).norm() <= 200 * ref.U * a.norm()
