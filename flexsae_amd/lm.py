@@ -22,6 +22,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from .ops import _DTYPES, _flag_for, _native, _on_device, _ptr, _stream
@@ -49,6 +50,14 @@ def _indices(name: str, t: Tensor) -> Tensor:
     if t.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{name} must be int64 or int32, got {t.dtype}")
     return t.to(torch.int64)
+
+
+def _no_tangents(*tensors: Optional[Tensor]) -> None:
+    """The ops have no forward-mode derivatives, and torch would leave them out without a word."""
+    if torch.compiler.is_compiling() or forward_ad._current_level < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("flexsae_amd's operators have no forward-mode derivatives")
 
 
 def _there(t: Tensor) -> Tensor:
@@ -190,6 +199,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
         y = native.layer_norm(x, weight, bias, eps, 0)
         if y is not None:
             return y
+    _no_tangents(x, weight, bias)
     _check_norm(x, weight, bias, float(eps))
     return _norm_fwd_op(x, weight, bias, float(eps))[0]
 
@@ -203,6 +213,7 @@ def layer_norm_stats(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[
         out = native.layer_norm(x, weight, bias, eps, 1)
         if out is not None:
             return out
+    _no_tangents(x, weight, bias)
     _check_norm(x, weight, bias, float(eps))
     y, mean, rstd = _norm_fwd_op(x, weight, bias, float(eps))
     return y, mean.detach(), rstd.detach()
@@ -325,6 +336,7 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: Union[None, float, T
         out = native.embedding_lookup(tokens, weight, scale, factor)
         if out is not None:
             return out
+    _no_tangents(weight, scale)
     _check_lookup(tokens, weight, scale, factor)
     return _lookup_fwd_op(tokens, weight, scale, factor)
 
@@ -463,5 +475,6 @@ def distillation_loss(logits: Tensor, top_logits: Tensor, top_indices: Tensor, *
         loss = native.distillation_loss(logits, top_logits, top_indices, row_weights, temperature, int(by_row))
         if loss is not None:
             return loss
+    _no_tangents(logits)
     _check_distill(logits, top_logits, top_indices, row_weights, float(temperature))
     return _distill_fwd_op(logits, top_logits.detach(), top_indices, row_weights, float(temperature), by_row)[0]

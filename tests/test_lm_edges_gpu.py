@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flexsae_amd as flex
 from flexsae_amd import _lib
@@ -264,3 +265,15 @@ def test_compiled_calls_of_changing_sizes_and_numbers(dynamic):
             results.append([loss, *torch.autograd.grad(loss, leaves)])
         for a, b in zip(*results):  # (the ops take gradients of a mean from other partial sums: rounding errors of sums of 70 terms)
             assert (a - b).norm() <= 200 * ref.U * a.norm()
+
+
+def test_forward_mode_is_refused():
+    x, tokens = torch.randn(6, 40, device=DEV), torch.randint(0, 6, (5,), device=DEV)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda t: flex.layer_norm(t), lambda t: flex.layer_norm(x, t[0]), lambda t: flex.layer_norm_stats(t),
+                     lambda t: flex.embedding_lookup(tokens, t), lambda t: flex.embedding_lookup(tokens, x, t[0, :5]),
+                     lambda t: flex.distillation_loss(t, x[:, :3], tokens.new_zeros(6, 3))):
+            call(x)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
