@@ -5,15 +5,16 @@
 //   L = T^2 a sum over k of p[k] (log p[k] - log q[i[k]]),   dL / dz[v] = T a (q[v] - sum over k with i[k] = v of p[k])
 //
 // with a the row's weight, divided by the sum of all where the mean is taken.  A place with an index that is negative or beyond the
-// vocabulary holds no logit.  A row of weight zero, or without a stored logit above minus infinity, is not read: it counts as zero
-// and has a gradient of zeros.
+// vocabulary holds no logit.  A row of weight zero, or without a stored logit above minus infinity, counts as zero and has a gradient of
+// zeros, whatever its logits are.
 //
 // Three ways.  With the gradient of a mean a row is read once, into the registers of one block (distill_held_kernel): maximum, sum
 // and gradient from there.  8192 rows of 131072 bf16: 855 us, 5.0 TB/s of reads and writes where a copy by the library reaches 4.8;
 // statistics and gradient by passes of their own take 1440, and one block a row that reads it twice 1270: a second read comes no
 // faster from the Infinity Cache.  At this size a block fills its compute unit, whose memory rests while it takes the sum.
 // Few long rows, rows that no block holds and losses without a gradient go by parts of rows (121 us for 537 MB), joined by a wavefront a
-// row; and gradients for an upstream gradient that the forward did not know by parts of rows again (46 us for 102 MB read and written).
+// row; and gradients for an upstream gradient that the forward did not know by parts of rows again (38 us for 102 MB read and as much
+// written), which the gradient that was made with the loss comes on top of: 8192 x 131072 bf16 1805 us for 948.
 //
 // The row's statistics are its maximum m and s = sum of exp((z - m) / T), in one pass: a running maximum per lane, sums rescaled
 // when it moves.  Exponents are of differences from the maximum, so that large logits cost no digits.

@@ -8,10 +8,11 @@
 // wavefronts' means and squares joined as those of parts of a sample, so that a large common offset costs no digits and one barrier
 // serves both sums.
 //
-// Memory bounds it: 16384 x 8192 bf16 forward 86 us (6.2 TB/s), 65536 x 2304 forward 130 us (4.7) and backward 184 + 5 us (4.9), where a
-// lane has less of a row to keep on its way.  What that took (us of the last forward): weight and bias once for several rows, whose next
-// one is on its way while a row is worked on, 304 to 194; the wavefronts' sums by one read of the LDS, not one after another, to 158;
-// sixteen elements a lane instead of eight, to 142.
+// Memory bounds it: 16384 x 8192 bf16 forward 86 us (6.2 TB/s), 65536 x 2304 forward 115 us (5.2) and backward 172 us (5.3), each one call
+// after another, where a lane has less of a row to keep on its way.  (A trace of single kernels says 132 and 185 + 5: there each waits for
+// its last stores.)  What that took (us of the last forward, traced): weight and bias once for several rows, whose next one is on its way
+// while a row is worked on, 304 to 194; the wavefronts' sums by one read of the LDS, not one after another, to 158; sixteen elements a
+// lane instead of eight, to 142.
 #pragma once
 
 #include "row_access.hpp"

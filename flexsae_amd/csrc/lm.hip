@@ -79,7 +79,9 @@ NormPlan norm_plan(int64_t cols, bool backward) {
   if (units <= 64 * kEight) return norm_shared<T, 64, kEight>(backward);
   if (units <= 64 * kSixteen) return norm_shared<T, 64, kSixteen>(backward);
   // Sixteen elements a lane leave fewer wavefronts to join (us of the forward, 65536 x 2304 bf16: 158 with eight, 142 with sixteen);
-  // the backward, with the sums of its columns, has the registers for eight while a block's wavefronts hold a row that way.
+  // the backward, with the sums of its columns, has the registers for eight while a block's wavefronts hold a row that way (8192 columns
+  // of 16-bit numbers; 16384 x 8192 bf16 165 us, 4.9 TB/s).  Beyond that it has sixteen too, and spills 8 registers of a lane, 39 of fp32:
+  // 16384 x 12288 bf16 276 us, 4.4 TB/s, 8192 x 16384 206, 3.9; rows that no block holds are read again, 8192 x 16392 326, 2.5.
   if (backward && units <= kNormMostWaves * 64 * kEight) return norm_block<T, kEight>(units, backward);
   if (units <= kNormMostWaves * 64 * kSixteen) return norm_block<T, kSixteen>(units, backward);
   return {backward ? layer_norm_bwd_long_kernel<T> : layer_norm_fwd_long_kernel<T>, 1024, 1, false};
@@ -449,7 +451,9 @@ DistillArgs distill_args(const flexsae_distill &d, const void *logits, const voi
 }
 
 using DistillKernel = void (*)(const DistillArgs);
-// A row in the registers of a block of so many threads: where it fits there, and each of the teacher's places has a thread.
+// A row in the registers of a block of so many threads: where it fits there (131072 entries of 16 bits, 65536 of fp32), and each of the
+// teacher's places has a thread.  Longer rows take passes of their own for statistics and gradient: us of a mean with its gradient,
+// 8192 x 131072 bf16 948, x 131080 1415; 4096 x 65536 fp32 415, x 65544 678.
 struct DistillHeld {
   DistillKernel kernel = nullptr;
   int threads = 0;

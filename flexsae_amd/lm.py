@@ -321,7 +321,8 @@ def embedding_lookup(tokens: Tensor, weight: Tensor, scale: Union[None, float, T
 
     tokens: int64 or int32, any shape.  A token of -1 stands for none (padding): a row of zeros without gradients, whose upstream
     gradient is not looked at.  So does any other outside ``[0, V)``, and is reported by ``check_index_flag``.
-    scale: a number, or a tensor that broadcasts to the tokens' shape (a gate of every token), of a type of its own.
+    scale: a number, or a tensor that broadcasts to the tokens' shape (a gate of every token), of a type of its own; shares of a
+    broadcast scale's gradient are added up in fp32.
     The weight's gradient is dense and written once, summed in fp32 by sorted tokens in a fixed order (the same bits on every
     run)."""
     factor = 1.0
@@ -461,7 +462,8 @@ def distillation_loss(logits: Tensor, top_logits: Tensor, top_indices: Tensor, *
     "none", each row's loss times its weight.
     logits: rows at any distance from each other are read where they are.  Their gradient is rounded once.  With the mean it is
     made along with the loss for an upstream gradient of one, except for float16 logits, and made again by a backward pass with
-    another."""
+    another, which reads and writes the logits' size once more.  One read serves the loss and that gradient for rows of up to 131072
+    logits of 16 bits, or 65536 of fp32, with up to 1024 stored; longer ones are read twice."""
     if reduction not in ("mean", "none"):
         raise ValueError(f"distillation_loss: reduction must be 'mean' or 'none', got {reduction!r}")
     top_indices = _indices("top_indices", top_indices)
