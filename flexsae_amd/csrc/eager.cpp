@@ -215,13 +215,14 @@ std::pair<Tensor, Tensor> forward(bool topk, const Inputs &given) {
 }
 
 // (dW, dvals, dbias), dvals and dbias times grad (undefined: one) in the leaves' types; dW_unit (undefined: none) times it in
-// the weight's, in place where it has that type
+// the weight's, in place where it has that type and is to be
 std::tuple<Tensor, Tensor, Tensor> finish(const Tensor &grad, const Tensor &weight, const Tensor &dW_unit, const Tensor &dvals,
-                                          c10::ScalarType vals_type, const Tensor &dbias, c10::ScalarType bias_type) {
+                                          c10::ScalarType vals_type, const Tensor &dbias, c10::ScalarType bias_type,
+                                          bool in_place = true) {
   const Tensor g = grad.defined() ? grad_scalar(grad, weight.device()) : Tensor();
   Tensor dW;
   if (dW_unit.defined())
-    dW = dW_unit.scalar_type() == weight.scalar_type() ? dW_unit : make(weight, dW_unit.sizes(), weight.scalar_type());
+    dW = in_place && dW_unit.scalar_type() == weight.scalar_type() ? dW_unit : make(weight, dW_unit.sizes(), weight.scalar_type());
   Tensor out_v = make(weight, dvals.sizes(), vals_type), out_b = make(weight, dbias.sizes(), bias_type);
   check(lib.finish_grads(dW.defined() ? dW.data_ptr() : nullptr, dtype_of(weight.scalar_type()),
                          dW.defined() ? dW_unit.data_ptr() : nullptr,
@@ -423,19 +424,22 @@ struct SlicedLoss : torch::autograd::Function<SlicedLoss> {
     const Tensor &grad = grads[0];
     if (!grad.defined()) return variable_list(6);
     const auto at = ctx->saved_data.find("dW");
-    // (not one of another graph, or of none, which every replay would scale again, or the forward's write anew; it stays for a
-    // backward that is of the forward's)
-    const bool mine = at != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_of(at->second.toTensor());
-    Tensor dW = mine ? at->second.toTensor() : Tensor();
+    // That of a graph which this backward is no part of is read alone: its replays write it again.  That of an eager forward is not
+    // for a graph: every replay would scale it again, or read memory that is another's by then.
+    const int64_t from = at != ctx->saved_data.end() ? ctx->saved_data["capture"].toInt() : 0;
+    const bool mine = at != ctx->saved_data.end() && from == capture_of(at->second.toTensor());
+    Tensor dW = mine || from != 0 ? at->second.toTensor() : Tensor();
     const StepPlan plan = saved_plan(ctx);
     if (!plain_backward(grad) || (lists_in_python && !dW.defined()) || !usable_inputs(saved) ||
         !usable_fp32(saved[5], saved[1], saved[2].sizes()) || !usable_fp32(saved[6], saved[1], saved[3].sizes()) ||
         (dW.defined() && dW.device() != saved[1].device())) {
+      if (!mine) dW = Tensor();
       auto out = backward_in_python(ctx, kSliced, grad, saved, {plan.need_dw, plan.flags}, &dW, 6);
       if (mine && !dW.defined()) ctx->saved_data.erase("dW");
       return out;
     }
     Tensor dvals = prepared(saved[5]), dbias = prepared(saved[6]);
+    const bool in_place = mine || !dW.defined();
     if (ctx->needs_input_grad(1)) {
       TORCH_CHECK(plan.need_dw, "the step ran without dW but weight requires a gradient");
       if (mine) ctx->saved_data.erase("dW");  // the buffer now belongs to whoever receives the gradient
@@ -449,7 +453,7 @@ struct SlicedLoss : torch::autograd::Function<SlicedLoss> {
       dW = Tensor();
     }
     const c10::DeviceGuard guard(saved[1].device());
-    auto [w, v, b] = finish(grad, saved[1], dW, dvals, saved[2].scalar_type(), dbias, saved[3].scalar_type());
+    auto [w, v, b] = finish(grad, saved[1], dW, dvals, saved[2].scalar_type(), dbias, saved[3].scalar_type(), in_place);
     return {Tensor(), w, v, b, Tensor(), Tensor()};
   }
 };

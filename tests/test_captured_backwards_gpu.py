@@ -1,5 +1,5 @@
-"""A hierarchical step whose forward runs before a graph is captured and whose backward is captured: every replay makes the gradients
-for the upstream gradient of its time."""
+"""A hierarchical step of which the forward is captured and the backward not, or the other way round, or each into a graph of its own:
+every backward makes the gradients for the upstream gradient of its time."""
 import pytest
 import torch
 
@@ -53,3 +53,43 @@ def test_a_captured_backward_of_an_eager_step(fn, dtype, monkeypatch):
         left = torch.autograd.grad(loss, leaves, up)
     torch.cuda.synchronize()
     assert all(torch.equal(a, c) for a, c in zip(left, want[0.5]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_backwards_of_a_captured_step(dtype, monkeypatch):
+    monkeypatch.setattr(ops, "_late_step", lambda *_: False)
+    inputs = [[x.to(DEV) for x in make_inputs(40, 16, 411, 256, dtype, seed=seed)] for seed in (6, 7)]
+    up = torch.tensor(2.0, device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    idx, W, v, b, t = (x.clone() for x in inputs[0])
+    leaves = [x.requires_grad_() for x in (W, v, b)]
+    want = {}
+    with torch.cuda.stream(stream):
+        for which, (i, w, a, c, y) in enumerate(inputs):
+            for value in (2.0, 0.5, 1.0):
+                up.fill_(value)
+                own = [x.clone().requires_grad_() for x in (w, a, c)]
+                want[which, value] = torch.autograd.grad(flex.triton_hierarchical_sae_loss(i, *own, y), own, up)
+        torch.cuda.synchronize()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=stream):
+        loss = flex.triton_hierarchical_sae_loss(idx, *leaves, t)
+    with torch.cuda.graph(backward, stream=stream, pool=forward.pool()):
+        got = torch.autograd.grad(loss, leaves, up, retain_graph=True)
+    for which in (0, 1, 0):
+        for to, x in zip((idx, *leaves, t), inputs[which]):
+            to.data.copy_(x)  # (the values alone: what autograd has saved is these very tensors)
+        torch.cuda.synchronize()
+        forward.replay()
+        for value in (2.0, 0.5, 1.0, 0.5):
+            up.fill_(value)
+            torch.cuda.synchronize()
+            backward.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(got, want[which, value])), (which, value)
+        with torch.cuda.stream(stream):  # (and an eager one)
+            eager = torch.autograd.grad(loss, leaves, up, retain_graph=True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(eager, want[which, 0.5]))
+    del forward, backward
